@@ -72,7 +72,8 @@ int moty_cuda_sync(int device);
  * waits for `stream` (NULL = the library's), returns 0 when no wait expired since the last check, else clears the
  * words, puts the grid-barrier counters back to zero and returns MOTY_CUDA_EKERNEL (last_error names the kernel
  * class).  It also reports a device-side position of moty_cuda_attn_core_posdev that left [0, pos_max] (the kernels
- * clamp it instead of writing past the KV cache).  The reference's kernels cannot fail (hw/hw.h:58-124 return no status); this is the GPU-side addition. */
+ * clamp it instead of writing past the KV cache), and batch arrays or page lists of the moty_cuda_kv4_* entries that
+ * were out of range.  The reference's kernels cannot fail (hw/hw.h:58-124 return no status); this is the GPU-side addition. */
 int moty_cuda_kernel_status(int device, void *stream);
 /* Diagnostic: enqueue a tiny kernel that runs the give-up path of one wait class on purpose -- the production wait
  * function on something nobody completes, with a limit well under a millisecond; it polls, gives up, sets the
@@ -444,6 +445,82 @@ int moty_cuda_attn_core_posdev(MotyCudaAttn *a, float *ctx_dev, float *q_dev, fl
 /* the last step of the gated variant (moty_nn_attention_gated, nn/attn.c:68-69): ctx[i] *= 1 / (1 + expf(-gate[i])),
  * ctx_dev and gate_dev [S][H*hd] on the handle's device */
 int moty_cuda_attn_gate_dev(MotyCudaAttn *a, float *ctx_dev, const float *gate_dev, int S, void *stream);
+
+/* ---- paged 4-bit KV cache ---------------------------------------------------
+ * For serving several sequences at once (the reference keeps one sequence per process; no counterpart there): the key
+ * and value rows of all layers in pages of 64 positions that sequences can share, 4.5 bits a value, and the attention
+ * that reads them.  Values are held as code * step: a group of 32 dims of a row shares one signed f16 step by the rule
+ * of the Q4R4 weights (nn/quant.c:157-179),
+ *     big = the first value of largest magnitude, other = the largest magnitude of the opposite sign,
+ *     step = max(|big| / 8, other / 7) in f32, d = f16(big > 0 ? -step : step), code = clamp(rint(x / d), -8, 7),
+ * d at most 65504 in magnitude, code 0 where d is 0; a group that holds an infinity or a NaN gets d = NaN.
+ * head_dim: a multiple of 32, at most 256.  A page is contiguous: moty_cuda_kv4_page_bytes = 72 * layers * kv_heads *
+ * head_dim bytes.  mem_dev: pages * page_bytes bytes of the caller's device memory (128-byte aligned; it outlives the
+ * handle, and its contents are taken as they are), or NULL: the library allocates and zeroes it. */
+typedef struct MotyCudaKv4 MotyCudaKv4;
+int64_t moty_cuda_kv4_page_bytes(int layers, int n_kv_heads, int head_dim);
+int moty_cuda_kv4_create(MotyCudaKv4 **out, int layers, int n_kv_heads, int head_dim, int pages, void *mem_dev, int device);
+int moty_cuda_kv4_free(MotyCudaKv4 *kv);
+/* Page bookkeeping on the host (no GPU work): alloc hands out n pages with one owner each, the lowest free ids in
+ * ascending order (MOTY_CUDA_ELIMIT, and nothing handed out, when fewer are free); retain adds an owner to each page of the
+ * list (sharing), release takes one away and frees a page that has none left.  -1 entries of a list are skipped; a list
+ * that names a page not in use changes nothing and fails.  compact_plan gives the moves that bring the pages in use to ids
+ * 0 .. live - 1 (src[i] -> dst[i], both ascending, *n of them) and renames them in the books: the caller then runs
+ * compact_dev with the same lists before anything else touches the pages.  More than cap moves: MOTY_CUDA_ELIMIT, *n set,
+ * nothing changed. */
+int moty_cuda_kv4_alloc(MotyCudaKv4 *kv, int n, int *ids);
+int moty_cuda_kv4_retain(MotyCudaKv4 *kv, int n, const int *ids);
+int moty_cuda_kv4_release(MotyCudaKv4 *kv, int n, const int *ids);
+int moty_cuda_kv4_free_pages(const MotyCudaKv4 *kv);
+int moty_cuda_kv4_compact_plan(MotyCudaKv4 *kv, int cap, int *src, int *dst, int *n);
+
+/* A ragged batch.  All arrays are device int32 and are read when the kernels run, so a captured graph follows them:
+ * rows row0[s] .. row0[s + 1] - 1 of the row buffers belong to sequence s and stand for the LAST positions of its len[s]
+ * (which counts them); position t lies in page table[s][t / 64].  A table entry of -1 is an absent page (freed in front
+ * of a sliding window, say): its positions are not there.  rows: height of the row buffers; rows from row0[nseq] on are
+ * neither read nor written.  max_rows / max_len: no sequence has more rows / positions (attend_dev sizes its launch by
+ * them; append and fetch do not use them).  Arrays that do not describe a batch (offsets outside the buffers, more rows
+ * than positions, a length past the table or max_len, page ids outside the pool) never move an access out of bounds: the
+ * rows concerned are skipped (attend_dev: set to 0; positions of a bad page are left out) and moty_cuda_kernel_status reports it. */
+typedef struct {
+    int nseq, rows, max_rows, max_len, table_ld;
+    const int *row0_dev, *len_dev, *table_dev;
+} MotyKv4Batch;
+/* norm and rotation in front of the store, with the meaning they have in moty_cuda_attn_create (gemma = 0) and
+ * moty_cuda_attn_create_gemma (gemma = 1: rot = rotated pairs, the gains are the multipliers, vn_dev the value norm); the gains
+ * are device arrays [head_dim] or NULL */
+typedef struct {
+    int rot, gemma;
+    float theta, eps;
+    const float *qn_dev, *kn_dev, *vn_dev;
+} MotyKv4Rope;
+/* append: rows k, v [rows][KV * hd] (row stride kv_ld values, 0 = KV * hd; a multiple of 4; 16-byte aligned) are quantised
+ * into the pages.  Pages that several sequences share must not be written: fork copies the partial one.
+ * append_rope: q [rows][H * hd] (stride q_ld) and k are first normed and rotated in place at their rows' positions (the
+ * statements of moty_cuda_attn_core_dev), then k and v stored; n_heads = 0 leaves q out.
+ * fetch: the values held for the batch's rows, k, v [rows][KV * hd] contiguous; 0 for an absent page. */
+int moty_cuda_kv4_append_dev(MotyCudaKv4 *kv, int layer, const float *k_dev, const float *v_dev, int kv_ld, const MotyKv4Batch *batch, void *stream);
+int moty_cuda_kv4_append_rope_dev(MotyCudaKv4 *kv, int layer, int n_heads, float *q_dev, int q_ld, float *k_dev, const float *v_dev, int kv_ld,
+                                  const MotyKv4Rope *rope, const MotyKv4Batch *batch, void *stream);
+int moty_cuda_kv4_fetch_dev(MotyCudaKv4 *kv, int layer, float *k_dev, float *v_dev, const MotyKv4Batch *batch, void *stream);
+/* attend: ctx [rows][H * hd] = softmax(scale * q k^T) v over positions 0 .. p of a row's own sequence (p its position),
+ * the last `window` of them when window > 0, absent pages left out; a row that sees nothing becomes 0.  Query head h reads
+ * KV head h / (n_heads / KV).  q [rows][H * hd], row stride q_ld (0 = H * hd), already rotated; scale 0 = 1/sqrt(head_dim).
+ * f32 in and out, f32 sums.  One to a few rows a sequence (decode) and whole prompts, mixed in one call; the same inputs
+ * and limits give the same bits. */
+int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_dev, const float *q_dev, int q_ld, int n_heads, int window, float scale,
+                             const MotyKv4Batch *batch, void *stream);
+/* fork: sequence dst[f] of the table [nseq][table_ld] and len [nseq] becomes a copy of sequence src[f], f = 0 .. n - 1: ids of full
+ * pages are shared (the caller retains them), a partial last page is copied, all layers, to page fresh[f] (from alloc; -1
+ * where len[src] is a multiple of 64); the rest of the row becomes -1.  A source may repeat; a target that is another
+ * fork's source or target, a fresh page given twice, or an index out of range is skipped and reported by kernel_status.
+ * compact: pages src[i] -> dst[i] for all layers, and out[j] = the new id of table[j] for count entries (ids not in src and
+ * -1 stay; out may be table).  src and dst strictly ascending and without a common id, as compact_plan gives them; moves
+ * that break this are skipped and reported. */
+int moty_cuda_kv4_fork_dev(MotyCudaKv4 *kv, int n, const int *src_dev, const int *dst_dev, const int *fresh_dev, int nseq, int *len_dev,
+                           int *table_dev, int table_ld, void *stream);
+int moty_cuda_kv4_compact_dev(MotyCudaKv4 *kv, int n, const int *src_dev, const int *dst_dev, int64_t count, const int *table_dev, int *out_dev,
+                              void *stream);
 
 /* ---- load-time quantizers (weights) -----------------------------------------
  * moty_quantize_rows (nn/quant.c:12-33) with bits = 8: w [O][I] f32 host ->

@@ -40,6 +40,7 @@ def lib() -> C.CDLL:
         _lib = C.CDLL(LIB_PATH)
         _lib.moty_cuda_last_error.restype = C.c_char_p
         _lib.moty_cuda_mat_bytes.restype = C.c_int64
+        _lib.moty_cuda_kv4_page_bytes.restype = C.c_int64
     return _lib
 
 
@@ -365,6 +366,115 @@ class Attn:
     def close(self):
         if self.h:
             lib().moty_cuda_attn_free(self.h); self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class _Kv4BatchC(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("nseq", "rows", "max_rows", "max_len", "table_ld")] + \
+               [(n, C.c_void_p) for n in ("row0_dev", "len_dev", "table_dev")]
+
+
+class _Kv4RopeC(C.Structure):
+    _fields_ = [("rot", C.c_int), ("gemma", C.c_int), ("theta", C.c_float), ("eps", C.c_float)] + \
+               [(n, C.c_void_p) for n in ("qn_dev", "kn_dev", "vn_dev")]
+
+
+class Kv4Batch:
+    """A ragged batch over a ``Kv4`` cache (device int32 arrays, read when the kernels run): rows row0[s] .. row0[s + 1] - 1
+    are the last of sequence s's len[s] positions, position t lies in page table[s][t // 64] (-1: absent)."""
+
+    def __init__(self, nseq, rows, row0_ptr, len_ptr, table_ptr, table_ld, max_rows=None, max_len=None):
+        self.c = _Kv4BatchC(nseq, rows, rows if max_rows is None else max_rows, table_ld * Kv4.PAGE if max_len is None else max_len,
+                            table_ld, row0_ptr, len_ptr, table_ptr)
+
+
+class Kv4:
+    """A paged 4-bit KV cache of all layers of a model: groups of 32 values share an f16 step (the rule of the Q4R4 weights),
+    pages of 64 positions that sequences can share.  ``mem_ptr``: device memory of pages * page_bytes(...) bytes that the
+    caller keeps alive, or 0 for the library's own."""
+
+    PAGE = 64
+
+    def __init__(self, layers, KV, hd, pages, device=0, mem_ptr=0):
+        self.layers, self.KV, self.hd, self.pages, self.device = layers, KV, hd, pages, device
+        self.h = None
+        h = C.c_void_p()
+        _ck(lib().moty_cuda_kv4_create(C.byref(h), layers, KV, hd, pages, C.c_void_p(mem_ptr), device))
+        self.h = h
+
+    @staticmethod
+    def page_bytes(layers, KV, hd) -> int:
+        n = int(lib().moty_cuda_kv4_page_bytes(layers, KV, hd))
+        if n < 0:
+            _ck(n)
+        return n
+
+    # -- page bookkeeping (host) --
+    def alloc(self, n) -> np.ndarray:
+        """n pages with one owner each: the lowest free ids, ascending."""
+        ids = np.empty(max(n, 0), np.int32)
+        _ck(lib().moty_cuda_kv4_alloc(self.h, n, _p(ids)))
+        return ids
+
+    def retain(self, ids) -> None:
+        ids = np.ascontiguousarray(ids, np.int32).ravel()
+        _ck(lib().moty_cuda_kv4_retain(self.h, ids.size, _p(ids)))
+
+    def release(self, ids) -> None:
+        ids = np.ascontiguousarray(ids, np.int32).ravel()
+        _ck(lib().moty_cuda_kv4_release(self.h, ids.size, _p(ids)))
+
+    def free_pages(self) -> int:
+        n = lib().moty_cuda_kv4_free_pages(self.h)
+        if n < 0:
+            _ck(n)
+        return n
+
+    def compact_plan(self):
+        """(src, dst): the moves that bring the pages in use to the lowest ids.  The books are renamed at once: run
+        ``compact_dev`` with these lists next."""
+        src, dst, n = np.empty(self.pages, np.int32), np.empty(self.pages, np.int32), C.c_int(0)
+        _ck(lib().moty_cuda_kv4_compact_plan(self.h, self.pages, _p(src), _p(dst), C.byref(n)))
+        return src[:n.value].copy(), dst[:n.value].copy()
+
+    # -- device entries --
+    def append_dev(self, layer, k_ptr, v_ptr, batch, stream=0, ld=0):
+        _ck(lib().moty_cuda_kv4_append_dev(self.h, layer, C.c_void_p(k_ptr), C.c_void_p(v_ptr), ld, C.byref(batch.c), C.c_void_p(stream)))
+
+    def append_rope_dev(self, layer, H, q_ptr, k_ptr, v_ptr, batch, rot, theta, eps, qn_ptr=0, kn_ptr=0, vn_ptr=0, gemma=False,
+                        stream=0, q_ld=0, kv_ld=0):
+        """Norm and rotate q and k in place at their rows' positions (as ``Attn.core_dev`` does), then store k and v."""
+        r = _Kv4RopeC(rot, 1 if gemma else 0, theta, eps, qn_ptr or None, kn_ptr or None, vn_ptr or None)
+        _ck(lib().moty_cuda_kv4_append_rope_dev(self.h, layer, H, C.c_void_p(q_ptr), q_ld, C.c_void_p(k_ptr), C.c_void_p(v_ptr), kv_ld,
+                                                C.byref(r), C.byref(batch.c), C.c_void_p(stream)))
+
+    def fetch_dev(self, layer, k_ptr, v_ptr, batch, stream=0):
+        """The values held for the batch's rows, f32 [rows][KV * hd]."""
+        _ck(lib().moty_cuda_kv4_fetch_dev(self.h, layer, C.c_void_p(k_ptr), C.c_void_p(v_ptr), C.byref(batch.c), C.c_void_p(stream)))
+
+    def attend_dev(self, layer, ctx_ptr, q_ptr, H, batch, window=0, scale=0.0, stream=0, q_ld=0):
+        """ctx [rows][H * hd] = softmax(scale q k^T) v over each row's own sequence up to its position."""
+        _ck(lib().moty_cuda_kv4_attend_dev(self.h, layer, C.c_void_p(ctx_ptr), C.c_void_p(q_ptr), q_ld, H, window, C.c_float(scale),
+                                           C.byref(batch.c), C.c_void_p(stream)))
+
+    def fork_dev(self, n, src_ptr, dst_ptr, fresh_ptr, nseq, len_ptr, table_ptr, table_ld, stream=0):
+        """Sequences dst[f] become copies of src[f]: full pages shared, a partial last page copied to fresh[f]."""
+        _ck(lib().moty_cuda_kv4_fork_dev(self.h, n, C.c_void_p(src_ptr), C.c_void_p(dst_ptr), C.c_void_p(fresh_ptr), nseq,
+                                         C.c_void_p(len_ptr), C.c_void_p(table_ptr), table_ld, C.c_void_p(stream)))
+
+    def compact_dev(self, n, src_ptr, dst_ptr, count, table_ptr, out_ptr, stream=0):
+        """Pages src[i] -> dst[i], and the table's ``count`` entries renamed into out (which may be the table)."""
+        _ck(lib().moty_cuda_kv4_compact_dev(self.h, n, C.c_void_p(src_ptr), C.c_void_p(dst_ptr), C.c_int64(count), C.c_void_p(table_ptr),
+                                            C.c_void_p(out_ptr), C.c_void_p(stream)))
+
+    def close(self):
+        if self.h:
+            lib().moty_cuda_kv4_free(self.h); self.h = None
 
     def __del__(self):
         try:

@@ -230,18 +230,19 @@ extern "C" int moty_cuda_kernel_status(int device, void *stream) {
     if (!c) return moty_set_error(MOTY_CUDA_EINIT, "device %d not initialised", device);
     MOTY_USE_DEVICE(device);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    int w[4] = {0, 0, 0, 0};
-    CK(cudaMemcpyAsync(w, c->err_dev, 16, cudaMemcpyDeviceToHost, st));
+    int w[5] = {0, 0, 0, 0, 0};
+    CK(cudaMemcpyAsync(w, c->err_dev, 20, cudaMemcpyDeviceToHost, st));
     CK(cudaStreamSynchronize(st));
-    if (!w[0] && !w[1] && !w[2] && !w[3]) return 0;
-    CK(cudaMemsetAsync(c->err_dev, 0, 16, st));
+    if (!w[0] && !w[1] && !w[2] && !w[3] && !w[4]) return 0;
+    CK(cudaMemsetAsync(c->err_dev, 0, 20, st));
     // a grid barrier that gave up leaves its arrival count and generation inconsistent: back to zero for the next launch
     if (w[1]) CK(cudaMemsetAsync(c->ctr + 4, 0, 8, st));
     CK(cudaStreamSynchronize(st));
-    return moty_set_error(MOTY_CUDA_EKERNEL, "kernel error since the last check:%s%s%s%s (results since then are incomplete or wrong)",
+    return moty_set_error(MOTY_CUDA_EKERNEL, "kernel error since the last check:%s%s%s%s%s (results since then are incomplete or wrong)",
                           w[0] ? " tensor-core GEMM pipeline wait expired;" : "", w[1] ? " grid barrier of a one-launch MoE/FFN decode kernel expired;" : "",
                           w[2] ? " bulk-copy wait of a Q4R4/Q8R4 decode kernel expired;" : "",
-                          w[3] ? " attention position on the device was outside [0, pos_max] (clamped);" : "");
+                          w[3] ? " attention position on the device was outside [0, pos_max] (clamped);" : "",
+                          w[4] ? " batch arrays or page lists of the paged 4-bit KV cache were out of range (those rows or pages were skipped);" : "");
 }
 
 extern "C" int moty_cuda_selftest_expire_wait(int device, int which, void *stream) {
