@@ -4,6 +4,7 @@
 //     s_t = scale * q . k_t,   ctx = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m)   over t in (p - window, p],
 // k_t and v_t the values held (code * step), positions of absent pages (table entry -1) left out, 0 where nothing is left.
 #include "kv4_frag.cuh"
+#include "kv4_attend.cuh"
 
 namespace {
 
@@ -17,25 +18,6 @@ namespace {
 // and exponent of the largest value step (so that weight * step fits f16); warps join in shared memory, spans through
 // `part` ({m, l, acc[hd]} per (row, head, split)) and kv4_merge_kernel.
 constexpr int DEC_W = 4;                                     // warps a CTA
-
-// what a CTA of sequence `seq` works on
-struct Kv4Seq { int r0, n, len; bool ok; };
-__device__ __forceinline__ Kv4Seq kv4_load_seq(const Kv4Attend &a, int seq) {
-    Kv4Seq q;
-    const int st = kv4_seq(a.b, seq, &q.r0, &q.n, &q.len);
-    q.ok = st == KV4_ROW_OK && q.n <= a.max_rows && q.len <= a.max_len;
-    if (st != KV4_ROW_NONE && !q.ok && threadIdx.x == 0) atomicExch(a.err, 1);
-    if (st == KV4_ROW_NONE) q.n = 0;
-    return q;
-}
-// rows of a sequence that is refused are zero (one CTA per KV head does it)
-__device__ __forceinline__ void kv4_zero_rows(const Kv4Attend &a, const Kv4Seq &q, int head) {
-    const int lo = q.r0 > 0 ? q.r0 : 0;
-    const long long hi = (long long)q.r0 + q.n < a.b.rows ? (long long)q.r0 + q.n : a.b.rows;
-    const int w = a.G * a.geo.hd;
-    for (long long r = lo; r < hi; r++)
-        for (int i = threadIdx.x; i < w; i += blockDim.x) a.ctx[r * a.H * a.geo.hd + (size_t)head * w + i] = 0.f;
-}
 
 template <int NG, int NT>
 __global__ void __launch_bounds__(DEC_W * 32) kv4_decode_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
@@ -57,13 +39,9 @@ __global__ void __launch_bounds__(DEC_W * 32) kv4_decode_kernel(Kv4Attend a, int
     if (ncol <= 0) return;
     const int pos0 = sq.len - sq.n;                          // position of the sequence's first row
     const int row_a = c0 / a.G, row_z = (c0 + ncol - 1) / a.G;
-    // the positions any column sees, and those that all of them see
-    const int lo_any = a.window > 0 && pos0 + row_a - a.window + 1 > 0 ? pos0 + row_a - a.window + 1 : 0, hi_any = pos0 + row_z + 1;
-    const int lo_all = a.window > 0 && pos0 + row_z - a.window + 1 > 0 ? pos0 + row_z - a.window + 1 : 0, hi_all = pos0 + row_a + 1;
-    const int t_lo = (lo_any & ~15) + split * span, t_hi = hi_any - t_lo < span ? hi_any : t_lo + span;
-    if (t_lo >= hi_any && nsplit > 1) {                      // nothing in this span: the merge does not look at it
-        return;
-    }
+    const Kv4Range cr = kv4_range(a, pos0 + row_a, pos0 + row_z);
+    const int t_lo = (cr.lo_any & ~15) + split * span, t_hi = cr.hi_any - t_lo < span ? cr.hi_any : t_lo + span;
+    if (t_lo >= cr.hi_any && nsplit > 1) return;             // nothing in this span: the merge does not look at it
     // query rows, then their two pieces as operands: column 2 c + piece, k = the dims of a word's nibble pairs
     for (int c = warp; c < NC; c += DEC_W) {
         float am = 0.f, x[NG];
@@ -149,7 +127,7 @@ __global__ void __launch_bounds__(DEC_W * 32) kv4_decode_kernel(Kv4Attend a, int
                 s[nt][1] = fmaf(db, c[2] + c[3], s[nt][1]);
             }
         }
-        const bool inside = t0 >= lo_all && t0 + 15 < hi_all;      // (columns past ncol hold zero rows, and are not written)
+        const bool inside = t0 >= cr.lo_all && t0 + 15 < cr.hi_all;      // (columns past ncol hold zero rows, and are not written)
         bool up = false;
         bool see[NT][2];
 #pragma unroll
@@ -173,6 +151,10 @@ __global__ void __launch_bounds__(DEC_W * 32) kv4_decode_kernel(Kv4Attend a, int
 #pragma unroll
                     for (int i = 0; i < 8; i++) acc[nt][g][i >> 2][i & 3] *= f;
             }
+        }
+        if (!inside) {
+            kv4_mask_steps<NG>(wa, t0 + 2 * j, cr.lo_any, cr.hi_any);
+            kv4_mask_steps<NG>(wb, t0 + 8 + 2 * j, cr.lo_any, cr.hi_any);
         }
         // the largest value step (NaN left aside) decides the power of two that weight * step is scaled by
         {
@@ -256,15 +238,15 @@ __global__ void __launch_bounds__(DEC_W * 32) kv4_decode_kernel(Kv4Attend a, int
         const size_t rh = (size_t)(sq.r0 + cc / a.G) * a.H + head * a.G + cc % a.G;
         if (nsplit == 1) a.ctx[rh * HD + d] = L == 0.f ? 0.f : __fdiv_rn(o, L);
         else {
-            float *p = part + (rh * nsplit + split) * (HD + 2);
-            p[2 + d] = o;
+            float *p = part + (rh * nsplit + split) * (HD + 4);
+            p[4 + d] = o;
             if (d == 0) { p[0] = M; p[1] = L; }
         }
     }
 }
 
 // joins the spans of one (row, head): the same sums over {m, l, acc} with the maximum over all spans
-__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attend a, int nsplit, int span, int ncols, const float *part) {
+__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
     const int row = blockIdx.x, h = blockIdx.y, hd = a.geo.hd, d = threadIdx.x;
     pdl_trigger();
     pdl_wait();
@@ -275,87 +257,41 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attend a, int nsplit,
     const int n = st == KV4_ROW_OK ? a.b.row0[seq + 1] - a.b.row0[seq] : 0;
     if (st == KV4_ROW_BAD || n > a.max_rows || a.b.len[seq] > a.max_len) { *out = 0.f; return; }
     // the spans that hold anything for this row's column tile
-    const int c = (row - a.b.row0[seq]) * a.G + h % a.G, c0 = c / ncols * ncols, cz = c0 + ncols - 1 < n * a.G - 1 ? c0 + ncols - 1 : n * a.G - 1;
-    const int pos0 = a.b.len[seq] - n, first = pos0 + c0 / a.G - a.window + 1, hi = pos0 + cz / a.G + 1;
-    const int lo = a.window > 0 && first > 0 ? first & ~15 : 0;
-    int live = (hi - lo + span - 1) / span;
-    if (live > nsplit) live = nsplit;
-    const float *p = part + ((size_t)row * a.H + h) * nsplit * (hd + 2);
+    const long long c = (long long)(row - a.b.row0[seq]) * a.G + h % a.G, c0 = c / pl.cols * pl.cols, last = (long long)n * a.G - 1;
+    const long long cz = c0 + pl.cols - 1 < last ? c0 + pl.cols - 1 : last;
+    const int pos0 = a.b.len[seq] - n;
+    const Kv4Range cr = kv4_range(a, pos0 + (int)(c0 / a.G), pos0 + (int)(cz / a.G));
+    int live = (cr.hi_any - (cr.lo_any & ~(pl.align - 1)) + pl.span - 1) / pl.span;
+    if (live > pl.nsplit) live = pl.nsplit;
+    const float *p = part + ((size_t)row * a.H + h) * pl.nsplit * (hd + 4);
     float M = -INFINITY, L = 0.f, o = 0.f;
-    for (int i = 0; i < live; i++) M = fmaxf(M, p[(size_t)i * (hd + 2)]);
+    for (int i = 0; i < live; i++) M = fmaxf(M, p[(size_t)i * (hd + 4)]);
     for (int i = 0; i < live; i++) {
-        const float li = p[(size_t)i * (hd + 2) + 1], f = li == 0.f ? 0.f : kv4_exp2(p[(size_t)i * (hd + 2)] - M);
+        const float li = p[(size_t)i * (hd + 4) + 1], f = li == 0.f ? 0.f : kv4_exp2(p[(size_t)i * (hd + 4)] - M);
         L = fmaf(li, f, L);
-        o = fmaf(li == 0.f ? 0.f : p[(size_t)i * (hd + 2) + 2 + d], f, o);
+        o = fmaf(li == 0.f ? 0.f : p[(size_t)i * (hd + 4) + 4 + d], f, o);
     }
     *out = L == 0.f ? 0.f : __fdiv_rn(o, L);
-}
-
-
-// ---- many rows ---------------------------------------------------------------------------------------------------------
-// One warp per (row, query head), lane = dim of a group; one pass with the running maximum and sum.
-__global__ void __launch_bounds__(128) kv4_attend_simple_kernel(Kv4Attend a) {
-    const int lane = threadIdx.x & 31, hd = a.geo.hd, NG = hd >> 5;
-    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    pdl_trigger();
-    pdl_wait();
-    if (w >= (long long)a.b.rows * a.H) return;
-    const int r = (int)(w / a.H), h = (int)(w % a.H);
-    int seq, pos;
-    const int st = kv4_row(a.b, r, &seq, &pos);
-    if (st == KV4_ROW_NONE) return;
-    float acc[8], q[8], m = -INFINITY, l = 0.f;
-    for (int g = 0; g < 8; g++) { acc[g] = 0.f; q[g] = 0.f; }
-    int n = 0;
-    if (st == KV4_ROW_BAD || a.b.len[seq] > a.max_len || a.b.row0[seq + 1] - a.b.row0[seq] > a.max_rows) {
-        if (lane == 0) atomicExch(a.err, 1);
-    } else {
-        n = pos + 1;
-        for (int g = 0; g < 8; g++) if (g < NG) q[g] = a.q[(size_t)r * a.q_ld + (size_t)h * hd + g * 32 + lane];
-    }
-    for (int t = a.window > 0 && n > a.window ? n - a.window : 0; t < n; t++) {
-        const int page = a.b.table[(size_t)seq * a.b.ld + t / KV4_PAGE];
-        if (!kv4_page_ok(a.geo, page)) { if (page != -1 && lane == 0) atomicExch(a.err, 1); continue; }
-        const uint8_t *u = a.mem + kv4_unit_off(a.geo, page, a.layer, h / a.G);
-        const int tt = t % KV4_PAGE;
-        float s = 0.f;
-        for (int g = 0; g < 8; g++)
-            if (g < NG) {
-                const unsigned kw = *reinterpret_cast<const unsigned *>(u + kv4_k_word(hd, tt, g, lane >> 3));
-                const float d = f16bits_to_f32(reinterpret_cast<const uint16_t *>(u + kv4_k_step_off(hd))[tt * NG + g]);
-                s = fmaf(q[g], (float)((int)((kw >> (4 * (lane & 7))) & 15u) - 8) * d, s);
-            }
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s *= a.scale;
-        const float mn = fmaxf(m, s), f = mn == -INFINITY ? 1.f : expf(m - mn), e = mn == -INFINITY ? s : expf(s - mn);
-        m = mn; l = fmaf(l, f, e);
-        for (int g = 0; g < 8; g++)
-            if (g < NG) {
-                const unsigned vw = *reinterpret_cast<const unsigned short *>(u + kv4_v_piece(hd, tt, g, lane >> 2));
-                const float d = f16bits_to_f32(reinterpret_cast<const uint16_t *>(u + kv4_v_step_off(hd))[tt * NG + g]);
-                acc[g] = fmaf(acc[g], f, e * ((float)((int)((vw >> (4 * (lane & 3))) & 15u) - 8) * d));
-            }
-    }
-    for (int g = 0; g < 8; g++)
-        if (g < NG) a.ctx[((size_t)r * a.H + h) * hd + g * 32 + lane] = l == 0.f ? 0.f : acc[g] / l;
 }
 
 }  // namespace
 
 // how a call is cut
-struct Kv4Plan { bool decode; int nt, ntile, nsplit, span; };
 static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     Kv4Plan p{};
     const long long cols = (long long)a.max_rows * a.G;
     p.decode = cols <= 32;
     p.nt = cols > 4 && a.geo.hd <= 128 ? 2 : 1;
-    p.ntile = (int)((cols + 4 * p.nt - 1) / (4 * p.nt));
+    p.cols = p.decode ? 4 * p.nt : KV4_LINES;
+    p.align = p.decode ? 16 : KV4_PAGE;
+    p.ntile = (int)((cols + p.cols - 1) / p.cols);
     if (p.ntile < 1) p.ntile = 1;
-    // the longest stretch of positions a CTA's columns see together, from a multiple of 16 on
+    // the longest stretch of positions a CTA's columns see together, from a multiple of `align` on
     long long range = a.max_len;
-    if (a.window > 0 && (long long)a.window + a.max_rows + 15 < range) range = (long long)a.window + a.max_rows + 15;
+    const long long rows_a_tile = p.cols / a.G + 2 < a.max_rows ? p.cols / a.G + 2 : a.max_rows;
+    if (a.window > 0 && (long long)a.window + rows_a_tile + p.align < range) range = (long long)a.window + rows_a_tile + p.align;
     const long long units = (long long)a.b.nseq * a.geo.KV * p.ntile, most = (range + 63) / 64;
-    long long n = (6LL * sms + units - 1) / units;
+    long long n = p.decode ? (6LL * sms + units - 1) / units : units < 2LL * sms ? (3LL * sms + units - 1) / units : 1;
     if (n > most) n = most;
     if (n < 1) n = 1;
     long long span = (range + n - 1) / n;
@@ -369,7 +305,7 @@ static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
 
 size_t kv4_attend_scratch_bytes(const Kv4Attend &a, int sms) {
     const Kv4Plan p = kv4_plan(a, sms);
-    return p.decode && p.nsplit > 1 ? (size_t)a.b.rows * a.H * p.nsplit * (a.geo.hd + 2) * 4 : 0;
+    return p.nsplit > 1 ? (size_t)a.b.rows * a.H * p.nsplit * (a.geo.hd + 4) * 4 : 0;
 }
 
 template <int NG, int NT>
@@ -384,15 +320,10 @@ static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, cuda
 
 int launch_kv4_attend(const Kv4Attend &a, float *part, int sms, cudaStream_t st) {
     const Kv4Plan p = kv4_plan(a, sms);
-    if (!p.decode) {
-        const long long warps = (long long)a.b.rows * a.H;
-        if ((warps + 3) / 4 > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend: %d rows of %d heads", a.b.rows, a.H);
-        CK(moty_launch_pdl(kv4_attend_simple_kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), (size_t)0, st, a));
-        return 0;
-    }
     if (p.nsplit > 1 && !part) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: scratch for %d spans missing", p.nsplit);
     int rc = 0;
-    switch (a.geo.hd / 32) {
+    if (!p.decode) rc = launch_kv4_prompt(a, p, part, st);
+    else switch (a.geo.hd / 32) {
         case 1: rc = p.nt == 2 ? kv4_decode_go<1, 2>(a, p, part, st) : kv4_decode_go<1, 1>(a, p, part, st); break;
         case 2: rc = p.nt == 2 ? kv4_decode_go<2, 2>(a, p, part, st) : kv4_decode_go<2, 1>(a, p, part, st); break;
         case 3: rc = p.nt == 2 ? kv4_decode_go<3, 2>(a, p, part, st) : kv4_decode_go<3, 1>(a, p, part, st); break;
@@ -404,6 +335,6 @@ int launch_kv4_attend(const Kv4Attend &a, float *part, int sms, cudaStream_t st)
     }
     CKR(rc);
     if (p.nsplit > 1)
-        CK(moty_launch_pdl(kv4_merge_kernel, dim3(a.b.rows, a.H), dim3(a.geo.hd), (size_t)0, st, a, p.nsplit, p.span, p.nt * 4, (const float *)part));
+        CK(moty_launch_pdl(kv4_merge_kernel, dim3(a.b.rows, a.H), dim3(a.geo.hd), (size_t)0, st, a, p, (const float *)part));
     return 0;
 }

@@ -61,6 +61,18 @@ __device__ __forceinline__ float kv4_half_of(unsigned w, int hi) {
     return __half2float(__ushort_as_half((unsigned short)(hi ? w >> 16 : w & 0xffffu)));
 }
 
+// steps of positions t and t + 1, NG each, two to a word: those outside [lo, hi) become 0 (a page's memory behind the last
+// position may hold anything)
+template <int NG>
+__device__ __forceinline__ void kv4_mask_steps(unsigned (&w)[NG], int t, int lo, int hi) {
+    const bool s0 = t >= lo && t < hi, s1 = t + 1 >= lo && t + 1 < hi;
+#pragma unroll
+    for (int i = 0; i < NG; i++) {
+        const unsigned a = 2 * i < NG ? (s0 ? 0xffffu : 0u) : (s1 ? 0xffffu : 0u), b = 2 * i + 1 < NG ? (s0 ? 0xffff0000u : 0u) : (s1 ? 0xffff0000u : 0u);
+        w[i] &= a | b;
+    }
+}
+
 // nibbles i and i + 4 of a word as f16 pairs of code values (n - 8): 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n
 __device__ __forceinline__ void kv4_codes(unsigned w, unsigned (&e)[4]) {
     constexpr unsigned M0 = 0x000f000fu, M1 = 0x00f000f0u, C = 0x64006400u;

@@ -685,3 +685,19 @@ def test_captured_steps_follow_the_batch_arrays(gpu, t):
     finally:
         gpu._ck(gpu.lib().moty_cuda_scratch_freeze(0, 0))
     p.status()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 70])
+def test_attend_over_memory_that_holds_anything(gpu, t, rows):
+    """The caller's memory is not zero: what lies behind the last position (infinite and NaN steps among it) has no effect."""
+    H, KV, hd, L = 8, 2, 64, 150
+    mem = t.full((5, gpu.Kv4.page_bytes(1, KV, hd)), 0xff, device="cuda", dtype=t.uint8)
+    mem.view(t.int16)[1:] = 0x7c00
+    p = Pool(gpu, t, KV, hd, [L], seed=13, pages=5)
+    p.kv.close()
+    p.kv = gpu.Kv4(1, KV, hd, 5, mem_ptr=mem.data_ptr())
+    p.store()
+    q = p.rng.standard_normal((rows, H, hd)).astype(np.float32)
+    got = p.attend(q, H, [rows])
+    want, tol = attend64(quant(p.k[0])[0], quant(p.v[0])[0], q, np.arange(L - rows, L), H // KV)
+    check(got, want, tol)
