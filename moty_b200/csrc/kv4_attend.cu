@@ -5,26 +5,44 @@
 // k_t and v_t the values held (code * step), positions of absent pages (table entry -1) left out, 0 where nothing is left.
 #include "kv4_frag.cuh"
 #include "kv4_attend.cuh"
+#include <type_traits>
 
 namespace {
 
 // ---- few rows a sequence (decode) ------------------------------------------------------------------------------------
-// A CTA takes one KV head of one sequence, up to 4 NT (row, query head) pairs of it ("columns"), and a span of positions;
-// its warps walk the span 16 positions at a time, straight from global memory into matrix operands:
-//     scores  [16 positions x 2 columns a pair] = codes [16 x 32] (a group) * q pieces, times the position's step, group by group
-//     output  [32 dims x 2 columns a pair]     += codes [dims x 16 positions] * (weight * value step) pieces
-// The two columns of a pair are the hi and lo piece of its f32 operand and land in the same thread, which adds them.  Every
-// warp keeps its own running maximum (moved only when a score passes it by 8 in base-2 units, so weights stay below 256)
-// and exponent of the largest value step (so that weight * step fits f16); warps join in shared memory, spans through
-// `part` ({m, l, acc[hd]} per (row, head, split)) and kv4_merge_kernel.
-constexpr int DEC_W = 4;                                     // warps a CTA
+// A CTA takes one KV head of one sequence, up to 4 or 8 (row, query head) pairs of it ("columns"), and a span of pages.
+// Warp w owns positions 16 w .. 16 w + 15 of every page of the span: it brings their codes and steps to its own ring in
+// shared memory (DEC_ST pages deep, 16-byte asynchronous copies, no barrier beyond the warp) and multiplies
+//     scores  [16 positions x columns] = codes [16 x 32] (a group) * q pieces, times the position's step, group by group
+//     output  [32 dims x columns]     += codes [dims x 16 positions] * (weight * value step) pieces
+// PAIR (up to four columns): hi and lo piece of a column are neighbouring columns of one product and land in the same
+// thread, which adds them.  Otherwise eight columns, and hi and lo are two products into the same sums: the same matrix
+// work a column, half the piece arithmetic.  Every warp keeps its own running maximum (moved only when a score passes it by
+// 8 in base-2 units, so weights stay below 256) and exponent of the largest value step (so that weight * step fits f16:
+// a value 2^9 times smaller than the largest of its 16 positions still has all 22 bits).  Warps join in shared memory, spans
+// through `part` ({m, l, acc[hd]} per (row, head, split)) and kv4_merge_kernel.
+constexpr int DEC_W = 4, DEC_ST = 4, DEC_NP = 256;           // warps a CTA, ring depth in pages, the most pages of a span
 
-template <int NG, int NT>
-__global__ void __launch_bounds__(DEC_W * 32) kv4_decode_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
-    constexpr int HD = NG * 32, NC = NT * 4;                 // columns (pairs) of the CTA
-    extern __shared__ float sm_kv4[];
-    float *qs = sm_kv4;                                      // [NC][HD] the query rows; later acc[DEC_W][NC][HD]
-    float *ml = sm_kv4 + DEC_W * NC * HD;                    // m, l [DEC_W][NC], then descale [NC]
+// CTAs an SM holds (registers)
+constexpr int kv4_decode_ctas(int NG, bool pair) { return NG <= 2 ? 4 : NG <= 4 ? (pair ? 4 : 3) : NG <= 6 ? (pair ? 3 : 2) : 2; }
+template <int NG, bool PAIR> struct DecL {
+    static constexpr int HD = NG * 32, NC = PAIR ? 4 : 8, STAGE = 18 * HD;       // bytes of 16 positions: codes 2 x 8 HD, steps 2 x HD
+    static constexpr int CTAS = kv4_decode_ctas(NG, PAIR);
+    static constexpr int RING = DEC_W * DEC_ST * STAGE, JOIN = DEC_W * NC * HD * 4;
+    static constexpr int BODY = RING > JOIN ? RING : JOIN;
+    static constexpr int SMEM = BODY + NC * HD * 4 + (2 * DEC_W * NC + 4 * NC + DEC_NP) * 4;
+};
+
+template <int NG, bool PAIR>
+__global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
+    using Lay = DecL<NG, PAIR>;
+    constexpr int HD = NG * 32, NC = Lay::NC, UNIT = 72 * HD, STAGE = Lay::STAGE, NS = PAIR ? 1 : 2, NCP = (36 * NG + 31) / 32;
+    extern __shared__ __align__(128) uint8_t sm_kv4[];
+    float *js = reinterpret_cast<float *>(sm_kv4);           // the ring, then acc[DEC_W][NC][HD]
+    float *qs = reinterpret_cast<float *>(sm_kv4 + Lay::BODY);   // the query rows [NC][HD]
+    float *ml = qs + NC * HD;                                // m, then factor, [DEC_W][NC]; l [DEC_W][NC]; descale [NC]
+    int *col = reinterpret_cast<int *>(ml + 2 * DEC_W * NC + NC);   // row of a column, its query head, its position [NC] each
+    int *list = col + 3 * NC;                                // page ids of the span, -1: not there
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, j = lane & 3;
     const int split = blockIdx.x % nsplit;
     const int u = blockIdx.x / nsplit, tile = u % ntile, head = (u / ntile) % a.geo.KV, seq = u / ntile / a.geo.KV;
@@ -40,265 +58,463 @@ __global__ void __launch_bounds__(DEC_W * 32) kv4_decode_kernel(Kv4Attend a, int
     const int pos0 = sq.len - sq.n;                          // position of the sequence's first row
     const int row_a = c0 / a.G, row_z = (c0 + ncol - 1) / a.G;
     const Kv4Range cr = kv4_range(a, pos0 + row_a, pos0 + row_z);
-    const int t_lo = (cr.lo_any & ~15) + split * span, t_hi = cr.hi_any - t_lo < span ? cr.hi_any : t_lo + span;
+    const int t_lo = (cr.lo_any & ~(KV4_PAGE - 1)) + split * span, t_hi = cr.hi_any - t_lo < span ? cr.hi_any : t_lo + span;
     if (t_lo >= cr.hi_any && nsplit > 1) return;             // nothing in this span: the merge does not look at it
-    // query rows, then their two pieces as operands: column 2 c + piece, k = the dims of a word's nibble pairs
-    for (int c = warp; c < NC; c += DEC_W) {
-        float am = 0.f, x[NG];
-        unsigned mb = 0;
-        const int cc = c0 + c;
-        if (c < ncol) {
-            const float *src = a.q + (size_t)(sq.r0 + cc / a.G) * a.q_ld + (size_t)(head * a.G + cc % a.G) * HD;
-#pragma unroll
-            for (int g = 0; g < NG; g++) { x[g] = src[g * 32 + lane]; const unsigned b = __float_as_uint(fabsf(x[g])); mb = b > mb ? b : mb; }
-        } else {
-#pragma unroll
-            for (int g = 0; g < NG; g++) x[g] = 0.f;
-        }
-        for (int off = 16; off > 0; off >>= 1) { const unsigned o = __shfl_xor_sync(0xffffffffu, mb, off); mb = o > mb ? o : mb; }
-        am = __uint_as_float(mb);
-        // |q| 2^k < 2^14; a row that is not finite has NaN scores
-        const bool fin = mb < 0x7f800000u;
-        const int k = fin && am > 0.f ? 13 - ilogbf(am) : 0;
-#pragma unroll
-        for (int g = 0; g < NG; g++) qs[c * HD + g * 32 + lane] = fin ? scalbnf(x[g], k) : 0.f;
-        if (lane == 0) ml[2 * DEC_W * NC + c] = fin ? (float)ldexp((double)a.scale * 1.4426950408889634, -k) : __int_as_float(0x7fffffff);
+    const int np = t_hi > t_lo ? (t_hi - t_lo + KV4_PAGE - 1) / KV4_PAGE : 0;
+    const int *tab = a.b.table + (size_t)seq * a.b.ld + t_lo / KV4_PAGE;
+    for (int i = tid; i < np; i += DEC_W * 32) {
+        const int id = tab[i];
+        const bool ok = kv4_page_ok(a.geo, id);
+        if (!ok && id != -1) atomicExch(a.err, 1);
+        list[i] = ok ? id : -1;
+    }
+    if (tid < NC) {
+        const int cc = c0 + tid, row = cc / a.G;
+        col[tid] = sq.r0 + row; col[NC + tid] = head * a.G + cc - row * a.G; col[2 * NC + tid] = tid < ncol ? pos0 + row : -1;
     }
     __syncthreads();
-    unsigned qf[NT][NG][4];
-    float desc[NT];
-    int clo[NT], chi[NT];
-    const float sel = (r & 1) ? 1.f : 0.f;                   // operand column r: pair r / 2, piece r & 1
+    // this lane's 16-byte pieces of a stage: [K codes | V codes | K steps | V steps] of positions 16 warp ..
+    uint8_t *ring = sm_kv4 + warp * (DEC_ST * STAGE);
+    const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
+    // chunk c = lane + 32 i of a stage; a round of 32 that lies within one part has the same offset to `mine` in every lane
+    const uint8_t *mine = base + warp * (8 * HD) + lane * 16;
+    constexpr int KC = 16 * NG;                              // chunks of one part's codes
+    int off[NCP];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const float *qc = qs + (nt * 4 + (r >> 1)) * HD;
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) qf[nt][g][i] = kv4_piece(qc[g * 32 + 8 * j + i], qc[g * 32 + 8 * j + i + 4], sel);
-        const int cc = c0 + nt * 4 + j;                      // the pair whose scores this thread holds
-        desc[nt] = ml[2 * DEC_W * NC + nt * 4 + j];
-        const int p = pos0 + cc / a.G;
-        chi[nt] = nt * 4 + j < ncol ? p : -1;
-        clo[nt] = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+    for (int i = 0; i < NCP; i++) {
+        const int c = lane + 32 * i;
+        const int o = c < KC ? warp * (8 * HD) + c * 16
+                    : c < 2 * KC ? kv4_v_code_off(HD) + warp * (8 * HD) + (c - KC) * 16
+                    : c < 34 * NG ? kv4_k_step_off(HD) + warp * HD + (c - 32 * NG) * 16
+                                  : kv4_v_step_off(HD) + warp * HD + (c - 34 * NG) * 16;
+        off[i] = o - warp * (8 * HD) - lane * 16;
+        if (32 * i + 31 < KC) off[i] = 512 * i;
+        else if (32 * i >= KC && 32 * i + 31 < 2 * KC) off[i] = kv4_v_code_off(HD) + 512 * i - KC * 16;
     }
-    __syncthreads();                                         // qs is reused for the join
-    float m[NT], l[NT], acc[NT][NG][2][4];
-    int ve = -24;                                            // exponent of the largest value step so far
+    const bool last = lane + 32 * (NCP - 1) < 36 * NG;       // the lane has a chunk in the last round
+    const unsigned page_bytes = (unsigned)kv4_page_bytes(a.geo);     // (65535 units of 18 KB at most)
+    auto issue = [&](int i, int slot) {                      // page i of the span to ring slot `slot`
+        if (i < np) {
+            const int id = list[i];
+            if (id >= 0) {
+                const uint8_t *src = mine + (size_t)(unsigned)id * page_bytes;
+                uint8_t *dst = ring + slot * STAGE + lane * 16;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY; l[nt] = 0.f;
+                for (int k = 0; k < NCP; k++)
+                    if (k < NCP - 1 || last) cp_async16(dst + k * 512, src + off[k]);
+            }
+        }
+        cp_async_commit();
+    };
 #pragma unroll
-        for (int g = 0; g < NG; g++)
+    for (int i = 0; i < DEC_ST - 1; i++) issue(i, i);
+    // query rows, scaled by a power of two so that |q| 2^k < 2^14; a row that is not finite has NaN scores
+    for (int c = warp; c < NC; c += DEC_W) {
+        float x[NG];
+        unsigned mb = 0;
+        const float *src = a.q + (size_t)col[c] * a.q_ld + (size_t)col[NC + c] * HD;
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc[nt][g][i >> 2][i & 3] = 0.f;
+        for (int g = 0; g < NG; g++) x[g] = c < ncol ? src[g * 32 + lane] : 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; g++) mb = max(mb, __float_as_uint(fabsf(x[g])));
+        mb = __reduce_max_sync(0xffffffffu, mb);
+        const bool fin = mb < 0x7f800000u;
+        const int k = fin ? kv4_q_shift(mb) : 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++) qs[c * HD + g * 32 + lane] = fin ? kv4_scale2(x[g], k) : 0.f;
+        if (lane == 0) ml[2 * DEC_W * NC + c] = fin ? kv4_scale2(a.scale * 1.44269504f, -k) : __int_as_float(0x7fffffff);
     }
-    const int *tab = a.b.table + (size_t)seq * a.b.ld;
-    for (int t0 = t_lo + warp * 16; t0 < t_hi; t0 += DEC_W * 16) {
-        const int page = tab[t0 / KV4_PAGE];
-        if (!kv4_page_ok(a.geo, page)) { if (page != -1 && lane == 0) atomicExch(a.err, 1); continue; }
-        const uint8_t *unit = a.mem + kv4_unit_off(a.geo, page, a.layer, head);
-        const int tp = t0 % KV4_PAGE;                        // 16 positions of one block
-        unsigned ka[NG], kb[NG], va[NG], vb[NG], sa[(NG + 1) / 2], sb[(NG + 1) / 2], wa[NG], wb[NG];
-        kv4_ldw<NG>(ka, unit + (tp + r) * (HD / 2) + j * (4 * NG));
-        kv4_ldw<NG>(kb, unit + (tp + r + 8) * (HD / 2) + j * (4 * NG));
-        kv4_ldsteps<NG>(sa, unit + kv4_k_step_off(HD) + (tp + r) * (2 * NG));
-        kv4_ldsteps<NG>(sb, unit + kv4_k_step_off(HD) + (tp + r + 8) * (2 * NG));
-        kv4_ldw<NG>(va, unit + kv4_v_code_off(HD) + (tp >> 4) * (8 * HD) + lane * (4 * NG));
-        kv4_ldw<NG>(vb, unit + kv4_v_code_off(HD) + (tp >> 4) * (8 * HD) + 4 * HD + lane * (4 * NG));
-        kv4_ldw<NG>(wa, unit + kv4_v_step_off(HD) + (tp + 2 * j) * (2 * NG));
-        kv4_ldw<NG>(wb, unit + kv4_v_step_off(HD) + (tp + 8 + 2 * j) * (2 * NG));
-        // scores of positions t0 + r and t0 + r + 8 for the thread's pairs
-        float s[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = 0.f;
+    __syncthreads();
+    // operand column r: PAIR: pair r / 2, piece r & 1; else column r, both pieces
+    unsigned qf[NS][NG][4];
+    const unsigned short sel = (r & 1) ? KV4_HM1 : KV4_H0;
+    {
+        const float *qc = qs + (PAIR ? r >> 1 : r) * HD;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            unsigned ea[4], eb[4];
-            kv4_codes(ka[g], ea);
-            kv4_codes(kb[g], eb);
-            const float da = kv4_half_of(sa[g >> 1], g & 1), db = kv4_half_of(sb[g >> 1], g & 1);
+            const float4 x = *reinterpret_cast<const float4 *>(qc + g * 32 + 8 * j), z = *reinterpret_cast<const float4 *>(qc + g * 32 + 8 * j + 4);
+            const float xs[4] = {x.x, x.y, x.z, x.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                kv4_mma(c, ea[0], eb[0], ea[1], eb[1], qf[nt][g][0], qf[nt][g][1]);
-                kv4_mma(c, ea[2], eb[2], ea[3], eb[3], qf[nt][g][2], qf[nt][g][3]);
-                s[nt][0] = fmaf(da, c[0] + c[1], s[nt][0]);
-                s[nt][1] = fmaf(db, c[2] + c[3], s[nt][1]);
+            for (int i = 0; i < 4; i++) {
+                if (PAIR) qf[0][g][i] = kv4_piece(xs[i], zs[i], sel);
+                else kv4_pieces(xs[i], zs[i], qf[0][g][i], qf[NS - 1][g][i]);
             }
         }
-        const bool inside = t0 >= cr.lo_all && t0 + 15 < cr.hi_all;      // (columns past ncol hold zero rows, and are not written)
-        bool up = false;
-        bool see[NT][2];
+    }
+    // the columns whose scores this thread holds: PAIR: j; else 2 j and 2 j + 1
+    float desc[NS];
+    int clo[NS], chi[NS];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            s[nt][0] *= desc[nt]; s[nt][1] *= desc[nt];
-            see[nt][0] = inside || (t0 + r >= clo[nt] && t0 + r <= chi[nt]);
-            see[nt][1] = inside || (t0 + r + 8 >= clo[nt] && t0 + r + 8 <= chi[nt]);
-            if (!see[nt][0]) s[nt][0] = -INFINITY;
-            if (!see[nt][1]) s[nt][1] = -INFINITY;
-            up |= fmaxf(s[nt][0], s[nt][1]) > m[nt] + 8.f;
-        }
-        if (__any_sync(0xffffffffu, up)) {
+    for (int k = 0; k < NS; k++) {
+        const int c = PAIR ? j : 2 * j + k, p = col[2 * NC + c];
+        desc[k] = ml[2 * DEC_W * NC + c];
+        chi[k] = p;
+        clo[k] = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+    }
+    const int phi = col[2 * NC + (PAIR ? r >> 1 : r)], plo = a.window > 0 ? phi - a.window + 1 : 0;      // limits of operand column r
+    float m[NS], l[NS], acc[NG][2][4];
+    float vth = 0.f, vn = 1.f, vl = 0.f;                     // 2^(e + 1), 64 * 2^-e and its base-2 log, for the exponent e of the largest value step so far
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float mx = fmaxf(s[nt][0], s[nt][1]);
-                for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                const float mn = fmaxf(m[nt], mx), f = mn == -INFINITY ? 1.f : kv4_exp2(m[nt] - mn);
-                m[nt] = mn; l[nt] *= f;
+    for (int k = 0; k < NS; k++) { m[k] = -INFINITY; l[k] = 0.f; }   // m: the running maximum less vl; l and acc: sums of weights times vn
 #pragma unroll
-                for (int g = 0; g < NG; g++)
+    for (int g = 0; g < NG; g++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) acc[nt][g][i >> 2][i & 3] *= f;
+        for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] = 0.f;
+    for (int it = 0, slot = 0; it < np; it++) {
+        cp_async_wait<DEC_ST - 2>();
+        __syncwarp();                                        // everyone's pieces of page `it` are here, and page it - 1 is done with
+        issue(it + DEC_ST - 1, slot ? slot - 1 : DEC_ST - 1);
+        const uint8_t *sg = ring + slot * STAGE;
+        slot = slot == DEC_ST - 1 ? 0 : slot + 1;
+        const int t0 = t_lo + it * KV4_PAGE + warp * 16;
+        if (list[it] < 0 || t0 >= cr.hi_any || t0 + 16 <= cr.lo_any) continue;
+        // two copies of the body: every position seen by every column, or limits to look at (columns past ncol hold zero
+        // rows, and are not written)
+        auto body = [&](auto in) {
+        constexpr bool inside = decltype(in)::value;
+        // scores of positions t0 + r and t0 + r + 8
+        float s[NS][2];
+#pragma unroll
+        for (int k = 0; k < NS; k++) s[k][0] = s[k][1] = 0.f;
+        {
+            unsigned ka[NG], kb[NG], sa[(NG + 1) / 2], sb[(NG + 1) / 2];
+            kv4_ldsw<NG>(ka, sg + r * (HD / 2) + j * (4 * NG));
+            kv4_ldsw<NG>(kb, sg + (r + 8) * (HD / 2) + j * (4 * NG));
+            kv4_ldsteps<NG>(sa, sg + 16 * HD + r * (2 * NG));
+            kv4_ldsteps<NG>(sb, sg + 16 * HD + (r + 8) * (2 * NG));
+            // the groups' products are independent of one another: their chains are written side by side
+            constexpr int GB = NG <= 4 ? NG : NG % 4 == 0 ? 4 : NG % 3 == 0 ? 3 : NG == 5 ? 5 : 7;
+#pragma unroll
+            for (int g0 = 0; g0 < NG; g0 += GB) {
+                unsigned ea[GB][4], eb[GB][4];
+                float c[GB][4];
+#pragma unroll
+                for (int g = 0; g < GB; g++) {
+                    kv4_codes(ka[g0 + g], ea[g]);
+                    kv4_codes(kb[g0 + g], eb[g]);
+                }
+#pragma unroll
+                for (int pc = NS - 1; pc >= 0; pc--)
+#pragma unroll
+                    for (int st = 0; st < 2; st++)
+#pragma unroll
+                        for (int g = 0; g < GB; g++)
+                            if (pc == NS - 1 && st == 0)
+                                kv4_mma0(c[g], ea[g][0], eb[g][0], ea[g][1], eb[g][1], qf[pc][g0 + g][0], qf[pc][g0 + g][1]);
+                            else kv4_mma(c[g], ea[g][2 * st], eb[g][2 * st], ea[g][2 * st + 1], eb[g][2 * st + 1], qf[pc][g0 + g][2 * st], qf[pc][g0 + g][2 * st + 1]);
+#pragma unroll
+                for (int g = 0; g < GB; g++) {
+                    const int gg = g0 + g;
+                    const float da = kv4_half_of(sa[gg >> 1], gg & 1), db = kv4_half_of(sb[gg >> 1], gg & 1);
+                    if (PAIR) {
+                        s[0][0] = fmaf(da, c[g][0] + c[g][1], s[0][0]); s[0][1] = fmaf(db, c[g][2] + c[g][3], s[0][1]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < NS; k++) { s[k][0] = fmaf(da, c[g][k], s[k][0]); s[k][1] = fmaf(db, c[g][2 + k], s[k][1]); }
+                    }
+                }
             }
         }
+        unsigned see = 0xffffffffu;                          // bit 2 k + half: that score is seen
         if (!inside) {
-            kv4_mask_steps<NG>(wa, t0 + 2 * j, cr.lo_any, cr.hi_any);
-            kv4_mask_steps<NG>(wb, t0 + 8 + 2 * j, cr.lo_any, cr.hi_any);
+#pragma unroll
+            for (int k = 0; k < NS; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int t = t0 + r + 8 * h;
+                    if (t < clo[k] || t > chi[k]) { see &= ~(1u << (2 * k + h)); s[k][h] = 0.f; }
+                }
         }
         // the largest value step (NaN left aside) decides the power of two that weight * step is scaled by
         {
             __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                mx = __hmax2(mx, __habs2(*reinterpret_cast<const __half2 *>(&wa[g])));
-                mx = __hmax2(mx, __habs2(*reinterpret_cast<const __half2 *>(&wb[g])));
+            for (int i = 0; i < (8 * NG + 31) / 32; i++) {
+                const int w = lane + 32 * i;                 // one word each: steps 2 w and 2 w + 1 of the 16 x NG
+                if (w < 8 * NG) {
+                    unsigned v = *reinterpret_cast<const unsigned *>(sg + 17 * HD + 4 * w);
+                    if (!inside) {
+                        const int ta = t0 + 2 * w / NG, tb = t0 + (2 * w + 1) / NG;
+                        v &= (ta >= cr.lo_any && ta < cr.hi_any ? 0xffffu : 0u) | (tb >= cr.lo_any && tb < cr.hi_any ? 0xffff0000u : 0u);
+                    }
+                    mx = __hmax2(mx, __habs2(*reinterpret_cast<const __half2 *>(&v)));
+                }
             }
             const float big = fmaxf(__low2float(mx), __high2float(mx));
-            if (__any_sync(0xffffffffu, big >= scalbnf(2.f, ve))) {
-                unsigned b = __float_as_uint(big);
-                for (int off = 16; off > 0; off >>= 1) { const unsigned o = __shfl_xor_sync(0xffffffffu, b, off); b = o > b ? o : b; }
-                const int e = (int)(b >> 23) - 127;          // (f16 subnormals are normal f32)
-                const float f = scalbnf(1.f, ve - e);
-                ve = e;
+            if (__any_sync(0xffffffffu, big >= vth)) {
+                const unsigned b = __reduce_max_sync(0xffffffffu, __float_as_uint(big)) & 0x7f800000u;   // 2^e
+                if (b) {                                     // (f16 subnormals are normal f32; all steps 0: nothing to add, any scale does)
+                    const float nn = 64.f / __uint_as_float(b), f = nn / vn, d = (float)(133 - (int)(b >> 23)) - vl;
+                    vth = 2.f * __uint_as_float(b); vn = nn; vl += d;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                    for (int k = 0; k < NS; k++) { m[k] -= d; l[k] *= f; }
 #pragma unroll
                     for (int g = 0; g < NG; g++)
 #pragma unroll
-                        for (int i = 0; i < 8; i++) acc[nt][g][i >> 2][i & 3] *= f;
+                        for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] *= f;
+                }
             }
         }
-        const float vn = scalbnf(64.f, -ve);                 // weight * step * vn < 256 * 2 * 64 = 2^15
-        float y[NT][4];                                      // scaled weights of positions 2 j, 2 j + 1, 2 j + 8, 2 j + 9 for column r; < 0: not seen
+        float e[NS][2];                                      // base-2 exponents of the scaled weights
+        bool up = false;
+        const float thr = 8.f + vl;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            float p0 = kv4_exp2(s[nt][0] - m[nt]), p1 = kv4_exp2(s[nt][1] - m[nt]);
-            if (!see[nt][0]) p0 = 0.f;
-            if (!see[nt][1]) p1 = 0.f;
-            l[nt] += p0 + p1;
-            p0 = see[nt][0] ? p0 * vn : -1.f; p1 = see[nt][1] ? p1 * vn : -1.f;
-            const int src = 8 * j + (r >> 1);
-            y[nt][0] = __shfl_sync(0xffffffffu, p0, src); y[nt][1] = __shfl_sync(0xffffffffu, p0, src + 4);
-            y[nt][2] = __shfl_sync(0xffffffffu, p1, src); y[nt][3] = __shfl_sync(0xffffffffu, p1, src + 4);
+        for (int k = 0; k < NS; k++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                e[k][h] = fmaf(s[k][h], desc[k], -m[k]);
+                if (!inside && !(see >> (2 * k + h) & 1)) e[k][h] = -INFINITY;
+                up |= e[k][h] > thr;
+            }
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+            for (int k = 0; k < NS; k++) {
+                float mx = m[k];
+#pragma unroll
+                for (int h = 0; h < 2; h++) if (see >> (2 * k + h) & 1) mx = fmaxf(mx, s[k][h] * desc[k] - vl);
+                for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                float f = mx == -INFINITY ? 1.f : kv4_exp2(m[k] - mx);
+                m[k] = mx; l[k] *= f;
+#pragma unroll
+                for (int h = 0; h < 2; h++) e[k][h] = see >> (2 * k + h) & 1 ? fmaf(s[k][h], desc[k], -mx) : -INFINITY;
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {            // the thread's output columns are its score columns
+                        acc[g][i >> 1][PAIR ? (i & 1) * 2 : (i & 1) * 2 + k] *= f;
+                        if (PAIR) acc[g][i >> 1][(i & 1) * 2 + 1] *= f;
+                    }
+            }
         }
+        // scaled weights (weight * step * vn < 256 * 2 * 64 = 2^15) of positions 2 j, 2 j + 1, 2 j + 8, 2 j + 9 for column r
+        float y[4];
+        bool hide[4];
+        {
+            float p[NS][2];
+#pragma unroll
+            for (int k = 0; k < NS; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    p[k][h] = kv4_exp2(e[k][h]);
+                    if (!inside && !(see >> (2 * k + h) & 1)) p[k][h] = 0.f;
+                    l[k] += p[k][h];
+                }
+            // score column c sits in lane 4 row + c (PAIR) or 4 row + c / 2, register c & 1
+            const int src = 8 * j + (r >> 1);
+            if (PAIR) {
+                y[0] = __shfl_sync(0xffffffffu, p[0][0], src); y[1] = __shfl_sync(0xffffffffu, p[0][0], src + 4);
+                y[2] = __shfl_sync(0xffffffffu, p[0][1], src); y[3] = __shfl_sync(0xffffffffu, p[0][1], src + 4);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float a0 = __shfl_sync(0xffffffffu, p[0][h], src), a1 = __shfl_sync(0xffffffffu, p[NS - 1][h], src);
+                    const float b0 = __shfl_sync(0xffffffffu, p[0][h], src + 4), b1 = __shfl_sync(0xffffffffu, p[NS - 1][h], src + 4);
+                    y[2 * h] = r & 1 ? a1 : a0; y[2 * h + 1] = r & 1 ? b1 : b0;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) hide[i] = false;
+            if (!inside) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = t0 + 2 * j + (i & 1) + 8 * (i >> 1);
+                    hide[i] = t < plo || t > phi;
+                }
+            }
+        }
+        {
+            unsigned va[NG], vb[NG], wa[NG], wb[NG];
+            kv4_ldsw<NG>(va, sg + 8 * HD + lane * (4 * NG));
+            kv4_ldsw<NG>(vb, sg + 12 * HD + lane * (4 * NG));
+            kv4_ldsw<NG>(wa, sg + 17 * HD + 2 * j * (2 * NG));
+            kv4_ldsw<NG>(wb, sg + 17 * HD + (8 + 2 * j) * (2 * NG));
+            unsigned b[NS][NG][2];                           // operand columns: PAIR: this lane's piece; else hi and lo
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                float x[4] = {y[0] * kv4_half_of(wa[g >> 1], g & 1), y[1] * kv4_half_of(wa[(NG + g) >> 1], (NG + g) & 1),
+                              y[2] * kv4_half_of(wb[g >> 1], g & 1), y[3] * kv4_half_of(wb[(NG + g) >> 1], (NG + g) & 1)};
+                if (!inside) {                               // a position that is not seen adds nothing, whatever its step holds
+#pragma unroll
+                    for (int i = 0; i < 4; i++) if (hide[i]) x[i] = 0.f;
+                }
+                if (PAIR) {
+                    b[0][g][0] = kv4_piece(x[0], x[1], sel); b[0][g][1] = kv4_piece(x[2], x[3], sel);
+                } else {
+                    kv4_pieces(x[0], x[1], b[0][g][0], b[NS - 1][g][0]);
+                    kv4_pieces(x[2], x[3], b[0][g][1], b[NS - 1][g][1]);
+                }
+            }
+            constexpr int GB = NG % 2 == 0 ? 2 : NG == 3 ? 3 : 1;
+#pragma unroll
+            for (int g0 = 0; g0 < NG; g0 += GB) {
+                unsigned ea[GB][4], eb[GB][4];
+#pragma unroll
+                for (int g = 0; g < GB; g++) { kv4_codes(va[g0 + g], ea[g]); kv4_codes(vb[g0 + g], eb[g]); }
+#pragma unroll
+                for (int pc = NS - 1; pc >= 0; pc--)
+#pragma unroll
+                    for (int g = 0; g < GB; g++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            kv4_mma(acc[g0 + g][h], ea[g][2 * h], ea[g][2 * h + 1], eb[g][2 * h], eb[g][2 * h + 1], b[pc][g0 + g][0], b[pc][g0 + g][1]);
+            }
+        }
+        };
+        if (t0 >= cr.lo_all && t0 + 15 < cr.hi_all) body(std::true_type{});
+        else body(std::false_type{});
+    }
+    // join the warps: a thread holds dims 32 g + 4 r + 0 .. 3 of its score columns
+    cp_async_wait<0>();
+    __syncthreads();
+    const float vs = 1.f / vn;                               // (a power of two)
+#pragma unroll
+    for (int k = 0; k < NS; k++) {
+        for (int o = 4; o < 32; o <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], o);
+        const int c = PAIR ? j : 2 * j + k;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            unsigned ea[4], eb[4];
-            kv4_codes(va[g], ea);
-            kv4_codes(vb[g], eb);
-            const float d0 = kv4_half_of(wa[g >> 1], g & 1), d1 = kv4_half_of(wa[(NG + g) >> 1], (NG + g) & 1);
-            const float d2 = kv4_half_of(wb[g >> 1], g & 1), d3 = kv4_half_of(wb[(NG + g) >> 1], (NG + g) & 1);
+            float o[4];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                // a position that is not seen adds nothing, whatever its step holds
-                const float x0 = y[nt][0] < 0.f ? 0.f : y[nt][0] * d0, x1 = y[nt][1] < 0.f ? 0.f : y[nt][1] * d1;
-                const float x2 = y[nt][2] < 0.f ? 0.f : y[nt][2] * d2, x3 = y[nt][3] < 0.f ? 0.f : y[nt][3] * d3;
-                const unsigned b0 = kv4_piece(x0, x1, sel), b1 = kv4_piece(x2, x3, sel);
-                kv4_mma(acc[nt][g][0], ea[0], ea[1], eb[0], eb[1], b0, b1);
-                kv4_mma(acc[nt][g][1], ea[2], ea[3], eb[2], eb[3], b0, b1);
-            }
+            for (int i = 0; i < 4; i++) o[i] = (PAIR ? acc[g][i >> 1][(i & 1) * 2] + acc[g][i >> 1][(i & 1) * 2 + 1] : acc[g][i >> 1][(i & 1) * 2 + k]) * vs;
+            *reinterpret_cast<float4 *>(js + ((size_t)warp * NC + c) * HD + g * 32 + 4 * r) = make_float4(o[0], o[1], o[2], o[3]);
         }
-    }
-    // join the warps: every thread holds, for pair j of each tile, dims 32 g + 4 r + 0 .. 3
-    const float vs = scalbnf(1.f / 64.f, ve);
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        for (int off = 4; off < 32; off <<= 1) l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], off);
-        const int c = nt * 4 + j;
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-            *reinterpret_cast<float4 *>(qs + ((size_t)warp * NC + c) * HD + g * 32 + 4 * r) =
-                make_float4((acc[nt][g][0][0] + acc[nt][g][0][1]) * vs, (acc[nt][g][0][2] + acc[nt][g][0][3]) * vs,
-                            (acc[nt][g][1][0] + acc[nt][g][1][1]) * vs, (acc[nt][g][1][2] + acc[nt][g][1][3]) * vs);
-        if (r == 0) { ml[warp * NC + c] = m[nt]; ml[DEC_W * NC + warp * NC + c] = l[nt]; }
+        if (r == 0) { ml[warp * NC + c] = m[k] + vl; ml[DEC_W * NC + warp * NC + c] = l[k] * vs; }
     }
     __syncthreads();
-    for (int i = tid; i < ncol * HD; i += DEC_W * 32) {
-        const int c = i / HD, d = i - c * HD, cc = c0 + c;
-        float M = -INFINITY, L = 0.f, o = 0.f;
+    if (warp == 0 && lane < NC) {                            // the factor of each warp's sums; m and l of all
+        float M = -INFINITY, L = 0.f, f[DEC_W];
 #pragma unroll
-        for (int w = 0; w < DEC_W; w++) M = fmaxf(M, ml[w * NC + c]);
+        for (int w = 0; w < DEC_W; w++) M = fmaxf(M, ml[w * NC + lane]);
 #pragma unroll
         for (int w = 0; w < DEC_W; w++) {
-            const float lw = ml[DEC_W * NC + w * NC + c], f = lw == 0.f ? 0.f : kv4_exp2(ml[w * NC + c] - M);
-            L = fmaf(lw, f, L);
-            o = fmaf(lw == 0.f ? 0.f : qs[((size_t)w * NC + c) * HD + d], f, o);
+            const float lw = ml[DEC_W * NC + w * NC + lane];
+            f[w] = lw == 0.f ? 0.f : kv4_exp2(ml[w * NC + lane] - M);
+            L = fmaf(lw, f[w], L);
         }
-        const size_t rh = (size_t)(sq.r0 + cc / a.G) * a.H + head * a.G + cc % a.G;
-        if (nsplit == 1) a.ctx[rh * HD + d] = L == 0.f ? 0.f : __fdiv_rn(o, L);
-        else {
+#pragma unroll
+        for (int w = 0; w < DEC_W; w++) ml[w * NC + lane] = f[w];
+        ml[DEC_W * NC + lane] = L; ml[2 * DEC_W * NC + lane] = M;
+    }
+    __syncthreads();
+    for (int i = tid; i < ncol * (HD / 4); i += DEC_W * 32) {
+        const int c = i / (HD / 4), d = (i - c * (HD / 4)) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < DEC_W; w++) {
+            const float f = ml[w * NC + c];
+            const float4 v = *reinterpret_cast<const float4 *>(js + ((size_t)w * NC + c) * HD + d);
+            if (f != 0.f) { o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w); }
+        }
+        const float L = ml[DEC_W * NC + c];
+        const size_t rh = (size_t)col[c] * a.H + col[NC + c];
+        if (nsplit == 1) {
+            *reinterpret_cast<float4 *>(a.ctx + rh * HD + d) = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                : make_float4(__fdiv_rn(o.x, L), __fdiv_rn(o.y, L), __fdiv_rn(o.z, L), __fdiv_rn(o.w, L));
+        } else {
             float *p = part + (rh * nsplit + split) * (HD + 4);
-            p[4 + d] = o;
-            if (d == 0) { p[0] = M; p[1] = L; }
+            *reinterpret_cast<float4 *>(p + 4 + d) = o;
+            if (d == 0) { p[0] = ml[2 * DEC_W * NC + c]; p[1] = L; }
         }
     }
 }
 
 // joins the spans of one (row, head): the same sums over {m, l, acc} with the maximum over all spans
-__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
-    const int row = blockIdx.x, h = blockIdx.y, hd = a.geo.hd, d = threadIdx.x;
+constexpr int MG_T = 256;
+__global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
+    __shared__ float red[MG_T / 32], ls[MG_T / 8];
+    __shared__ float4 os[MG_T];
+    const int row = blockIdx.x, h = blockIdx.y, hd = a.geo.hd, tid = threadIdx.x;
     pdl_trigger();
     pdl_wait();
     int seq, pos;
     const int st = kv4_row(a.b, row, &seq, &pos);
     if (st == KV4_ROW_NONE) return;
-    float *out = a.ctx + ((size_t)row * a.H + h) * hd + d;
+    float *out = a.ctx + ((size_t)row * a.H + h) * hd;
     const int n = st == KV4_ROW_OK ? a.b.row0[seq + 1] - a.b.row0[seq] : 0;
-    if (st == KV4_ROW_BAD || n > a.max_rows || a.b.len[seq] > a.max_len) { *out = 0.f; return; }
+    if (st == KV4_ROW_BAD || n > a.max_rows || a.b.len[seq] > a.max_len) {
+        if (tid < hd) out[tid] = 0.f;
+        return;
+    }
     // the spans that hold anything for this row's column tile
     const long long c = (long long)(row - a.b.row0[seq]) * a.G + h % a.G, c0 = c / pl.cols * pl.cols, last = (long long)n * a.G - 1;
     const long long cz = c0 + pl.cols - 1 < last ? c0 + pl.cols - 1 : last;
     const int pos0 = a.b.len[seq] - n;
     const Kv4Range cr = kv4_range(a, pos0 + (int)(c0 / a.G), pos0 + (int)(cz / a.G));
-    int live = (cr.hi_any - (cr.lo_any & ~(pl.align - 1)) + pl.span - 1) / pl.span;
+    int live = (cr.hi_any - (cr.lo_any & ~(KV4_PAGE - 1)) + pl.span - 1) / pl.span;
     if (live > pl.nsplit) live = pl.nsplit;
     const float *p = part + ((size_t)row * a.H + h) * pl.nsplit * (hd + 4);
-    float M = -INFINITY, L = 0.f, o = 0.f;
-    for (int i = 0; i < live; i++) M = fmaxf(M, p[(size_t)i * (hd + 4)]);
-    for (int i = 0; i < live; i++) {
-        const float li = p[(size_t)i * (hd + 4) + 1], f = li == 0.f ? 0.f : kv4_exp2(p[(size_t)i * (hd + 4)] - M);
-        L = fmaf(li, f, L);
-        o = fmaf(li == 0.f ? 0.f : p[(size_t)i * (hd + 4) + 4 + d], f, o);
+    float M = -INFINITY;
+    for (int i = tid; i < live; i += MG_T) M = fmaxf(M, p[(size_t)i * (hd + 4)]);
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if ((tid & 31) == 0) red[tid >> 5] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < MG_T / 32; w++) M = fmaxf(M, red[w]);
+    // thread group k takes spans k, k + ng, ...: four dims a thread, group order fixed
+    const int q4 = hd / 4, ng = MG_T / q4, k = tid / q4, d = tid - k * q4;
+    float L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (k < ng)
+        for (int i = k; i < live; i += ng) {
+            const float *pi = p + (size_t)i * (hd + 4);
+            const float li = pi[1], f = li == 0.f ? 0.f : kv4_exp2(pi[0] - M);
+            const float4 v = *reinterpret_cast<const float4 *>(pi + 4 + 4 * d);
+            L = fmaf(li, f, L);
+            if (li != 0.f) { o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w); }
+        }
+    if (k < ng) { os[k * q4 + d] = o; if (d == 0) ls[k] = L; }
+    __syncthreads();
+    if (k == 0) {
+        for (int i = 1; i < ng; i++) {
+            const float4 v = os[i * q4 + d];
+            L += ls[i]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+        }
+        *reinterpret_cast<float4 *>(out + 4 * d) = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+            : make_float4(__fdiv_rn(o.x, L), __fdiv_rn(o.y, L), __fdiv_rn(o.z, L), __fdiv_rn(o.w, L));
     }
-    *out = L == 0.f ? 0.f : __fdiv_rn(o, L);
 }
 
 }  // namespace
 
-// how a call is cut
+// How a call is cut.  Host numbers only (the limits the caller gave), so a captured call stays valid for any batch within
+// them.  Decode or prompt kernel: the decode kernel re-reads the pages for every 8 columns, the prompt kernel fills 16
+// lines a warp: 32 columns (Q_DEC) is where they meet at 4096 positions of 128-wide heads.
+// Spans: with `units` (sequence, KV head, tile) triples of P pages on `slots` resident CTAs, a CTA costs its pages plus
+// about FIX pages' time of set-up and join.  When all CTAs are resident at once the longest one counts; otherwise the total
+// work over the slots plus a last CTA (lengths of a ragged batch are taken as 0.6 of the limit).  The cut with the least of
+// that: 64 sequences of up to 8192 positions 136 us uncut, 108 us with 5 spans of 26 pages, 113 us with 3; one sequence of
+// 131072 positions 62 us on 148 CTAs, 38 us on 444 (one full set), 55 us on 1184.
 static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     Kv4Plan p{};
     const long long cols = (long long)a.max_rows * a.G;
+    const int NG = a.geo.hd / 32;
     p.decode = cols <= 32;
-    p.nt = cols > 4 && a.geo.hd <= 128 ? 2 : 1;
-    p.cols = p.decode ? 4 * p.nt : KV4_LINES;
-    p.align = p.decode ? 16 : KV4_PAGE;
+    p.cols = !p.decode ? KV4_LINES : cols > 4 ? 8 : 4;
     p.ntile = (int)((cols + p.cols - 1) / p.cols);
     if (p.ntile < 1) p.ntile = 1;
-    // the longest stretch of positions a CTA's columns see together, from a multiple of `align` on
+    // the longest stretch of positions a CTA's columns see together, from a page's first on
     long long range = a.max_len;
     const long long rows_a_tile = p.cols / a.G + 2 < a.max_rows ? p.cols / a.G + 2 : a.max_rows;
-    if (a.window > 0 && (long long)a.window + rows_a_tile + p.align < range) range = (long long)a.window + rows_a_tile + p.align;
-    const long long units = (long long)a.b.nseq * a.geo.KV * p.ntile, most = (range + 63) / 64;
-    long long n = p.decode ? (6LL * sms + units - 1) / units : units < 2LL * sms ? (3LL * sms + units - 1) / units : 1;
-    if (n > most) n = most;
-    if (n < 1) n = 1;
-    long long span = (range + n - 1) / n;
-    span = (span + 63) / 64 * 64;
-    if (span < 64) span = 64;
-    p.span = (int)span;
-    p.nsplit = (int)((range + span - 1) / span);
+    if (a.window > 0 && (long long)a.window + rows_a_tile + KV4_PAGE < range) range = (long long)a.window + rows_a_tile + KV4_PAGE;
+    const int occ = !p.decode ? 2 : p.cols == 4 ? kv4_decode_ctas(NG, true) : kv4_decode_ctas(NG, false);
+    const double units = (double)a.b.nseq * a.geo.KV * p.ntile, slots = (double)sms * occ, FIX = p.decode ? 6 : 2;
+    const long long P = (range + KV4_PAGE - 1) / KV4_PAGE, least = p.decode ? (P + DEC_NP - 1) / DEC_NP : 1;
+    const double w = a.b.nseq > 1 ? 0.6 : 1.0;
+    long long best = least > 0 ? least : 1;
+    double cost = 1e300;
+    for (long long n = best; n <= P && n <= 1024 + best; n++) {
+        const long long pages = (P + n - 1) / n;
+        if (n > best && (P + n - 2) / (n - 1) == pages) continue;            // the same spans with fewer cuts
+        const double c = (units * n <= slots ? pages + FIX : units * (w * P + FIX * n) / slots + pages + FIX) + (n > 1 ? 2 : 0);
+        if (c < cost) { cost = c; best = n; }
+    }
+    // a prompt is cut only to fill the GPU (4096 rows at 4096 positions: 587 us whole, 820 us in two spans, whose joins move
+    // rows x heads x hd x spans f32 values)
+    if (!p.decode) best = units < slots ? (long long)(slots / units) : 1;
+    if (best > P) best = P > 0 ? P : 1;
+    const long long pages = P ? (P + best - 1) / best : 1;
+    p.span = (int)(pages * KV4_PAGE);
+    p.nsplit = (int)((range + p.span - 1) / p.span);
     if (p.nsplit < 1) p.nsplit = 1;
     return p;
 }
@@ -308,14 +524,25 @@ size_t kv4_attend_scratch_bytes(const Kv4Attend &a, int sms) {
     return p.nsplit > 1 ? (size_t)a.b.rows * a.H * p.nsplit * (a.geo.hd + 4) * 4 : 0;
 }
 
-template <int NG, int NT>
+template <int NG, bool PAIR>
 static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st) {
-    constexpr size_t smem = ((size_t)DEC_W * NT * 4 * NG * 32 + 2 * DEC_W * NT * 4 + NT * 4) * 4;
-    static_assert(smem <= 48 * 1024, "fits without an attribute");
+    constexpr size_t smem = DecL<NG, PAIR>::SMEM;
+    static bool attr[MOTY_MAX_DEV];
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= MOTY_MAX_DEV) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: device %d", dev);
+    if (!attr[dev]) {
+        CK(cudaFuncSetAttribute(kv4_decode_kernel<NG, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        attr[dev] = true;
+    }
     const long long grid = (long long)a.b.nseq * a.geo.KV * p.ntile * p.nsplit;
     if (grid > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend: %lld CTAs", grid);
-    CK(moty_launch_pdl(kv4_decode_kernel<NG, NT>, dim3((unsigned)grid), dim3(DEC_W * 32), smem, st, a, p.ntile, p.nsplit, p.span, part));
+    CK(moty_launch_pdl(kv4_decode_kernel<NG, PAIR>, dim3((unsigned)grid), dim3(DEC_W * 32), smem, st, a, p.ntile, p.nsplit, p.span, part));
     return 0;
+}
+template <int NG>
+static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st) {
+    return p.cols == 4 ? kv4_decode_go<NG, true>(a, p, part, st) : kv4_decode_go<NG, false>(a, p, part, st);
 }
 
 int launch_kv4_attend(const Kv4Attend &a, float *part, int sms, cudaStream_t st) {
@@ -324,17 +551,17 @@ int launch_kv4_attend(const Kv4Attend &a, float *part, int sms, cudaStream_t st)
     int rc = 0;
     if (!p.decode) rc = launch_kv4_prompt(a, p, part, st);
     else switch (a.geo.hd / 32) {
-        case 1: rc = p.nt == 2 ? kv4_decode_go<1, 2>(a, p, part, st) : kv4_decode_go<1, 1>(a, p, part, st); break;
-        case 2: rc = p.nt == 2 ? kv4_decode_go<2, 2>(a, p, part, st) : kv4_decode_go<2, 1>(a, p, part, st); break;
-        case 3: rc = p.nt == 2 ? kv4_decode_go<3, 2>(a, p, part, st) : kv4_decode_go<3, 1>(a, p, part, st); break;
-        case 4: rc = p.nt == 2 ? kv4_decode_go<4, 2>(a, p, part, st) : kv4_decode_go<4, 1>(a, p, part, st); break;
-        case 5: rc = kv4_decode_go<5, 1>(a, p, part, st); break;
-        case 6: rc = kv4_decode_go<6, 1>(a, p, part, st); break;
-        case 7: rc = kv4_decode_go<7, 1>(a, p, part, st); break;
-        default: rc = kv4_decode_go<8, 1>(a, p, part, st); break;
+        case 1: rc = kv4_decode_go<1>(a, p, part, st); break;
+        case 2: rc = kv4_decode_go<2>(a, p, part, st); break;
+        case 3: rc = kv4_decode_go<3>(a, p, part, st); break;
+        case 4: rc = kv4_decode_go<4>(a, p, part, st); break;
+        case 5: rc = kv4_decode_go<5>(a, p, part, st); break;
+        case 6: rc = kv4_decode_go<6>(a, p, part, st); break;
+        case 7: rc = kv4_decode_go<7>(a, p, part, st); break;
+        default: rc = kv4_decode_go<8>(a, p, part, st); break;
     }
     CKR(rc);
     if (p.nsplit > 1)
-        CK(moty_launch_pdl(kv4_merge_kernel, dim3(a.b.rows, a.H), dim3(a.geo.hd), (size_t)0, st, a, p, (const float *)part));
+        CK(moty_launch_pdl(kv4_merge_kernel, dim3(a.b.rows, a.H), dim3(MG_T), (size_t)0, st, a, p, (const float *)part));
     return 0;
 }

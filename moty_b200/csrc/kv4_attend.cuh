@@ -5,7 +5,7 @@
 // decode: the kernel for few rows.  A CTA takes `cols` (row, query head) pairs of one KV head of one sequence, ntile such
 // tiles a sequence at most, and one of nsplit spans of `span` positions.
 constexpr int KV4_LINES = 64;             // (row, query head) pairs a CTA of the prompt kernel takes
-struct Kv4Plan { bool decode; int nt, cols, ntile, nsplit, span, align; };
+struct Kv4Plan { bool decode; int cols, ntile, nsplit, span; };
 int launch_kv4_prompt(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st);
 
 #ifdef __CUDACC__

@@ -7,20 +7,13 @@
 #pragma once
 #include "kv4.cuh"
 
-// Pages are written by the launch before (append), which a chained launch may overlap until pdl_wait: plain loads, not the
-// read-only path.  They are read once: not kept in L1.
-__device__ __forceinline__ int4 kv4_ld16(const uint8_t *p) {
-    int4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-// N 32-bit words from a 4 N byte aligned address (16-, 8- or 4-byte loads as N allows)
+// N words from shared memory, 4 N byte aligned
 template <int N>
-__device__ __forceinline__ void kv4_ldw(unsigned (&w)[N], const uint8_t *p) {
+__device__ __forceinline__ void kv4_ldsw(unsigned (&w)[N], const uint8_t *p) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
-            const int4 v = kv4_ld16(p + 16 * i);
+            const uint4 v = *reinterpret_cast<const uint4 *>(p + 16 * i);
             w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
     } else if constexpr (N % 2 == 0) {
@@ -34,6 +27,7 @@ __device__ __forceinline__ void kv4_ldw(unsigned (&w)[N], const uint8_t *p) {
         for (int i = 0; i < N; i++) w[i] = *reinterpret_cast<const unsigned *>(p + 4 * i);
     }
 }
+
 // NG f16 steps of one key row (2 NG bytes aligned), two to a word
 template <int NG>
 __device__ __forceinline__ void kv4_ldsteps(unsigned (&w)[(NG + 1) / 2], const uint8_t *p) {
@@ -73,14 +67,22 @@ __device__ __forceinline__ void kv4_mask_steps(unsigned (&w)[NG], int t, int lo,
     }
 }
 
+// (The bare bits are n in f16 subnormals and need four operations less a word, with -8 sum(q) as the sum's start; but the
+// matrix unit cuts sums off, and there the larger terms left 1.9e-6 instead of 2e-7.)
+constexpr unsigned KV4_C = 0x64006400u;
 // nibbles i and i + 4 of a word as f16 pairs of code values (n - 8): 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n
 __device__ __forceinline__ void kv4_codes(unsigned w, unsigned (&e)[4]) {
-    constexpr unsigned M0 = 0x000f000fu, M1 = 0x00f000f0u, C = 0x64006400u;
+    constexpr unsigned M0 = 0x000f000fu, M1 = 0x00f000f0u;
+    const unsigned C = KV4_C;
     const unsigned s = w >> 8;
     const __half2 b0 = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));      // 1032
     const __half2 c1 = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));      // 1 / 16
     const __half2 b1 = __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480));      // -72 = -(1024 / 16 + 8)
-    unsigned r[4] = {(w & M0) | C, (w & M1) | C, (s & M0) | C, (s & M1) | C};
+    unsigned r[4];                                           // (w & M) | C in one operation: C in a register, M in the instruction
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[0]) : "r"(w), "n"(M0), "r"(C));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[1]) : "r"(w), "n"(M1), "r"(C));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[2]) : "r"(s), "n"(M0), "r"(C));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r[3]) : "r"(s), "n"(M1), "r"(C));
     __half2 h;
     h = __hsub2(*reinterpret_cast<__half2 *>(&r[0]), b0); e[0] = *reinterpret_cast<unsigned *>(&h);
     h = __hfma2(*reinterpret_cast<__half2 *>(&r[1]), c1, b1); e[1] = *reinterpret_cast<unsigned *>(&h);
@@ -89,19 +91,39 @@ __device__ __forceinline__ void kv4_codes(unsigned w, unsigned (&e)[4]) {
 }
 
 __device__ __forceinline__ void kv4_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same with a sum that starts from zero
+__device__ __forceinline__ void kv4_mma0(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ unsigned kv4_pack_f16(float lo_half, float hi_half) {                // two f32, rounded, low half first
     const __half2 h = __floats2half2_rn(lo_half, hi_half);
     return *reinterpret_cast<const unsigned *>(&h);
 }
-// the pair (x0, x1) as f16: its leading pieces (sel = 0) or what they leave over (sel = 1)
-__device__ __forceinline__ unsigned kv4_piece(float x0, float x1, float sel) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 f = __half22float2(h);
-    return kv4_pack_f16(fmaf(-sel, f.x, x0), fmaf(-sel, f.y, x1));
+// x0 + s h.low and x1 + s h.high for a pair h and a factor s of f16 (s h is exact here: s is 0 or -1)
+__device__ __forceinline__ void kv4_rest(float &x0, float &x1, unsigned h, unsigned short s) {
+    asm("{.reg .f16 l, u; mov.b32 {l, u}, %2; fma.rn.f32.f16 %0, l, %3, %0; fma.rn.f32.f16 %1, u, %3, %1;}" : "+f"(x0), "+f"(x1) : "r"(h), "h"(s));
 }
+constexpr unsigned short KV4_H0 = 0x8000, KV4_HM1 = 0xbc00;  // -0 and -1
+// the pair (x0, x1) as f16: its leading pieces (s = -0) or what they leave over (s = -1)
+__device__ __forceinline__ unsigned kv4_piece(float x0, float x1, unsigned short s) {
+    kv4_rest(x0, x1, kv4_pack_f16(x0, x1), s);
+    return kv4_pack_f16(x0, x1);
+}
+// both: x = h + lo
+__device__ __forceinline__ void kv4_pieces(float x0, float x1, unsigned &h, unsigned &lo) {
+    h = kv4_pack_f16(x0, x1);
+    kv4_rest(x0, x1, h, KV4_HM1);
+    lo = kv4_pack_f16(x0, x1);
+}
+// 2^k for -126 <= k <= 127, and x 2^k for any k of the f32 range (two factors, each a normal number)
+__device__ __forceinline__ float kv4_pow2(int k) { return __int_as_float((k + 127) << 23); }
+__device__ __forceinline__ float kv4_scale2(float x, int k) { const int h = k >> 1; return x * kv4_pow2(h) * kv4_pow2(k - h); }
+// the power of two that brings a query row whose largest magnitude has the bits mb below 2^14 (0 for a row of zeros)
+__device__ __forceinline__ int kv4_q_shift(unsigned mb) { return mb ? 13 + 127 - (int)(mb >> 23 ? mb >> 23 : 1) : 0; }
 __device__ __forceinline__ float kv4_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

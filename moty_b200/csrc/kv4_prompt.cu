@@ -21,27 +21,6 @@ template <int NG> struct PrL {
     static constexpr size_t SMEM = (size_t)PR_W * NG * 4 * 512 + 2 * UNIT;
 };
 
-// N words from shared memory, 4 N byte aligned
-template <int N>
-__device__ __forceinline__ void kv4_ldsw(unsigned (&w)[N], const uint8_t *p) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(p + 16 * i);
-            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-        }
-    } else if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(p + 8 * i);
-            w[2 * i] = v.x; w[2 * i + 1] = v.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = *reinterpret_cast<const unsigned *>(p + 4 * i);
-    }
-}
-
 template <int NG>
 __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
     constexpr int HD = NG * 32, UNIT = PrL<NG>::UNIT, PT = PrL<NG>::PT, NL = 16 * PR_W;
@@ -93,8 +72,8 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
         mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
         mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
         const bool fin = mb < 0x7f800000u;                   // |q| 2^k < 2^14; a line that is not finite has NaN scores
-        const int k = fin && mb ? 13 - ilogbf(__uint_as_float(mb)) : 0;
-        desc[hlf] = fin ? (float)ldexp((double)a.scale * 1.4426950408889634, -k) : __int_as_float(0x7fffffff);
+        const int k = fin ? kv4_q_shift(mb) : 0;
+        desc[hlf] = fin ? kv4_scale2(a.scale * 1.44269504f, -k) : __int_as_float(0x7fffffff);
         const int p = pos0 + row;
         chi[hlf] = have ? p : -1;
         clo[hlf] = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
@@ -105,8 +84,9 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
             for (int i = 0; i < 8; i++) x[i] = 0.f;
             if (have && fin) {
                 const float4 v0 = *reinterpret_cast<const float4 *>(src + g * 32 + 8 * j), v1 = *reinterpret_cast<const float4 *>(src + g * 32 + 8 * j + 4);
-                x[0] = scalbnf(v0.x, k); x[1] = scalbnf(v0.y, k); x[2] = scalbnf(v0.z, k); x[3] = scalbnf(v0.w, k);
-                x[4] = scalbnf(v1.x, k); x[5] = scalbnf(v1.y, k); x[6] = scalbnf(v1.z, k); x[7] = scalbnf(v1.w, k);
+                x[0] = v0.x; x[1] = v0.y; x[2] = v0.z; x[3] = v0.w; x[4] = v1.x; x[5] = v1.y; x[6] = v1.z; x[7] = v1.w;
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = kv4_scale2(x[i], k);
             }
             // step s covers nibbles 2 s and 2 s + 1 of a word and their partners 4 on: registers 0, 2 (line r) and 1, 3 (line r + 8)
 #pragma unroll
@@ -114,8 +94,8 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
 #pragma unroll
                 for (int pc = 0; pc < 2; pc++) {
                     unsigned *dst = reinterpret_cast<unsigned *>(qw + ((g * 2 + s) * 2 + pc) * 512 + lane * 16);
-                    dst[hlf] = kv4_piece(x[2 * s], x[2 * s + 4], (float)pc);
-                    dst[2 + hlf] = kv4_piece(x[2 * s + 1], x[2 * s + 5], (float)pc);
+                    dst[hlf] = kv4_piece(x[2 * s], x[2 * s + 4], pc ? KV4_HM1 : KV4_H0);
+                    dst[2 + hlf] = kv4_piece(x[2 * s + 1], x[2 * s + 5], pc ? KV4_HM1 : KV4_H0);
                 }
         }
     }
@@ -125,7 +105,7 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
     for (int g = 0; g < NG; g++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[g][i >> 2][i & 3] = 0.f;
-    int ve = -24;
+    float vth = 0.f, vn = 0.f;                               // 2^(e + 1) and 64 * 2^-e for the exponent e of the largest value step so far
     const int *tab = a.b.table + (size_t)seq * a.b.ld;
     const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
     const size_t page_bytes = kv4_page_bytes(a.geo);
@@ -175,10 +155,11 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
                     for (int nt = 0; nt < PT; nt++) {
                         unsigned e[4];
                         kv4_codes(kw[nt][g], e);
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
+                        float c[4];
 #pragma unroll
                         for (int st = 0; st < 2; st++) {
-                            kv4_mma(c, qf[st][1].x, qf[st][1].y, qf[st][1].z, qf[st][1].w, e[2 * st], e[2 * st + 1]);
+                            if (st == 0) kv4_mma0(c, qf[st][1].x, qf[st][1].y, qf[st][1].z, qf[st][1].w, e[2 * st], e[2 * st + 1]);
+                            else kv4_mma(c, qf[st][1].x, qf[st][1].y, qf[st][1].z, qf[st][1].w, e[2 * st], e[2 * st + 1]);
                             kv4_mma(c, qf[st][0].x, qf[st][0].y, qf[st][0].z, qf[st][0].w, e[2 * st], e[2 * st + 1]);
                         }
                         const float d0 = kv4_half_of(ks[nt][g >> 1], g & 1), d1 = kv4_half_of(ks[nt][(NG + g) >> 1], (NG + g) & 1);
@@ -251,18 +232,17 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
             }
             // the largest value step (NaN left aside) decides the power of two that weight * step is scaled by
             const float big = fmaxf(__low2float(mx), __high2float(mx));
-            if (__any_sync(0xffffffffu, big >= scalbnf(2.f, ve))) {
-                unsigned bb = __float_as_uint(big);
-                for (int off = 16; off > 0; off >>= 1) bb = max(bb, __shfl_xor_sync(0xffffffffu, bb, off));
-                const int e = (int)(bb >> 23) - 127;
-                const float f = scalbnf(1.f, ve - e);
-                ve = e;
+            if (__any_sync(0xffffffffu, big >= vth)) {
+                const unsigned bb = __reduce_max_sync(0xffffffffu, __float_as_uint(big)) & 0x7f800000u;   // 2^e
+                if (bb) {
+                    const float nn = 64.f / __uint_as_float(bb), f = vn == 0.f ? 1.f : nn / vn;
+                    vth = 2.f * __uint_as_float(bb); vn = nn;
 #pragma unroll
-                for (int g = 0; g < NG; g++)
+                    for (int g = 0; g < NG; g++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) acc[g][i >> 2][i & 3] *= f;
+                        for (int i = 0; i < 16; i++) acc[g][i >> 2][i & 3] *= f;
+                }
             }
-            const float vn = scalbnf(64.f, -ve);
 #pragma unroll
             for (int nt = 0; nt < PT; nt++)                  // block b: line r: positions 2j, 2j+1 | line r+8 | the same 8 positions on
 #pragma unroll
@@ -270,8 +250,6 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 float c[4][4];
-#pragma unroll
-                for (int i = 0; i < 16; i++) c[i >> 2][i & 3] = 0.f;
 #pragma unroll
                 for (int b = 0; b < PT / 2; b++) {
                     const float d[4] = {kv4_half_of(wa[b][g >> 1], g & 1), kv4_half_of(wa[b][(NG + g) >> 1], (NG + g) & 1),
@@ -285,18 +263,14 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
                     }
                     unsigned h[4], lo[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {            // x = h + lo
-                        const __half2 hh = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-                        const float2 f = __half22float2(hh);
-                        h[i] = *reinterpret_cast<const unsigned *>(&hh);
-                        lo[i] = kv4_pack_f16(x[2 * i] - f.x, x[2 * i + 1] - f.y);
-                    }
+                    for (int i = 0; i < 4; i++) kv4_pieces(x[2 * i], x[2 * i + 1], h[i], lo[i]);
                     unsigned ea[4], eb[4];
                     kv4_codes(va[b][g], ea);
                     kv4_codes(vb[b][g], eb);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        kv4_mma(c[i], lo[0], lo[1], lo[2], lo[3], ea[i], eb[i]);
+                        if (b == 0) kv4_mma0(c[i], lo[0], lo[1], lo[2], lo[3], ea[i], eb[i]);
+                        else kv4_mma(c[i], lo[0], lo[1], lo[2], lo[3], ea[i], eb[i]);
                         kv4_mma(c[i], h[0], h[1], h[2], h[3], ea[i], eb[i]);
                     }
                 }
@@ -306,7 +280,7 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
         }
     }
     // a thread holds, for lines r and r + 8, dims 32 g + 8 j + 0 .. 7: dim i + 4 k of them in acc[g][i][line half * 2 + k]
-    const float vs = scalbnf(1.f / 64.f, ve);
+    const float vs = vn == 0.f ? 1.f : 1.f / vn;             // (a power of two)
 #pragma unroll
     for (int hlf = 0; hlf < 2; hlf++) {
         l[hlf] += __shfl_xor_sync(0xffffffffu, l[hlf], 1);
