@@ -45,37 +45,133 @@ __device__ __forceinline__ void kv4_put_v(uint8_t *unit, int hd, int t, int g, i
     if (lane == 0) reinterpret_cast<unsigned short *>(unit + kv4_v_step_off(hd))[t * (hd >> 5) + g] = d;
 }
 
-// the unit and slot of batch row r for (layer, head), or null (a row behind the last sequence; a bad one sets *err)
-__device__ __forceinline__ uint8_t *kv4_find(const Kv4Geom &geo, uint8_t *mem, const Kv4Batch &b, int r, int layer, int head, int *t,
-                                             int *pos, int *err, bool absent_ok) {
-    int seq;
-    const int st = kv4_row(b, r, &seq, pos);
-    if (st == KV4_ROW_NONE) return nullptr;
-    if (st == KV4_ROW_BAD) { atomicExch(err, 1); return nullptr; }
-    const int page = b.table[(size_t)seq * b.ld + *pos / KV4_PAGE];
-    if (!kv4_page_ok(geo, page)) { if (!(absent_ok && page == -1)) atomicExch(err, 1); return nullptr; }
-    *t = *pos % KV4_PAGE;
-    return mem + kv4_unit_off(geo, page, layer, head);
+// ---- many rows at once -----------------------------------------------------------------------------------------------
+// A CTA takes ST_ROWS rows of one KV head, a thread eight dims of a row at a time: a group is the four threads of a quad
+// (two shuffles a reduction), eight key codes are one word of the page, the value codes go through shared memory so that
+// two positions of a pair leave as one word and neighbouring threads write neighbouring bytes.
+constexpr int ST_ROWS = 16, ST_T = 256;
+
+// The quad's step for x[8] a thread: *d = its bits, returns it (0 for a group of zeros, NaN for one that is not finite).
+__device__ __forceinline__ float kv4_quad_step(const float (&x)[8], unsigned short *d) {
+    int pb = 0, nb = 0;                                        // largest positive value and largest magnitude of a negative one, as bits
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int b = __float_as_int(x[i]);
+        pb = max(pb, b);
+        nb = max(nb, b ^ (int)0x80000000);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        pb = max(pb, __shfl_xor_sync(0xffffffffu, pb, o));
+        nb = max(nb, __shfl_xor_sync(0xffffffffu, nb, o));
+    }
+    const bool bad = pb >= 0x7f800000 || nb >= 0x7f800000;
+    bool neg = nb > pb;                                        // the sign of the first value of largest magnitude
+    if (__any_sync(0xffffffffu, pb == nb && pb > 0)) {         // both signs reach it: look which comes first
+        int first = 64;                                        // 2 * dim + (negative)
+#pragma unroll
+        for (int i = 7; i >= 0; i--) {
+            const int b = __float_as_int(x[i]);
+            if (b == pb) first = 2 * i;
+            if ((b ^ (int)0x80000000) == nb) first = 2 * i + 1;
+        }
+        first += first < 64 ? 16 * (threadIdx.x & 3) : 0;
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+        if (pb == nb) neg = first & 1;
+    }
+    const float big = __int_as_float(neg ? nb : pb), other = __int_as_float(neg ? pb : nb);
+    const float step = fminf(fmaxf(__fdiv_rn(big, 8.f), __fdiv_rn(other, 7.f)), 65504.f);
+    const __half h = __float2half_rn(neg || big == 0.f ? step : -step);
+    *d = bad ? (unsigned short)0x7fff : __half_as_ushort(h);
+    return bad ? 0.f : __half2float(h);                        // codes of a bad group are 0, as with a step of 0
+}
+// The eight nibbles (code + 8) of x for step d.  t = x / d approximately, rounded to an integer in the low bits of an f32;
+// the remainder x - t d is exact, and where it is half a step or more (a tie, or the approximation on the wrong side of
+// one, or out of range) the quotient is divided out.
+__device__ __forceinline__ unsigned kv4_quant8(const float (&x)[8], float d) {
+    constexpr float MAGIC = 12582912.f;                        // 1.5 * 2^23
+    const float inv = d == 0.f ? 0.f : __frcp_rn(d), half = 0.5f * fabsf(d);
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float c = __fsub_rn(__fmaf_rn(x[i], inv, MAGIC), MAGIC);
+        if (!(fabsf(__fmaf_rn(-c, d, x[i])) < half)) c = d == 0.f ? 0.f : rintf(__fdiv_rn(x[i], d));
+        c = fminf(fmaxf(c, -8.f), 7.f);
+        w |= (__float_as_uint(__fadd_rn(c, MAGIC + 8.f)) & 15u) << (4 * i);
+    }
+    return w;
+}
+// what the rows of a CTA are: unit (null: skip) and position in the page
+struct Kv4Rows { uint8_t *unit[ST_ROWS]; int t[ST_ROWS], seq[ST_ROWS]; };
+__device__ __forceinline__ void kv4_rows(Kv4Rows &s, const Kv4Geom &geo, uint8_t *mem, const Kv4Batch &b, int row0, int layer, int head, int *err,
+                                         bool absent_ok) {
+    const int i = threadIdx.x, r = row0 + i;
+    if (i < ST_ROWS) {
+        uint8_t *unit = nullptr;
+        int seq = -1, pos = 0;
+        if (r < b.rows) {
+            const int st = kv4_row(b, r, &seq, &pos);
+            if (st == KV4_ROW_BAD) atomicExch(err, 1);
+            if (st == KV4_ROW_OK) {
+                const int page = b.table[(size_t)seq * b.ld + pos / KV4_PAGE];
+                if (kv4_page_ok(geo, page)) unit = mem + kv4_unit_off(geo, page, layer, head);
+                else if (!(absent_ok && page == -1)) atomicExch(err, 1);
+            }
+            if (st == KV4_ROW_NONE) seq = -1;
+        }
+        s.unit[i] = unit; s.t[i] = pos % KV4_PAGE; s.seq[i] = seq;
+    }
+    __syncthreads();
 }
 
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4Geom geo, uint8_t *mem, int layer, const float *k, const float *v, long long ld,
-                                                         Kv4Batch b, int *err) {
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);      // one warp per (row, head)
+__global__ void __launch_bounds__(ST_T) kv4_append_kernel(Kv4Geom geo, uint8_t *mem, int layer, const float *k, const float *v, long long ld,
+                                                          Kv4Batch b, int *err) {
+    __shared__ Kv4Rows rs;
+    __shared__ unsigned short vp[ST_ROWS][64 + 2];             // value pieces of four dims: [row][g * 8 + r]
+    const int tid = threadIdx.x, hd = geo.hd, NG = hd >> 5, row0 = blockIdx.x * ST_ROWS, head = blockIdx.y;
     pdl_trigger();
     pdl_wait();
-    if (w >= (long long)b.rows * geo.KV) return;
-    const int r = (int)(w / geo.KV), head = (int)(w % geo.KV);
-    int t = 0, pos;
-    uint8_t *unit = kv4_find(geo, mem, b, r, layer, head, &t, &pos, err, false);
-    if (!unit) return;
-    for (int g = 0; g < geo.hd >> 5; g++) {
-        unsigned short d;
-        const size_t at = (size_t)r * ld + head * geo.hd + g * 32 + lane;
-        unsigned nib = kv4_quant_lane(k[at], lane, &d);
-        kv4_put_k(unit, geo.hd, t, g, lane, nib, d);
-        nib = kv4_quant_lane(v[at], lane, &d);
-        kv4_put_v(unit, geo.hd, t, g, lane, nib, d);
+    kv4_rows(rs, geo, mem, b, row0, layer, head, err, false);
+    const int per = hd >> 3, items = ST_ROWS * per;            // eight dims an item; a quad never leaves its group
+    for (int it = tid; it < (items + ST_T - 1) / ST_T * ST_T; it += ST_T) {
+        const int i = it / per, d8 = it - i * per, g = d8 >> 2, j = d8 & 3;
+        uint8_t *unit = it < items ? rs.unit[i] : nullptr;
+        float kx[8], vx[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) kx[e] = vx[e] = 0.f;
+        if (unit) {
+            const size_t at = (size_t)(row0 + i) * ld + (size_t)head * hd + d8 * 8;
+            *reinterpret_cast<float4 *>(kx) = *reinterpret_cast<const float4 *>(k + at);
+            *reinterpret_cast<float4 *>(kx + 4) = *reinterpret_cast<const float4 *>(k + at + 4);
+            *reinterpret_cast<float4 *>(vx) = *reinterpret_cast<const float4 *>(v + at);
+            *reinterpret_cast<float4 *>(vx + 4) = *reinterpret_cast<const float4 *>(v + at + 4);
+        }
+        unsigned short kd, vd;
+        const float ks = kv4_quad_step(kx, &kd), vs = kv4_quad_step(vx, &vd);
+        if (unit) {
+            const int t = rs.t[i];
+            *reinterpret_cast<unsigned *>(unit + kv4_k_word(hd, t, g, j)) = kv4_quant8(kx, ks);
+            const unsigned w = kv4_quant8(vx, vs);
+            vp[i][g * 8 + 2 * j] = (unsigned short)w; vp[i][g * 8 + 2 * j + 1] = (unsigned short)(w >> 16);
+            if (j == 0) reinterpret_cast<unsigned short *>(unit + kv4_k_step_off(hd))[t * NG + g] = kd;
+            if (j == 1) reinterpret_cast<unsigned short *>(unit + kv4_v_step_off(hd))[t * NG + g] = vd;
+        }
+    }
+    __syncthreads();
+    for (int it = tid; it < ST_ROWS * NG * 8; it += ST_T) {    // [r][row][g]: consecutive threads, consecutive bytes of a block
+        const int g = it % NG, q = it / NG, i = q % ST_ROWS, r = q / ST_ROWS;
+        uint8_t *unit = rs.unit[i];
+        if (!unit) continue;
+        const int t = rs.t[i];
+        const unsigned lo = vp[i][g * 8 + r];
+        if (t & 1) {
+            if (i > 0 && rs.unit[i - 1] == unit && rs.seq[i - 1] == rs.seq[i]) continue;             // stored with its partner
+        } else if (i + 1 < ST_ROWS && rs.unit[i + 1] == unit && rs.seq[i + 1] == rs.seq[i]) {
+            *reinterpret_cast<unsigned *>(unit + kv4_v_piece(hd, t, g, r)) = lo | (unsigned)vp[i + 1][g * 8 + r] << 16;
+            continue;
+        }
+        *reinterpret_cast<unsigned short *>(unit + kv4_v_piece(hd, t, g, r)) = (unsigned short)lo;
     }
 }
 
@@ -146,26 +242,36 @@ __global__ void __launch_bounds__(256) kv4_append_rope_kernel(Kv4Geom geo, uint8
 }
 
 // the batch's own positions back as f32: k, v [rows][KV * hd]; 0 where the page is absent
-__global__ void __launch_bounds__(256) kv4_fetch_kernel(Kv4Geom geo, const uint8_t *mem, int layer, float *k, float *v, Kv4Batch b, int *err) {
-    const int lane = threadIdx.x & 31, hd = geo.hd, NG = hd >> 5;
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);      // one warp per (row, head)
+__device__ __forceinline__ void kv4_values8(float *out, unsigned w, float d) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = __fmul_rn((float)((int)(w >> (4 * e) & 15u) - 8), d);
+    *reinterpret_cast<float4 *>(out) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4 *>(out + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__global__ void __launch_bounds__(ST_T) kv4_fetch_kernel(Kv4Geom geo, const uint8_t *mem, int layer, float *k, float *v, Kv4Batch b, int *err) {
+    __shared__ Kv4Rows rs;
+    const int tid = threadIdx.x, hd = geo.hd, NG = hd >> 5, row0 = blockIdx.x * ST_ROWS, head = blockIdx.y;
     pdl_trigger();
     pdl_wait();
-    if (w >= (long long)b.rows * geo.KV) return;
-    const int r = (int)(w / geo.KV), head = (int)(w % geo.KV);
-    int seq, pos, t = 0, p2;
-    if (kv4_row(b, r, &seq, &pos) == KV4_ROW_NONE) return;
-    const uint8_t *unit = kv4_find(geo, const_cast<uint8_t *>(mem), b, r, layer, head, &t, &p2, err, true);
-    for (int g = 0; g < NG; g++) {
-        const size_t at = ((size_t)r * geo.KV + head) * hd + g * 32 + lane;
-        float kx = 0.f, vx = 0.f;
+    kv4_rows(rs, geo, const_cast<uint8_t *>(mem), b, row0, layer, head, err, true);
+    const int per = hd >> 3;
+    for (int it = tid; it < ST_ROWS * per; it += ST_T) {
+        const int i = it / per, d8 = it - i * per, g = d8 >> 2, j = d8 & 3, t = rs.t[i];
+        if (rs.seq[i] < 0) continue;
+        const uint8_t *unit = rs.unit[i];
+        unsigned kw = 0, vw = 0;
+        float kd = 0.f, vd = 0.f;
         if (unit) {
-            const unsigned kw = *reinterpret_cast<const unsigned *>(unit + kv4_k_word(hd, t, g, lane >> 3));
-            const unsigned vw = *reinterpret_cast<const unsigned short *>(unit + kv4_v_piece(hd, t, g, lane >> 2));
-            kx = __fmul_rn((float)((int)((kw >> (4 * (lane & 7))) & 15u) - 8), f16bits_to_f32(reinterpret_cast<const uint16_t *>(unit + kv4_k_step_off(hd))[t * NG + g]));
-            vx = __fmul_rn((float)((int)((vw >> (4 * (lane & 3))) & 15u) - 8), f16bits_to_f32(reinterpret_cast<const uint16_t *>(unit + kv4_v_step_off(hd))[t * NG + g]));
+            kw = *reinterpret_cast<const unsigned *>(unit + kv4_k_word(hd, t, g, j));
+            vw = *reinterpret_cast<const unsigned short *>(unit + kv4_v_piece(hd, t, g, 2 * j)) |
+                 (unsigned)*reinterpret_cast<const unsigned short *>(unit + kv4_v_piece(hd, t, g, 2 * j + 1)) << 16;
+            kd = f16bits_to_f32(reinterpret_cast<const uint16_t *>(unit + kv4_k_step_off(hd))[t * NG + g]);
+            vd = f16bits_to_f32(reinterpret_cast<const uint16_t *>(unit + kv4_v_step_off(hd))[t * NG + g]);
         }
-        k[at] = kx; v[at] = vx;
+        const size_t at = ((size_t)(row0 + i) * geo.KV + head) * hd + d8 * 8;
+        kv4_values8(k + at, kw, kd);
+        kv4_values8(v + at, vw, vd);
     }
 }
 
@@ -173,10 +279,8 @@ __global__ void __launch_bounds__(256) kv4_fetch_kernel(Kv4Geom geo, const uint8
 
 int launch_kv4_append(const Kv4Geom &geo, uint8_t *mem, int layer, const float *k, const float *v, long long ld, const Kv4Batch &b,
                       int *err, cudaStream_t st) {
-    const long long warps = (long long)b.rows * geo.KV;
-    if (warps <= 0) return 0;
-    if ((warps + 7) / 8 > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_append: %d rows", b.rows);
-    CK(moty_launch_pdl(kv4_append_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), (size_t)0, st, geo, mem, layer, k, v, ld, b, err));
+    if (b.rows <= 0) return 0;
+    CK(moty_launch_pdl(kv4_append_kernel, dim3((unsigned)((b.rows + (long long)ST_ROWS - 1) / ST_ROWS), geo.KV), dim3(ST_T), (size_t)0, st, geo, mem, layer, k, v, ld, b, err));
     return 0;
 }
 
@@ -189,9 +293,7 @@ int launch_kv4_append_rope(const Kv4Geom &geo, uint8_t *mem, int layer, int H, f
 }
 
 int launch_kv4_fetch(const Kv4Geom &geo, const uint8_t *mem, int layer, float *k, float *v, const Kv4Batch &b, int *err, cudaStream_t st) {
-    const long long warps = (long long)b.rows * geo.KV;
-    if (warps <= 0) return 0;
-    if ((warps + 7) / 8 > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_fetch: %d rows", b.rows);
-    CK(moty_launch_pdl(kv4_fetch_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), (size_t)0, st, geo, mem, layer, k, v, b, err));
+    if (b.rows <= 0) return 0;
+    CK(moty_launch_pdl(kv4_fetch_kernel, dim3((unsigned)((b.rows + (long long)ST_ROWS - 1) / ST_ROWS), geo.KV), dim3(ST_T), (size_t)0, st, geo, mem, layer, k, v, b, err));
     return 0;
 }
