@@ -14,7 +14,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import Attn, Mat, MotyCudaError, lib, stream_handle, ACT_GELU_TANH, ACT_SILU
+from . import Attn, Kv4, Kv4Batch, Mat, MotyCudaError, lib, stream_handle, ACT_GELU_TANH, ACT_SILU
 
 
 def _ck(rc):
@@ -384,3 +384,252 @@ class GemmaDecoder(DenseDecoder):
         self.hist.index_copy_(0, self.cnt, self.out_id)
         self.pos_dev += 1
         self.cnt += 1
+
+
+class PagedDecoder(DenseDecoder):
+    """Several sequences of one dense (or routed) model at once over a paged 4-bit KV cache (``moty_b200.Kv4``): prompts
+    and single tokens of any mix of sequences go through the layers as one batch of rows; sequences can be forked (full
+    pages shared, the last one copied), ended, and the pages in use moved together.  The layer order is DenseDecoder's;
+    only the attention core differs (append_rope + attend on the pages instead of ``Attn``).
+
+    ``pages``: pages of 64 positions in the pool (all layers of a position lie in one page).  ``max_pages``: the most a
+    sequence may hold.  ``run`` raises when the pool is out of pages, and changes nothing then."""
+
+    def __init__(self, layers, head: Mat, final_norm, n_heads, n_kv_heads, head_dim, pages, max_seqs=64, max_pages=64, theta=1e6, eps=1e-6,
+                 rot=None, device=0, max_S=64):
+        import torch
+        self.torch = torch
+        self.dev = torch.device(f"cuda:{device}")
+        self.layers, self.head = layers, head
+        self.H, self.KV, self.hd, self.eps = n_heads, n_kv_heads, head_dim, float(eps)
+        self.theta, self.rot = float(theta), head_dim if rot is None else rot
+        self.D = head.I
+        f = lambda a: None if a is None else torch.from_numpy(np.ascontiguousarray(a, np.float32)).to(self.dev)
+        self.final_norm = f(final_norm)
+        self.ln = [(f(l.in_ln), f(l.post_ln)) for l in layers]
+        self.qk_gain = [(f(l.qn), f(l.kn)) for l in layers]
+        self.kv = Kv4(len(layers), n_kv_heads, head_dim, pages, device=device)
+        self.max_seqs, self.max_pages = max_seqs, max_pages
+        self.table = np.full((max_seqs, max_pages), -1, np.int32)        # row = sequence id
+        self.lens = np.zeros(max_seqs, np.int32)
+        self.used = np.zeros(max_seqs, bool)
+        self.stream = torch.cuda.Stream(device=self.dev)
+        self._alloc(max_S)
+
+    def _alloc(self, S):
+        t, dev = self.torch, self.dev
+        qw, kw = self.H * self.hd, self.KV * self.hd
+        e = lambda *shape: t.empty(shape, device=dev, dtype=t.float32)
+        self._drop_graph()
+        self.cap = S
+        self.x, self.nrm, self.tmp, self.ctx = e(S, self.D), e(S, self.D), e(S, self.D), e(S, qw)
+        self.qkvb = e(S, qw + 2 * kw)
+        self.ids = t.empty((S,), device=dev, dtype=t.int32)
+        self.out_id = t.empty((S,), device=dev, dtype=t.int32)
+        self.logits = None
+
+    # -- sequences ------------------------------------------------------------------------------------------------------
+    def new(self) -> int:
+        """An empty sequence; returns its id."""
+        free = np.flatnonzero(~self.used)
+        if not free.size:
+            raise MotyCudaError(f"all {self.max_seqs} sequences are in use")
+        self.used[free[0]] = True
+        return int(free[0])
+
+    def end(self, sid) -> None:
+        """Forget a sequence; pages it does not share are free again."""
+        self._check(sid)
+        self._drop_graph()
+        self.kv.release(self.table[sid])
+        self.table[sid] = -1; self.lens[sid] = 0; self.used[sid] = False
+
+    def fork(self, sid, n=1) -> list:
+        """n copies of a sequence: they share its full pages, the last partial page is copied on the device."""
+        self._check(sid)
+        self._drop_graph()
+        L = int(self.lens[sid]); full = L // Kv4.PAGE
+        free = np.flatnonzero(~self.used)[:n]
+        if free.size < n:
+            raise MotyCudaError(f"{n} forks, {free.size} sequences free")
+        fresh = self.kv.alloc(n) if L % Kv4.PAGE else np.full(n, -1, np.int32)
+        for _ in range(n):
+            self.kv.retain(self.table[sid, :full])
+        t = self.torch
+        with t.cuda.stream(self.stream):
+            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
+            table, lens = up(self.table), up(self.lens)
+            src, dst, new = up(np.full(n, sid)), up(free), up(fresh)
+            self.kv.fork_dev(n, src.data_ptr(), dst.data_ptr(), new.data_ptr(), self.max_seqs, lens.data_ptr(), table.data_ptr(),
+                             self.max_pages, stream=stream_handle(self.stream))
+            self.table, self.lens = table.cpu().numpy(), lens.cpu().numpy()
+            self._check_kernels()
+        self.used[free] = True
+        return [int(s) for s in free]
+
+    def compact(self) -> int:
+        """Move the pages in use to the lowest ids; returns how many moved."""
+        self._drop_graph()
+        src, dst = self.kv.compact_plan()
+        if not src.size:
+            return 0
+        t = self.torch
+        with t.cuda.stream(self.stream):
+            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
+            table, s, d = up(self.table), up(src), up(dst)
+            self.kv.compact_dev(src.size, s.data_ptr(), d.data_ptr(), table.numel(), table.data_ptr(), table.data_ptr(), stream=stream_handle(self.stream))
+            self.table = table.cpu().numpy()
+            self._check_kernels()
+        return int(src.size)
+
+    def _check(self, sid):
+        if not (0 <= sid < self.max_seqs and self.used[sid]):
+            raise MotyCudaError(f"sequence {sid} is not in use")
+
+    def _reserve(self, sids, more):
+        """Pages for `more[i]` further positions of each sequence: all of them or none."""
+        grow = []
+        for s, n in zip(sids, more):
+            have, want = -(-int(self.lens[s]) // Kv4.PAGE), -(-(int(self.lens[s]) + int(n)) // Kv4.PAGE)
+            if want > self.max_pages:
+                raise MotyCudaError(f"sequence {s} would hold {want} pages, more than {self.max_pages}")
+            grow.append([p for p in range(have, want) if self.table[s, p] < 0])
+        ids = self.kv.alloc(sum(map(len, grow)))
+        at = 0
+        for s, g in zip(sids, grow):
+            self.table[s, g] = ids[at:at + len(g)]; at += len(g)
+
+    # -- steps ----------------------------------------------------------------------------------------------------------
+    def run(self, batch, want_logits=False):
+        """batch: [(sequence id, token ids), ...], each sequence once.  Appends every sequence's tokens to it and returns the
+        greedy next token after the last of each (and those rows' logits when asked)."""
+        t, L = self.torch, lib()
+        sids = [int(s) for s, _ in batch]
+        toks = [np.ascontiguousarray(i, np.int32).ravel() for _, i in batch]
+        for s in sids:
+            self._check(s)
+        if len(set(sids)) != len(sids) or any(not i.size for i in toks):
+            raise MotyCudaError("each sequence of a batch once, with at least one token")
+        counts = [i.size for i in toks]
+        S, n = sum(counts), len(sids)
+        self._reserve(sids, counts)
+        self._drop_graph()                       # a batch of another shape may grow the library's scratch
+        if S > self.cap:
+            self._alloc(S)
+        self.lens[sids] += np.array(counts, np.int32)
+        row0 = np.concatenate([[0], np.cumsum(counts)])
+        with t.cuda.stream(self.stream):
+            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
+            d_row0, d_len, d_tab = up(row0), up(self.lens[sids]), up(self.table[sids])
+            b = Kv4Batch(n, S, d_row0.data_ptr(), d_len.data_ptr(), d_tab.data_ptr(), self.max_pages, max_rows=max(counts),
+                         max_len=int(self.lens[sids].max()))
+            self.ids[:S].copy_(t.from_numpy(np.concatenate(toks)))
+            self._embed_rows(S)
+            self._layers_paged(S, b)
+            last = self.x[:S].index_select(0, (d_row0[1:] - 1).long())
+            logits = t.empty((n, self.head.O), device=self.dev, dtype=t.float32)
+            self._head(last, n, logits)
+            out = self.out_id[:n].cpu().numpy().copy()
+            self._check_kernels()
+            return (out, logits.cpu().numpy()) if want_logits else out
+
+    def greedy(self, sids, tokens, n):
+        """n greedy tokens for each of the sequences after ``tokens``, the step captured ONCE into a CUDA graph and replayed
+        (lengths move on the device).  Returns int32 [len(sids)][n]."""
+        t = self.torch
+        sids = [int(s) for s in sids]
+        for s in sids:
+            self._check(s)
+        if len(set(sids)) != len(sids) or not sids or n < 1:
+            raise MotyCudaError("each sequence once, at least one, and at least one token")
+        k = len(sids)
+        self._reserve(sids, [n] * k)
+        if k > self.cap:
+            self._alloc(k)
+        self._drop_graph()
+        start = self.lens[sids].copy()
+        with t.cuda.stream(self.stream):
+            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
+            row0, tab, lens = up(np.arange(k + 1)), up(self.table[sids]), up(start)
+            first = up(tokens)
+            hist, cnt = t.zeros((n + 1, k), device=self.dev, dtype=t.int32), t.zeros((1,), device=self.dev, dtype=t.int64)
+            logits = t.empty((k, self.head.O), device=self.dev, dtype=t.float32)
+            b = Kv4Batch(k, k, row0.data_ptr(), lens.data_ptr(), tab.data_ptr(), self.max_pages, max_rows=1, max_len=int(start.max()) + n)
+
+            def body():
+                lens.add_(1)
+                self._embed_rows(k)
+                self._layers_paged(k, b)
+                self._head(self.x[:k], k, logits)
+                self.ids[:k].copy_(self.out_id[:k])
+                hist.index_copy_(0, cnt, self.out_id[:k].view(1, k))
+                cnt.add_(1)
+
+            def reset():
+                self.ids[:k].copy_(first); lens.copy_(up(start)); cnt.zero_()
+
+            reset()
+            body()                               # one plain run: scratch, kernel attributes (its rows are written again below)
+        self.stream.synchronize()
+        _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 1))
+        try:
+            g = t.cuda.CUDAGraph()
+            with t.cuda.graph(g, stream=self.stream):
+                body()
+            with t.cuda.stream(self.stream):
+                reset()
+                for _ in range(n):
+                    g.replay()
+            self.stream.synchronize()
+            self._check_kernels()
+            del g
+        finally:
+            _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 0))
+        self.lens[sids] += n
+        return hist[:n].cpu().numpy().T.copy()
+
+    def _embed_rows(self, S):
+        p = lambda ten: C.c_void_p(ten.data_ptr())
+        _ck(lib().moty_cuda_embed_rows_dev(self.head.h, p(self.x), p(self.ids), S, C.c_float(1.0), C.c_void_p(stream_handle(self.torch.cuda.current_stream()))))
+
+    def _head(self, rows, n, logits):
+        p = lambda ten: C.c_void_p(ten.data_ptr())
+        sh = C.c_void_p(stream_handle(self.torch.cuda.current_stream()))
+        _ck(lib().moty_cuda_rmsnorm_dev(p(self.nrm), p(rows), p(self.final_norm), n, self.D, C.c_float(self.eps), sh))
+        _ck(lib().moty_cuda_head_argmax_dev(self.head.h, p(self.nrm), n, p(self.out_id), p(logits), sh))
+
+    def _layers_paged(self, S, b):
+        """DenseDecoder._layers on self.x [S][D] with the rows' attention on the pages."""
+        L, D, eps = lib(), self.D, C.c_float(self.eps)
+        stream = stream_handle(self.torch.cuda.current_stream())
+        sh = C.c_void_p(stream)
+        p = lambda ten: C.c_void_p(ten.data_ptr())
+        qw, kw = self.H * self.hd, self.KV * self.hd
+        nl = len(self.layers)
+        _ck(L.moty_cuda_rmsnorm_dev(p(self.nrm), p(self.x), p(self.ln[0][0]), S, D, eps, sh))
+        base = self.qkvb.data_ptr()
+        for i, (l, (in_ln, post_ln), (qn, kn)) in enumerate(zip(self.layers, self.ln, self.qk_gain)):
+            if l.qkv is not None:                # one product, rows [q | k | v]
+                _ck(L.moty_cuda_mat_apply_dev(l.qkv.h, p(self.qkvb), p(self.nrm), S, sh))
+                qp, kp, vp, ldq, ldk = base, base + 4 * qw, base + 4 * (qw + kw), qw + 2 * kw, qw + 2 * kw
+            else:
+                qp, kp, vp, ldq, ldk = base, base + 4 * S * qw, base + 4 * S * (qw + kw), 0, 0
+                for m, ptr in ((l.q, qp), (l.k, kp), (l.v, vp)):
+                    _ck(L.moty_cuda_mat_apply_dev(m.h, C.c_void_p(ptr), p(self.nrm), S, sh))
+            self.kv.append_rope_dev(i, self.H, qp, kp, vp, b, self.rot, self.theta, self.eps, qn.data_ptr() if qn is not None else 0,
+                                    kn.data_ptr() if kn is not None else 0, stream=stream, q_ld=ldq, kv_ld=ldk)
+            self.kv.attend_dev(i, self.ctx.data_ptr(), qp, self.H, b, stream=stream, q_ld=ldq)
+            _ck(L.moty_cuda_mat_apply_dev(l.o.h, p(self.tmp), p(self.ctx), S, sh))
+            _ck(L.moty_cuda_add_rmsnorm_dev(p(self.x), p(self.tmp), p(self.nrm), p(post_ln), S, D, eps, sh))
+            if l.moe is not None:
+                _ck(L.moty_cuda_moe_apply_dev(l.moe.h, p(self.tmp), p(self.nrm), S, None, 0, l.norm_topk, None, None, sh))
+            else:
+                _ck(L.moty_cuda_ffn_dev(l.gate.h, l.up.h, l.down.h, ACT_SILU, p(self.tmp), p(self.nrm), S, sh))
+            if i + 1 < nl:
+                _ck(L.moty_cuda_add_rmsnorm_dev(p(self.x), p(self.tmp), p(self.nrm), p(self.ln[i + 1][0]), S, D, eps, sh))
+            else:
+                _ck(L.moty_cuda_add_dev(p(self.x), p(self.tmp), C.c_longlong(S * D), sh))
+
+    def close(self):
+        self._drop_graph()
+        self.kv.close()
