@@ -489,16 +489,17 @@ static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     const long long cols = (long long)a.max_rows * a.G;
     const int NG = a.geo.hd / 32;
     p.decode = cols <= 32;
-    p.cols = !p.decode ? KV4_LINES : cols > 4 ? 8 : 4;
+    p.tc = cols > KV4_LINES && NG >= 2 && NG <= 4;
+    p.cols = p.tc ? KV4_TC_LINES : !p.decode ? KV4_LINES : cols > 4 ? 8 : 4;
     p.ntile = (int)((cols + p.cols - 1) / p.cols);
     if (p.ntile < 1) p.ntile = 1;
     // the longest stretch of positions a CTA's columns see together, from a page's first on
     long long range = a.max_len;
     const long long rows_a_tile = p.cols / a.G + 2 < a.max_rows ? p.cols / a.G + 2 : a.max_rows;
     if (a.window > 0 && (long long)a.window + rows_a_tile + KV4_PAGE < range) range = (long long)a.window + rows_a_tile + KV4_PAGE;
-    const int occ = !p.decode ? 2 : p.cols == 4 ? kv4_decode_ctas(NG, true) : kv4_decode_ctas(NG, false);
+    const int occ = p.tc ? 1 : !p.decode ? 2 : p.cols == 4 ? kv4_decode_ctas(NG, true) : kv4_decode_ctas(NG, false);
     const double units = (double)a.b.nseq * a.geo.KV * p.ntile, slots = (double)sms * occ, FIX = p.decode ? 6 : 2;
-    const long long P = (range + KV4_PAGE - 1) / KV4_PAGE, least = p.decode ? (P + DEC_NP - 1) / DEC_NP : 1;
+    const long long P = (range + KV4_PAGE - 1) / KV4_PAGE, least = p.decode ? (P + DEC_NP - 1) / DEC_NP : p.tc ? (P + KV4_TC_PAGES - 1) / KV4_TC_PAGES : 1;
     const double w = a.b.nseq > 1 ? 0.6 : 1.0;
     long long best = least > 0 ? least : 1;
     double cost = 1e300;
@@ -511,6 +512,7 @@ static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     // a prompt is cut only to fill the GPU (4096 rows at 4096 positions: 587 us whole, 820 us in two spans, whose joins move
     // rows x heads x hd x spans f32 values)
     if (!p.decode) best = units < slots ? (long long)(slots / units) : 1;
+    if (best < least) best = least;
     if (best > P) best = P > 0 ? P : 1;
     const long long pages = P ? (P + best - 1) / best : 1;
     p.span = (int)(pages * KV4_PAGE);
@@ -549,7 +551,8 @@ int launch_kv4_attend(const Kv4Attend &a, float *part, int sms, cudaStream_t st)
     const Kv4Plan p = kv4_plan(a, sms);
     if (p.nsplit > 1 && !part) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: scratch for %d spans missing", p.nsplit);
     int rc = 0;
-    if (!p.decode) rc = launch_kv4_prompt(a, p, part, st);
+    if (p.tc) rc = launch_kv4_prompt_tc(a, p, part, st);
+    else if (!p.decode) rc = launch_kv4_prompt(a, p, part, st);
     else switch (a.geo.hd / 32) {
         case 1: rc = kv4_decode_go<1>(a, p, part, st); break;
         case 2: rc = kv4_decode_go<2>(a, p, part, st); break;

@@ -1,0 +1,531 @@
+// kv4_prompt_tc.cu -- attention over the paged 4-bit KV cache for prompts, on the 5th-generation tensor cores.
+//
+// A CTA takes 128 lines ((row, query head) pairs of one KV head of one sequence) and walks the pages of its span, 64
+// positions a step:
+//     S = Q K^T   [128 x 64]     three products: q lo * k hi, q hi * k lo, q hi * k hi
+//     O = P V     [128 x hd]     three products: p lo * v hi, p hi * v lo, p hi * v hi
+// f32 accuracy from f16 operands: an operand is hi + lo, f16 each.  A value held is code * step, 4 x 11 bits, so k and v are
+// exact as hi + lo (the rest of an f16 product is a multiple of the smallest f16); q (scaled by a power of two a line) and
+// the softmax weights carry 22 bits; the dropped lo * lo term is 2^-22 of a product.  Steps of 4096 and more would overflow
+// f16: a page that has one is brought down by 2^4.  O starts from zero at every page and is added to f32 registers, because
+// the tensor core's own sum drifts over a long prompt.
+//   warps 0-7   softmax, two threads a line (half the positions, half the dims each): S from TMEM, running maximum (moved when
+//               passed by 8 in base-2 units), weights back to TMEM as the A operand of the second product, then the O of the
+//               page before added to the registers
+//   warps 8-11  a page's codes and steps into shared memory (two pages ahead), then as k and v^T operand tiles (K-major,
+//               128-byte swizzle): eight key dims of a position, or eight positions of a value dim, are one 16-byte piece
+//   warp 12     issues the products: S of page j + 1 before O of page j, so that the softmax of a page runs behind two
+//               products
+// Everything between the roles is a double buffer (all 512 TMEM columns).  What bounds it: the six products, 1536
+// cycles of tensor core a page at hd = 128.  Every wait is bounded; on expiry all roles leave and the error word is set.
+// An infinity or NaN of a key makes its scores NaN; a NaN step of a value is taken out of the product (a weight of 0 would
+// spread it to lines that do not see it) and set in the result of the lines that do.
+#include "kv4_frag.cuh"
+#include "kv4_attend.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+constexpr int PT_M = KV4_TC_LINES, PT_NP = KV4_TC_PAGES, PT_T = 416, PT_REGS = 128, PT_REGS_SOFT = 152, PT_REGS_STAGE = 80;
+static_assert(256 * PT_REGS_SOFT + 128 * PT_REGS_STAGE + 32 * PT_REGS <= PT_T * PT_REGS, "register shares");
+constexpr uint32_t TM_S = 0, TM_P = 128, TM_O = 256;         // TMEM columns: S 2 x 64, P 2 x (32 hi + 32 lo), O 2 x 128
+
+template <int NG> struct PtL {
+    static constexpr int HD = NG * 32, NSUB = (NG + 1) / 2;
+    static constexpr int KS = (NG % 2 ? NG : NG + 1) * 16;   // bytes between staged key rows (an odd number of 16-byte pieces)
+    static constexpr int VS = 4 * HD + 16;                   // bytes between staged value halves (eight positions)
+    static constexpr int RK = 64 * KS, RV = 8 * VS, RST = 128 * NG, RAW = RK + RV + 2 * RST;
+    static constexpr int Q = NSUB * PT_M * 128, K = NSUB * 64 * 128, V = HD * 128;      // one piece (hi or lo) of an operand
+    static constexpr int OFF_K = 2 * Q, OFF_V = OFF_K + 4 * K, OFF_RAW = OFF_V + 4 * V, OFF_LIST = OFF_RAW + 2 * RAW;
+    static constexpr int SMEM = OFF_LIST + PT_NP * 8 + 1024;
+};
+
+struct PtShared {
+    uint64_t kfull[2], vfull[2], sfull[2], sempty[2], pfull[2], pvdone[2], oempty[2];
+    uint32_t tmem;
+    int abort, n;
+    float fk[8], fv[8];                                      // by page (the staging warps are up to five pages ahead of the last reader): what scores and outputs are to be multiplied by
+    unsigned long long nan[8][4];                            // by page and group: positions whose value step is NaN
+    int anynan[8];
+    float mx[2][2][PT_M];                                    // by page, half: a line's largest score; at the end a line's sum of weights
+    int big;                                                 // a step of the staged page that would overflow: bit 0 keys, bit 1 values
+};
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// D [tmem] (+)= A * B^T, f16 in, f32 sums; A from shared memory or from TMEM
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tm_ld32(float (&v)[32], uint32_t addr) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+        "%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tm_ld16(uint32_t (&r)[16], uint32_t addr) {                  // (tm_wait before the registers are used)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tm_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_st16(uint32_t addr, const unsigned (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                   "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// bounded (a page is about a microsecond; each poll may itself wait a while)
+constexpr uint32_t PT_LIMIT = 1u << 22;
+__device__ __forceinline__ bool pt_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    return moty_mbar_wait_abortable(smem_u32(bar), parity, abort_flag, PT_LIMIT);
+}
+// the whole warp waits, or leaves, together
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    const bool ok = pt_wait(bar, parity, abort_flag);
+    return __all_sync(0xffffffffu, ok);
+}
+// the two warps of a line quarter: one reads what the other wrote; both go on, or leave, together
+__device__ __forceinline__ bool pair_and(int quarter, bool ok) {
+    int all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, %2, 64, q;\n\tselp.s32 %0, 1, 0, p;\n\t}"
+                 : "=r"(all) : "r"((int)ok), "r"(2 + quarter) : "memory");
+    return all != 0;
+}
+__device__ __forceinline__ void stager_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// the same, and whether all 128 threads say yes: they go on, or leave, together
+__device__ __forceinline__ bool stager_and(bool ok) {
+    int all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, 1, 128, q;\n\tselp.s32 %0, 1, 0, p;\n\t}"
+                 : "=r"(all) : "r"((int)ok) : "memory");
+    return all != 0;
+}
+
+// the word's values times the step pair d (one step twice for keys, two positions' steps for values): 4 pairs hi, 4 pairs lo
+__device__ __forceinline__ void kv4_values_hl(unsigned w, __half2 d, unsigned (&hi)[4], unsigned (&lo)[4]) {
+    unsigned e[4];
+    kv4_codes(w, e);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 c = *reinterpret_cast<__half2 *>(&e[i]), h = __hmul2(c, d), l = __hfma2(c, d, __hneg2(h));
+        hi[i] = *reinterpret_cast<const unsigned *>(&h);
+        lo[i] = *reinterpret_cast<const unsigned *>(&l);
+    }
+}
+
+template <int NG>
+__global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part, int *err_wait) {
+    using L = PtL<NG>;
+    constexpr int HD = L::HD, UNIT = 72 * HD;
+    extern __shared__ uint8_t sm_raw_[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw_) + 1023) & ~(uintptr_t)1023);
+    __shared__ PtShared sh;
+    int2 *list = reinterpret_cast<int2 *>(sm + L::OFF_LIST);                 // {page, first position} of the pages that are there
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int split = blockIdx.x % nsplit, u = blockIdx.x / nsplit;
+    const int tile = ntile - 1 - u / (a.geo.KV * a.b.nseq), hs = u % (a.geo.KV * a.b.nseq), head = hs % a.geo.KV, seq = hs / a.geo.KV;
+    pdl_trigger();
+    pdl_wait();
+    const Kv4Seq sq = kv4_load_seq(a, seq);
+    if (!sq.ok) {
+        if (nsplit == 1 && tile == 0) kv4_zero_rows(a, sq, head);
+        return;
+    }
+    const long long lines = (long long)sq.n * a.G, c0 = (long long)tile * PT_M;
+    if (c0 >= lines) return;
+    const int ncol = lines - c0 < PT_M ? (int)(lines - c0) : PT_M;
+    const int pos0 = sq.len - sq.n;
+    const Kv4Range cr = kv4_range(a, pos0 + (int)(c0 / a.G), pos0 + (int)((c0 + ncol - 1) / a.G));
+    const int t_lo = (cr.lo_any & ~(KV4_PAGE - 1)) + split * span, t_hi = cr.hi_any - t_lo < span ? cr.hi_any : t_lo + span;
+    if (t_lo >= cr.hi_any && nsplit > 1) return;
+
+    if (tid == 0) {
+        sh.abort = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.kfull[i], 128); mbar_init(&sh.vfull[i], 128);
+            mbar_init(&sh.sfull[i], 1); mbar_init(&sh.sempty[i], 256); mbar_init(&sh.pfull[i], 256); mbar_init(&sh.pvdone[i], 1);
+            mbar_init(&sh.oempty[i], 256);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 8) {                                         // the pages of the span that are there, in order
+        const int np = t_hi > t_lo ? (t_hi - t_lo + KV4_PAGE - 1) / KV4_PAGE : 0;
+        const int *tab = a.b.table + (size_t)seq * a.b.ld + t_lo / KV4_PAGE;
+        int n = 0;
+        for (int i0 = 0; i0 < np; i0 += 32) {
+            const int i = i0 + lane, id = i < np ? tab[i] : -1;
+            const bool ok = kv4_page_ok(a.geo, id);
+            if (!ok && id != -1) atomicExch(a.err, 1);
+            const unsigned m = __ballot_sync(0xffffffffu, ok);
+            if (ok) list[n + __popc(m & ((1u << lane) - 1))] = make_int2(id, t_lo + i * KV4_PAGE);
+            n += __popc(m);
+        }
+        if (lane == 0) sh.n = n;
+    }
+    // a softmax thread's line: its query row, limits, scale; the row goes to shared memory in two pieces
+    float desc = 0.f;
+    int clo = 0, chi = 0x7fffffff;                           // (lines that are not there see everything, and are not written)
+    size_t rh = 0;
+    const int quarter = warp & 3, half = warp >> 2, line = quarter * 32 + lane;
+    if (warp < 8) {
+        const bool have = line < ncol;
+        const float *src = a.q;
+        if (have) {
+            const long long cc = c0 + line;
+            const int row = (int)(cc / a.G), g0 = (int)(cc - (long long)row * a.G), p = pos0 + row;
+            src = a.q + (size_t)(sq.r0 + row) * a.q_ld + (size_t)(head * a.G + g0) * HD;
+            rh = (size_t)(sq.r0 + row) * a.H + head * a.G + g0;
+            chi = p;
+            clo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+        }
+        unsigned mb = 0;
+        if (have)
+#pragma unroll 8
+            for (int i = 0; i < HD / 4; i++) {
+                const uint4 v = reinterpret_cast<const uint4 *>(src)[i];
+                mb = max(max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu)), mb);
+            }
+        const bool fin = mb < 0x7f800000u;
+        const int k = fin ? kv4_q_shift(mb) : 0;
+        // (not below the smallest normal number: -infinity times it has to stay -infinity)
+        desc = fin ? fmaxf(kv4_scale2(a.scale * 1.44269504f, -k), 1.17549435e-38f) : __int_as_float(0x7fffffff);
+#pragma unroll 2
+        for (int c = half * 2 * NG; c < (half + 1) * 2 * NG; c++) {                   // piece c = 4 g + j: dims 8 c + 0, 4, 1, 5, 2, 6, 3, 7 (the order of a code word's pairs)
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = 0.f;
+            if (have && fin) {
+                const float4 v0 = reinterpret_cast<const float4 *>(src)[2 * c], v1 = reinterpret_cast<const float4 *>(src)[2 * c + 1];
+                x[0] = v0.x; x[1] = v0.y; x[2] = v0.z; x[3] = v0.w; x[4] = v1.x; x[5] = v1.y; x[6] = v1.z; x[7] = v1.w;
+            }
+            unsigned h[4], l[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) kv4_pieces(kv4_scale2(x[i], k), kv4_scale2(x[i + 4], k), h[i], l[i]);
+            uint8_t *dst = sm + (c >> 3) * (PT_M * 128) + line * 128 + (((c & 7) ^ (line & 7)) << 4);
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(dst + L::Q) = make_uint4(l[0], l[1], l[2], l[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = sh.tmem;
+    const int n = sh.n;
+    volatile int *abort_flag = &sh.abort;
+
+    if (warp == 12) {
+        // ---- the products ----
+        if (lane == 0) {
+            const uint32_t id_s = (1u << 4) | (64u >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
+            const uint32_t id_o = (1u << 4) | ((uint32_t)HD >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
+            const uint32_t q0 = smem_u32(sm), k0 = q0 + L::OFF_K, v0 = q0 + L::OFF_V;
+            bool ok = true;
+            auto pv = [&](int j) {                           // O of page j
+                const int b = j & 1;
+                ok = ok && pt_wait(&sh.vfull[b], j >> 1 & 1, abort_flag) && pt_wait(&sh.pfull[b], j >> 1 & 1, abort_flag) &&
+                     pt_wait(&sh.oempty[b], (j >> 1 & 1) ^ 1, abort_flag);
+                if (!ok) return;
+                tc_after();
+                const uint32_t d = tmem + TM_O + b * 128, p = tmem + TM_P + b * 64;
+#pragma unroll
+                for (int term = 0; term < 3; term++)         // p lo * v hi, p hi * v lo, p hi * v hi
+#pragma unroll
+                    for (int s = 0; s < 4; s++)
+                        umma_ts(d, p + (term == 0 ? 32 : 0) + s * 8, umma_desc(v0 + (2 * b + (term == 1)) * L::V + s * 32), id_o, (term | s) != 0);
+                umma_commit(&sh.pvdone[b]);
+            };
+            for (int j = 0; j < n && ok; j++) {
+                const int b = j & 1;
+                ok = pt_wait(&sh.kfull[b], j >> 1 & 1, abort_flag) && pt_wait(&sh.sempty[b], (j >> 1 & 1) ^ 1, abort_flag);
+                if (!ok) break;
+                tc_after();
+                const uint32_t d = tmem + TM_S + b * 64;
+#pragma unroll
+                for (int term = 0; term < 3; term++)         // q lo * k hi, q hi * k lo, q hi * k hi
+#pragma unroll
+                    for (int s = 0; s < 2 * NG; s++)
+                        umma_ss(d, umma_desc(q0 + (term == 0 ? L::Q : 0) + (s >> 2) * (PT_M * 128) + (s & 3) * 32),
+                                umma_desc(k0 + (2 * b + (term == 1)) * L::K + (s >> 2) * (64 * 128) + (s & 3) * 32), id_s, (term | s) != 0);
+                umma_commit(&sh.sfull[b]);
+                if (j > 0) pv(j - 1);
+            }
+            if (n > 0 && ok) pv(n - 1);
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // ---- pages into shared memory, then as operand tiles ----
+        // (registers: 416 threads x 128 at launch = 256 x 152 softmax + 128 x 80 staging + 32 x 128)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_STAGE));
+        const int w = tid - 256;
+        const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
+        const size_t page_bytes = kv4_page_bytes(a.geo);
+        auto stage = [&](int j) {
+            if (j < n) {
+                const uint8_t *src = base + (size_t)list[j].x * page_bytes;
+                uint8_t *dst = sm + L::OFF_RAW + (j & 1) * L::RAW;
+                for (int c = w; c < 64 * NG; c += 128) {     // rows of NG pieces; halves of 8 NG pieces
+                    cp_async16(dst + (c / NG) * L::KS + (c % NG) * 16, src + c * 16);
+                    cp_async16(dst + L::RK + (c / (8 * NG)) * L::VS + (c % (8 * NG)) * 16, src + kv4_v_code_off(HD) + c * 16);
+                }
+                if (w < 16 * NG)
+                    cp_async16(dst + L::RK + L::RV + w * 16, src + (w < 8 * NG ? kv4_k_step_off(HD) + w * 16 : kv4_v_step_off(HD) + (w - 8 * NG) * 16));
+            }
+            cp_async_commit();
+        };
+        stage(0); stage(1);
+        bool ok = true;
+        for (int j = 0; j < n; j++) {
+            const int b = j & 1, t0 = list[j].y;
+            uint8_t *raw = sm + L::OFF_RAW + b * L::RAW;
+            const uint16_t *kst = reinterpret_cast<const uint16_t *>(raw + L::RK + L::RV), *vst = kst + 64 * NG;
+            cp_async_wait<1>();
+            if (w == 0) sh.big = 0;
+            if (w < NG) sh.nan[j & 7][w] = 0ull;
+            if (w == 4) sh.anynan[j & 7] = 0;
+            stager_sync();                                   // the page is here for all
+            // steps: positions that no line sees become 0 (their memory may hold anything); NaN and overflow are looked for
+            for (int i = w; i < 64 * NG; i += 128) {
+                const int t = i / NG, g = i - t * NG;
+                uint16_t ks = kst[i], vs = vst[i];
+                if (t0 + t < cr.lo_any || t0 + t >= cr.hi_any) ks = vs = 0;
+                if ((ks & 0x7fff) >= 0x6c00 && (ks & 0x7fff) < 0x7c00) atomicOr(&sh.big, 1);
+                if ((vs & 0x7fff) >= 0x6c00 && (vs & 0x7fff) < 0x7c00) atomicOr(&sh.big, 2);
+                if ((vs & 0x7fff) >= 0x7c00) {
+                    atomicOr(&sh.nan[j & 7][g], 1ull << t);
+                    sh.anynan[j & 7] = 1;
+                    vs = 0;
+                }
+                const_cast<uint16_t *>(kst)[i] = ks;
+                const_cast<uint16_t *>(vst)[i] = vs;
+            }
+            stager_sync();
+            const int big = sh.big;
+            const __half2 down = __half2half2(__ushort_as_half(0x2c00));     // 1 / 16
+            if (w == 0) { sh.fk[j & 7] = big & 1 ? 16.f : 1.f; sh.fv[j & 7] = big & 2 ? 16.f : 1.f; }
+            if (j > 1) ok = warp_wait(&sh.sfull[b], (j - 2) >> 1 & 1, abort_flag);                       // the keys of page j - 2 are done with
+            if (ok) {
+#pragma unroll
+            for (int it = 0; it < 2; it++) {
+                const int jj = w >> 3 & 3, t = ((w >> 5) + 4 * it) * 8 + (w & 7);
+                unsigned kw[NG];
+                kv4_ldsw<NG>(kw, raw + t * L::KS + jj * (4 * NG));
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    __half2 d = __half2half2(__ushort_as_half(kst[t * NG + g]));
+                    if (big & 1) d = __hmul2(d, down);
+                    unsigned h[4], l[4];
+                    kv4_values_hl(kw[g], d, h, l);
+                    const int c = 4 * g + jj;
+                    uint8_t *dst = sm + L::OFF_K + 2 * b * L::K + (c >> 3) * (64 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(dst + L::K) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&sh.kfull[b]);
+            }
+            if (ok && j > 1) ok = warp_wait(&sh.pvdone[b], (j - 2) >> 1 & 1, abort_flag);                // the values of page j - 2 are done with
+            if (ok) {
+                const int o = w & 7, r = w >> 3 & 7;         // eight positions 8 o .., dims 32 g + 4 r + 0 .. 3
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    if ((g & 1) != w >> 6) continue;
+                    unsigned h[4][4], l[4][4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {            // positions 8 o + 2 q, + 1
+                        const unsigned vw = *reinterpret_cast<const unsigned *>(raw + L::RK + o * L::VS + (r * 4 + q) * (4 * NG) + 4 * g);
+                        const int t = 8 * o + 2 * q;
+                        __half2 d = __halves2half2(__ushort_as_half(vst[t * NG + g]), __ushort_as_half(vst[(t + 1) * NG + g]));
+                        if (big & 2) d = __hmul2(d, down);
+                        unsigned hh[4], ll[4];
+                        kv4_values_hl(vw, d, hh, ll);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) { h[i][q] = hh[i]; l[i][q] = ll[i]; }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int dim = 32 * g + 4 * r + i;
+                        uint8_t *dst = sm + L::OFF_V + 2 * b * L::V + dim * 128 + ((o ^ (dim & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[i][0], h[i][1], h[i][2], h[i][3]);
+                        *reinterpret_cast<uint4 *>(dst + L::V) = make_uint4(l[i][0], l[i][1], l[i][2], l[i][3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&sh.vfull[b]);
+            }
+            if (!stager_and(ok)) break;                      // everyone has read the stage
+            stage(j + 2);
+        }
+        cp_async_wait<0>();
+    } else {
+        // ---- softmax: two threads a line ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFT));
+        constexpr int HO = HD / 2;                           // dims of this thread: half * HO ..
+        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+        float m = -INFINITY, l = 0.f, o[HO];
+        unsigned nanbits = 0;
+#pragma unroll
+        for (int i = 0; i < HO; i++) o[i] = 0.f;
+        float pf = 1.f;                                      // what the O of the page before is still to be multiplied by
+        bool ok = true;
+        auto add_o = [&](int j) {                            // O of page j to the registers
+            const int b = j & 1;
+            ok = ok && warp_wait(&sh.pvdone[b], j >> 1 & 1, abort_flag);
+            if (!ok) return;
+            tc_after();
+            const float f = pf * sh.fv[j & 7];
+            const uint32_t at = mine + TM_O + b * 128 + half * HO;
+#pragma unroll
+            for (int c = 0; c < HO; c += 32) {
+                uint32_t v[16], w[16];
+                tm_ld16(v, at + c);
+                if (c + 16 < HO) tm_ld16(w, at + c + 16);
+                tm_wait();
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[c + i] = fmaf(__uint_as_float(v[i]), f, o[c + i]);
+                if (c + 16 < HO)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[c + 16 + i] = fmaf(__uint_as_float(w[i]), f, o[c + 16 + i]);
+            }
+            tc_before();
+            mbar_arrive(&sh.oempty[b]);
+            if (sh.anynan[j & 7]) {
+                const int t0 = list[j].y;
+                for (int g = 0; g < NG; g++)
+                    for (unsigned long long mk = sh.nan[j & 7][g]; mk; mk &= mk - 1) {
+                        const int t = t0 + __ffsll((long long)mk) - 1;
+                        if (t >= clo && t <= chi) nanbits |= 1u << g;
+                    }
+                __syncwarp();
+            }
+        };
+        for (int j = 0; j < n; j++) {
+            const int b = j & 1, t0 = list[j].y + half * 32;
+            ok = ok && warp_wait(&sh.sfull[b], j >> 1 & 1, abort_flag);
+            float v[32], mx = -INFINITY, ds = 0.f;
+            if (ok) {
+                tc_after();
+                ds = desc * sh.fk[j & 7];
+                tm_ld32(v, mine + TM_S + b * 64 + half * 32);
+                if (!(t0 >= cr.lo_all && t0 + 32 <= cr.hi_all)) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) if (t0 + i < clo || t0 + i > chi) v[i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i++) mx = fmaxf(mx, v[i]);
+                sh.mx[b][half][line] = mx;
+            }
+            ok = pair_and(quarter, ok);
+            if (!ok) break;
+            mx = fmaxf(mx, sh.mx[b][half ^ 1][line]) * ds;   // (the scale is positive)
+            float f = 1.f;
+            const bool up = mx > m + 8.f;
+            if (__any_sync(0xffffffffu, up)) {
+                if (up) { f = kv4_exp2(m - mx); m = mx; }
+                __syncwarp();
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < HO; i++) o[i] *= f;
+            }
+            // weights times 2^6, as hi and lo pairs of consecutive positions (a line that has seen nothing yet: all 0)
+            const float mm = m == -INFINITY ? 0.f : m - 6.f;
+            unsigned ph[16], pl[16];
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float p0 = kv4_exp2(fmaf(v[2 * i], ds, -mm)), p1 = kv4_exp2(fmaf(v[2 * i + 1], ds, -mm));
+                s0 += p0; s1 += p1;
+                kv4_pieces(p0, p1, ph[i], pl[i]);
+            }
+            l += s0 + s1;
+            tm_st16(mine + TM_P + b * 64 + half * 16, ph);
+            tm_st16(mine + TM_P + b * 64 + 32 + half * 16, pl);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_before();
+            mbar_arrive(&sh.pfull[b]);
+            mbar_arrive(&sh.sempty[b]);
+            pf = f;
+            if (j > 0) add_o(j - 1);
+        }
+        pf = 1.f;
+        if (n > 0 && ok) add_o(n - 1);
+        sh.mx[n & 1][half][line] = l;
+        ok = pair_and(quarter, ok);
+        l += sh.mx[n & 1][half ^ 1][line];
+        if (ok && line < ncol) {
+            float *out = nsplit == 1 ? a.ctx + rh * HD : part + (rh * nsplit + split) * (HD + 4) + 4;
+            if (nsplit > 1 && half == 0) { out[-4] = m; out[-3] = l; }
+            const float qnan = __int_as_float(0x7fffffff);
+#pragma unroll
+            for (int c = 0; c < HO; c += 4) {
+                float4 v = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                if (nsplit == 1)
+                    v = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__fdiv_rn(v.x, l), __fdiv_rn(v.y, l), __fdiv_rn(v.z, l), __fdiv_rn(v.w, l));
+                if (nanbits >> ((half * HO + c) >> 5) & 1) v = make_float4(qnan, qnan, qnan, qnan);
+                *reinterpret_cast<float4 *>(out + half * HO + c) = v;
+            }
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (sh.abort) {                                          // products still on their way are given time before their memory goes
+        if (tid == 0) atomicExch(err_wait, 1);
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+template <int NG>
+int go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *err_wait, cudaStream_t st) {
+    static bool attr[MOTY_MAX_DEV];
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= MOTY_MAX_DEV) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: device %d", dev);
+    if (!attr[dev]) {
+        CK(cudaFuncSetAttribute(kv4_prompt_tc_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PtL<NG>::SMEM));
+        // the register shares of the roles (setmaxnreg) add up to what the threads are launched with
+        cudaFuncAttributes fa;
+        CK(cudaFuncGetAttributes(&fa, kv4_prompt_tc_kernel<NG>));
+        if (fa.numRegs != PT_REGS) return moty_set_error(MOTY_CUDA_ECUDA, "kv4_attend: prompt kernel built with %d registers, not %d", fa.numRegs, PT_REGS);
+        attr[dev] = true;
+    }
+    const long long grid = (long long)a.b.nseq * a.geo.KV * p.ntile * p.nsplit;
+    if (grid > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend: %lld CTAs", grid);
+    CK(moty_launch_pdl(kv4_prompt_tc_kernel<NG>, dim3((unsigned)grid), dim3(PT_T), (size_t)PtL<NG>::SMEM, st, a, p.ntile, p.nsplit, p.span, part, err_wait));
+    return 0;
+}
+
+}  // namespace
+
+int launch_kv4_prompt_tc(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st) {
+    int *err_wait = a.err - 4;                               // the library's error words: [0] tensor-core pipeline waits, [4] this cache's batches
+    switch (a.geo.hd / 32) {
+        case 2: return go<2>(a, p, part, err_wait, st);
+        case 3: return go<3>(a, p, part, err_wait, st);
+        default: return go<4>(a, p, part, err_wait, st);
+    }
+}
