@@ -1,7 +1,7 @@
 // kv4_prompt_tc.cu -- attention over the paged 4-bit KV cache for prompts, on the 5th-generation tensor cores.
 //
-// A CTA takes 128 lines ((row, query head) pairs of one KV head of one sequence) and walks the pages of its span, 64
-// positions a step:
+// A CTA takes 256 lines ((row, query head) pairs of one KV head of one sequence) as two tiles of 128 that share a page's
+// operand tiles, and walks the pages of its span, 64 positions a step:
 //     S = Q K^T   [128 x 64]     three products: q lo * k hi, q hi * k lo, q hi * k hi
 //     O = P V     [128 x hd]     three products: p lo * v hi, p hi * v lo, p hi * v hi
 // f32 accuracy from f16 operands: an operand is hi + lo, f16 each.  A value held is code * step, 4 x 11 bits, so k and v are
@@ -9,15 +9,16 @@
 // the softmax weights carry 22 bits; the dropped lo * lo term is 2^-22 of a product.  Steps of 4096 and more would overflow
 // f16: a page that has one is brought down by 2^4.  O starts from zero at every page and is added to f32 registers, because
 // the tensor core's own sum drifts over a long prompt.
-//   warps 0-7   softmax, two threads a line (half the positions, half the dims each): S from TMEM, running maximum (moved when
-//               passed by 8 in base-2 units), weights back to TMEM as the A operand of the second product, then the O of the
-//               page before added to the registers
-//   warps 8-11  a page's codes and steps into shared memory (two pages ahead), then as k and v^T operand tiles (K-major,
+//   warps 0-3, 4-7   softmax of a tile, a thread a line: S from TMEM, running maximum (moved when passed by 8 in base-2
+//               units), weights back to TMEM over the scores as the A operand of the second product, then the O of the page
+//               before added to the registers
+//   warps 8-10  a page's codes and steps into shared memory (two pages ahead), then as k and v^T operand tiles (K-major,
 //               128-byte swizzle): eight key dims of a position, or eight positions of a value dim, are one 16-byte piece
-//   warp 12     issues the products: S of page j + 1 before O of page j, so that the softmax of a page runs behind two
-//               products
-// Everything between the roles is a double buffer (all 512 TMEM columns).  What bounds it: the six products, 1536
-// cycles of tensor core a page at hd = 128.  Every wait is bounded; on expiry all roles leave and the error word is set.
+//   warp 11     issues the products: both S of page j + 1, then both O of page j, so that a tile's softmax of a page has the
+//               time of three products, and each operand tile is rebuilt during the two products that do not read it
+// TMEM (512 columns): scores / weights two buffers a tile, O one a tile.  What bounds it: the twelve products of a page and
+// two tiles, 3072 cycles of tensor core at hd = 128; with one tile a CTA the staging alone took longer than its products
+// (6400 cycles a page).  Every wait is bounded; on expiry all roles leave and the error word is set.
 // An infinity or NaN of a key makes its scores NaN; a NaN step of a value is taken out of the product (a weight of 0 would
 // spread it to lines that do not see it) and set in the result of the lines that do.
 #include "kv4_frag.cuh"
@@ -26,9 +27,10 @@
 
 namespace {
 
-constexpr int PT_M = KV4_TC_LINES, PT_NP = KV4_TC_PAGES, PT_T = 416, PT_REGS = 128, PT_REGS_SOFT = 152, PT_REGS_STAGE = 80;
-static_assert(256 * PT_REGS_SOFT + 128 * PT_REGS_STAGE + 32 * PT_REGS <= PT_T * PT_REGS, "register shares");
-constexpr uint32_t TM_S = 0, TM_P = 128, TM_O = 256;         // TMEM columns: S 2 x 64, P 2 x (32 hi + 32 lo), O 2 x 128
+constexpr int PT_M = 128, PT_NP = KV4_TC_PAGES, PT_T = 384, PT_ST = 96;      // lines a tile, pages a span, threads, staging threads
+constexpr int PT_REGS = 168, PT_REGS_SOFT = 208, PT_REGS_REST = 80;
+static_assert(KV4_TC_LINES == 2 * PT_M && 256 * PT_REGS_SOFT + 128 * PT_REGS_REST <= PT_T * PT_REGS, "lines; register shares");
+constexpr uint32_t TM_S = 0, TM_O = 256;                     // TMEM columns: scores / weights [tile][page & 1] x 64, O [tile] x 128
 
 template <int NG> struct PtL {
     static constexpr int HD = NG * 32, NSUB = (NG + 1) / 2;
@@ -36,32 +38,42 @@ template <int NG> struct PtL {
     static constexpr int VS = 4 * HD + 16;                   // bytes between staged value halves (eight positions)
     static constexpr int RK = 64 * KS, RV = 8 * VS, RST = 128 * NG, RAW = RK + RV + 2 * RST;
     static constexpr int Q = NSUB * PT_M * 128, K = NSUB * 64 * 128, V = HD * 128;      // one piece (hi or lo) of an operand
-    static constexpr int OFF_K = 2 * Q, OFF_V = OFF_K + 4 * K, OFF_RAW = OFF_V + 4 * V, OFF_LIST = OFF_RAW + 2 * RAW;
+    static constexpr int OFF_K = 4 * Q, OFF_V = OFF_K + 2 * K, OFF_RAW = OFF_V + 2 * V, OFF_LIST = OFF_RAW + 2 * RAW;
     static constexpr int SMEM = OFF_LIST + PT_NP * 8 + 1024;
 };
 
 struct PtShared {
-    uint64_t kfull[2], vfull[2], sfull[2], sempty[2], pfull[2], pvdone[2], oempty[2];
+    uint64_t kfull, vfull, sfull[2][2], pfull[2][2], pvdone[2], oempty[2];   // [tile][page & 1]; the others one phase a page
     uint32_t tmem;
     int abort, n;
-    float fk[8], fv[8];                                      // by page (the staging warps are up to five pages ahead of the last reader): what scores and outputs are to be multiplied by
+    float fk[8], fv[8];                                      // by page (the staging warps run ahead): what scores and outputs are to be multiplied by
     unsigned long long nan[8][4];                            // by page and group: positions whose value step is NaN
     int anynan[8];
-    float mx[2][2][PT_M];                                    // by page, half: a line's largest score; at the end a line's sum of weights
     int big;                                                 // a step of the staged page that would overflow: bit 0 keys, bit 1 values
 };
 
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// D [tmem] (+)= A * B^T, f16 in, f32 sums; A from shared memory or from TMEM
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+// D [tmem] (+)= A * B^T, f16 in, f32 sums; A from shared memory or from TMEM.  The whole warp runs the issuing code with
+// uniform values and one lane issues (`lead`), so that addresses and descriptors stay in uniform registers: formed by a
+// single lane they took 75 cycles a product.  A descriptor is its constant high word and an address word.
+constexpr uint32_t DESC_HI = (uint32_t)(1024 >> 4) | 1u << 14 | 2u << 29;     // umma_desc's upper half: rows of 8 x 128 bytes, version 1, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr) { return (saddr >> 4 & 0x3fffu) | 1u << 16; }
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "mov.b64 x, {%1, %6};\n\tmov.b64 y, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "r"(DESC_HI) : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "mov.b64 y, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "r"(DESC_HI) : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
 }
 // 32 columns of this warp's 32 lanes
 __device__ __forceinline__ void tm_ld32(float (&v)[32], uint32_t addr) {
@@ -76,16 +88,9 @@ __device__ __forceinline__ void tm_ld32(float (&v)[32], uint32_t addr) {
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tm_ld16(uint32_t (&r)[16], uint32_t addr) {                  // (tm_wait before the registers are used)
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void tm_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tm_st16(uint32_t addr, const unsigned (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-                   "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+__device__ __forceinline__ void tm_st8(uint32_t addr, const unsigned (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -99,19 +104,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     const bool ok = pt_wait(bar, parity, abort_flag);
     return __all_sync(0xffffffffu, ok);
 }
-// the two warps of a line quarter: one reads what the other wrote; both go on, or leave, together
-__device__ __forceinline__ bool pair_and(int quarter, bool ok) {
-    int all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, %2, 64, q;\n\tselp.s32 %0, 1, 0, p;\n\t}"
-                 : "=r"(all) : "r"((int)ok), "r"(2 + quarter) : "memory");
-    return all != 0;
-}
-__device__ __forceinline__ void stager_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-// the same, and whether all 128 threads say yes: they go on, or leave, together
+__device__ __forceinline__ void stager_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PT_ST) : "memory"); }
+// the same, and whether all of them say yes: they go on, or leave, together
 __device__ __forceinline__ bool stager_and(bool ok) {
     int all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, 1, 128, q;\n\tselp.s32 %0, 1, 0, p;\n\t}"
-                 : "=r"(all) : "r"((int)ok) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, 1, %2, q;\n\tselp.s32 %0, 1, 0, p;\n\t}"
+                 : "=r"(all) : "r"((int)ok), "n"(PT_ST) : "memory");
     return all != 0;
 }
 
@@ -145,9 +143,9 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         if (nsplit == 1 && tile == 0) kv4_zero_rows(a, sq, head);
         return;
     }
-    const long long lines = (long long)sq.n * a.G, c0 = (long long)tile * PT_M;
+    const long long lines = (long long)sq.n * a.G, c0 = (long long)tile * KV4_TC_LINES;
     if (c0 >= lines) return;
-    const int ncol = lines - c0 < PT_M ? (int)(lines - c0) : PT_M;
+    const int ncol = lines - c0 < KV4_TC_LINES ? (int)(lines - c0) : KV4_TC_LINES, nx = ncol > PT_M ? 2 : 1;      // lines, tiles
     const int pos0 = sq.len - sq.n;
     const Kv4Range cr = kv4_range(a, pos0 + (int)(c0 / a.G), pos0 + (int)((c0 + ncol - 1) / a.G));
     const int t_lo = (cr.lo_any & ~(KV4_PAGE - 1)) + split * span, t_hi = cr.hi_any - t_lo < span ? cr.hi_any : t_lo + span;
@@ -155,15 +153,15 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
 
     if (tid == 0) {
         sh.abort = 0;
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.kfull[i], 128); mbar_init(&sh.vfull[i], 128);
-            mbar_init(&sh.sfull[i], 1); mbar_init(&sh.sempty[i], 256); mbar_init(&sh.pfull[i], 256); mbar_init(&sh.pvdone[i], 1);
-            mbar_init(&sh.oempty[i], 256);
+        mbar_init(&sh.kfull, PT_ST); mbar_init(&sh.vfull, PT_ST);
+        for (int x = 0; x < 2; x++) {
+            for (int i = 0; i < 2; i++) { mbar_init(&sh.sfull[x][i], 1); mbar_init(&sh.pfull[x][i], PT_M); }
+            mbar_init(&sh.pvdone[x], 1); mbar_init(&sh.oempty[x], PT_M);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 11) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -185,12 +183,12 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
     float desc = 0.f;
     int clo = 0, chi = 0x7fffffff;                           // (lines that are not there see everything, and are not written)
     size_t rh = 0;
-    const int quarter = warp & 3, half = warp >> 2, line = quarter * 32 + lane;
-    if (warp < 8) {
-        const bool have = line < ncol;
+    const int x = warp >> 2;                                 // the tile of a softmax warp
+    if (x < nx) {
+        const bool have = tid < ncol;
         const float *src = a.q;
         if (have) {
-            const long long cc = c0 + line;
+            const long long cc = c0 + tid;
             const int row = (int)(cc / a.G), g0 = (int)(cc - (long long)row * a.G), p = pos0 + row;
             src = a.q + (size_t)(sq.r0 + row) * a.q_ld + (size_t)(head * a.G + g0) * HD;
             rh = (size_t)(sq.r0 + row) * a.H + head * a.G + g0;
@@ -209,18 +207,18 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         // (not below the smallest normal number: -infinity times it has to stay -infinity)
         desc = fin ? fmaxf(kv4_scale2(a.scale * 1.44269504f, -k), 1.17549435e-38f) : __int_as_float(0x7fffffff);
 #pragma unroll 2
-        for (int c = half * 2 * NG; c < (half + 1) * 2 * NG; c++) {                   // piece c = 4 g + j: dims 8 c + 0, 4, 1, 5, 2, 6, 3, 7 (the order of a code word's pairs)
-            float x[8];
+        for (int c = 0; c < NG * 4; c++) {                   // piece c = 4 g + j: dims 8 c + 0, 4, 1, 5, 2, 6, 3, 7 (the order of a code word's pairs)
+            float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.f;
+            for (int i = 0; i < 8; i++) y[i] = 0.f;
             if (have && fin) {
                 const float4 v0 = reinterpret_cast<const float4 *>(src)[2 * c], v1 = reinterpret_cast<const float4 *>(src)[2 * c + 1];
-                x[0] = v0.x; x[1] = v0.y; x[2] = v0.z; x[3] = v0.w; x[4] = v1.x; x[5] = v1.y; x[6] = v1.z; x[7] = v1.w;
+                y[0] = v0.x; y[1] = v0.y; y[2] = v0.z; y[3] = v0.w; y[4] = v1.x; y[5] = v1.y; y[6] = v1.z; y[7] = v1.w;
             }
             unsigned h[4], l[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) kv4_pieces(kv4_scale2(x[i], k), kv4_scale2(x[i + 4], k), h[i], l[i]);
-            uint8_t *dst = sm + (c >> 3) * (PT_M * 128) + line * 128 + (((c & 7) ^ (line & 7)) << 4);
+            for (int i = 0; i < 4; i++) kv4_pieces(kv4_scale2(y[i], k), kv4_scale2(y[i + 4], k), h[i], l[i]);
+            uint8_t *dst = sm + 2 * x * L::Q + (c >> 3) * (PT_M * 128) + (tid & 127) * 128 + (((c & 7) ^ (tid & 7)) << 4);
             *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4 *>(dst + L::Q) = make_uint4(l[0], l[1], l[2], l[3]);
         }
@@ -233,256 +231,287 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
     const int n = sh.n;
     volatile int *abort_flag = &sh.abort;
 
-    if (warp == 12) {
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_REST));      // (384 x 168 at launch)
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFT));
+    if (warp == 11) {
         // ---- the products ----
-        if (lane == 0) {
-            const uint32_t id_s = (1u << 4) | (64u >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
-            const uint32_t id_o = (1u << 4) | ((uint32_t)HD >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
-            const uint32_t q0 = smem_u32(sm), k0 = q0 + L::OFF_K, v0 = q0 + L::OFF_V;
-            bool ok = true;
-            auto pv = [&](int j) {                           // O of page j
-                const int b = j & 1;
-                ok = ok && pt_wait(&sh.vfull[b], j >> 1 & 1, abort_flag) && pt_wait(&sh.pfull[b], j >> 1 & 1, abort_flag) &&
-                     pt_wait(&sh.oempty[b], (j >> 1 & 1) ^ 1, abort_flag);
-                if (!ok) return;
-                tc_after();
-                const uint32_t d = tmem + TM_O + b * 128, p = tmem + TM_P + b * 64;
-#pragma unroll
-                for (int term = 0; term < 3; term++)         // p lo * v hi, p hi * v lo, p hi * v hi
-#pragma unroll
-                    for (int s = 0; s < 4; s++)
-                        umma_ts(d, p + (term == 0 ? 32 : 0) + s * 8, umma_desc(v0 + (2 * b + (term == 1)) * L::V + s * 32), id_o, (term | s) != 0);
-                umma_commit(&sh.pvdone[b]);
-            };
-            for (int j = 0; j < n && ok; j++) {
-                const int b = j & 1;
-                ok = pt_wait(&sh.kfull[b], j >> 1 & 1, abort_flag) && pt_wait(&sh.sempty[b], (j >> 1 & 1) ^ 1, abort_flag);
+        const uint32_t id_s = (1u << 4) | (64u >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
+        const uint32_t id_o = (1u << 4) | ((uint32_t)HD >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
+        const uint32_t q0 = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t dq = desc_lo(q0), dk = desc_lo(q0 + L::OFF_K), dv = desc_lo(q0 + L::OFF_V);     // (offsets below do not leave 14 bits)
+        const uint32_t lead = elect_one();
+        bool ok = true;
+        for (int j = 0; j <= n && ok; j++) {
+            if (j < n) {                                     // S of page j (its buffer: the O of page j - 2 was issued before)
+                ok = warp_wait(&sh.kfull, j & 1, abort_flag);
                 if (!ok) break;
                 tc_after();
-                const uint32_t d = tmem + TM_S + b * 64;
+#pragma unroll 1
+                for (int y = 0; y < nx; y++) {
+                    const uint32_t d = tm + TM_S + (y * 2 + (j & 1)) * 64, q = dq + y * (2 * L::Q >> 4);
 #pragma unroll
-                for (int term = 0; term < 3; term++)         // q lo * k hi, q hi * k lo, q hi * k hi
+                    for (int term = 0; term < 3; term++)     // q lo * k hi, q hi * k lo, q hi * k hi
 #pragma unroll
-                    for (int s = 0; s < 2 * NG; s++)
-                        umma_ss(d, umma_desc(q0 + (term == 0 ? L::Q : 0) + (s >> 2) * (PT_M * 128) + (s & 3) * 32),
-                                umma_desc(k0 + (2 * b + (term == 1)) * L::K + (s >> 2) * (64 * 128) + (s & 3) * 32), id_s, (term | s) != 0);
-                umma_commit(&sh.sfull[b]);
-                if (j > 0) pv(j - 1);
+                        for (int s = 0; s < 2 * NG; s++)
+                            umma_ss(d, q + (((term == 0 ? L::Q : 0) + (s >> 2) * (PT_M * 128) + (s & 3) * 32) >> 4),
+                                    dk + (((term == 1 ? L::K : 0) + (s >> 2) * (64 * 128) + (s & 3) * 32) >> 4), id_s, (term | s) != 0, lead);
+                    if (lead) umma_commit(&sh.sfull[y][j & 1]);
+                    __syncwarp();
+                }
             }
-            if (n > 0 && ok) pv(n - 1);
+            if (j > 0) {                                     // O of page j - 1
+                const int i = j - 1;
+                ok = warp_wait(&sh.vfull, i & 1, abort_flag);
+#pragma unroll 1
+                for (int y = 0; y < nx && ok; y++) {
+                    ok = warp_wait(&sh.pfull[y][i & 1], i >> 1 & 1, abort_flag) && warp_wait(&sh.oempty[y], (i & 1) ^ 1, abort_flag);
+                    if (!ok) break;
+                    tc_after();
+                    const uint32_t d = tm + TM_O + y * 128, p = tm + TM_S + (y * 2 + (i & 1)) * 64;
+#pragma unroll
+                    for (int term = 0; term < 3; term++)     // p lo * v hi, p hi * v lo, p hi * v hi
+#pragma unroll
+                        for (int s = 0; s < 4; s++)
+                            umma_ts(d, p + (s >> 1) * 32 + (s & 1) * 8 + (term == 0 ? 16 : 0), dv + (((term == 1 ? L::V : 0) + s * 32) >> 4), id_o,
+                                    (term | s) != 0, lead);
+                    if (lead) umma_commit(&sh.pvdone[y]);
+                    __syncwarp();
+                }
+            }
         }
-        __syncwarp();
     } else if (warp >= 8) {
         // ---- pages into shared memory, then as operand tiles ----
-        // (registers: 416 threads x 128 at launch = 256 x 152 softmax + 128 x 80 staging + 32 x 128)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_STAGE));
         const int w = tid - 256;
         const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
         const size_t page_bytes = kv4_page_bytes(a.geo);
-        auto stage = [&](int j) {
+        // keys of a page are taken one page before its values: K of page j + 1 while the O of page j - 1 is formed, V of page j
+        // while the S of page j + 1 is
+        auto stage = [&](int j, bool keys) {
             if (j < n) {
-                const uint8_t *src = base + (size_t)list[j].x * page_bytes;
-                uint8_t *dst = sm + L::OFF_RAW + (j & 1) * L::RAW;
-                for (int c = w; c < 64 * NG; c += 128) {     // rows of NG pieces; halves of 8 NG pieces
-                    cp_async16(dst + (c / NG) * L::KS + (c % NG) * 16, src + c * 16);
-                    cp_async16(dst + L::RK + (c / (8 * NG)) * L::VS + (c % (8 * NG)) * 16, src + kv4_v_code_off(HD) + c * 16);
-                }
-                if (w < 16 * NG)
-                    cp_async16(dst + L::RK + L::RV + w * 16, src + (w < 8 * NG ? kv4_k_step_off(HD) + w * 16 : kv4_v_step_off(HD) + (w - 8 * NG) * 16));
+                const uint8_t *src = base + (size_t)list[j].x * page_bytes + (keys ? 0 : kv4_v_code_off(HD));
+                uint8_t *dst = sm + L::OFF_RAW + (j & 1) * L::RAW + (keys ? 0 : L::RK + L::RST);
+                for (int c = w; c < 72 * NG; c += PT_ST)     // rows of NG pieces (keys), halves of 8 NG (values), then the steps
+                    cp_async16(dst + (c >= 64 * NG ? (keys ? L::RK : L::RV) + (c - 64 * NG) * 16
+                                      : keys ? (c / NG) * L::KS + (c % NG) * 16 : (c / (8 * NG)) * L::VS + (c % (8 * NG)) * 16), src + c * 16);
             }
             cp_async_commit();
         };
-        stage(0); stage(1);
-        bool ok = true;
-        for (int j = 0; j < n; j++) {
-            const int b = j & 1, t0 = list[j].y;
-            uint8_t *raw = sm + L::OFF_RAW + b * L::RAW;
-            const uint16_t *kst = reinterpret_cast<const uint16_t *>(raw + L::RK + L::RV), *vst = kst + 64 * NG;
-            cp_async_wait<1>();
+        // steps of a staged part: positions that no line sees become 0 (their memory may hold anything), steps that would
+        // overflow and NaN steps of values are noted; all of it rare, and looked for two steps at a time
+        auto look = [&](int j, bool keys) {
+            uint32_t *st = reinterpret_cast<uint32_t *>(sm + L::OFF_RAW + (j & 1) * L::RAW + (keys ? L::RK : L::RK + L::RST + L::RV));
+            const int t0 = list[j].y;
+            bool odd = t0 < cr.lo_any || t0 + KV4_PAGE > cr.hi_any;
+            for (int i = w; i < 32 * NG; i += PT_ST) odd |= (((st[i] & 0x7fff7fffu) + 0x14001400u) & 0x80008000u) != 0;      // |step| >= 4096, infinity, NaN
+            if (stager_and(!odd)) return 1.f;
             if (w == 0) sh.big = 0;
-            if (w < NG) sh.nan[j & 7][w] = 0ull;
-            if (w == 4) sh.anynan[j & 7] = 0;
-            stager_sync();                                   // the page is here for all
-            // steps: positions that no line sees become 0 (their memory may hold anything); NaN and overflow are looked for
-            for (int i = w; i < 64 * NG; i += 128) {
+            stager_sync();
+            uint16_t *h = reinterpret_cast<uint16_t *>(st);
+            for (int i = w; i < 64 * NG; i += PT_ST) {
                 const int t = i / NG, g = i - t * NG;
-                uint16_t ks = kst[i], vs = vst[i];
-                if (t0 + t < cr.lo_any || t0 + t >= cr.hi_any) ks = vs = 0;
-                if ((ks & 0x7fff) >= 0x6c00 && (ks & 0x7fff) < 0x7c00) atomicOr(&sh.big, 1);
-                if ((vs & 0x7fff) >= 0x6c00 && (vs & 0x7fff) < 0x7c00) atomicOr(&sh.big, 2);
-                if ((vs & 0x7fff) >= 0x7c00) {
-                    atomicOr(&sh.nan[j & 7][g], 1ull << t);
-                    sh.anynan[j & 7] = 1;
-                    vs = 0;
-                }
-                const_cast<uint16_t *>(kst)[i] = ks;
-                const_cast<uint16_t *>(vst)[i] = vs;
+                uint16_t v = h[i];
+                if (t0 + t < cr.lo_any || t0 + t >= cr.hi_any) v = 0;
+                if ((v & 0x7fff) >= 0x7c00) {
+                    if (!keys) { atomicOr(&sh.nan[j & 7][g], 1ull << t); sh.anynan[j & 7] = 1; v = 0; }
+                } else if ((v & 0x7fff) >= 0x6c00) sh.big = 1;
+                h[i] = v;
             }
             stager_sync();
-            const int big = sh.big;
-            const __half2 down = __half2half2(__ushort_as_half(0x2c00));     // 1 / 16
-            if (w == 0) { sh.fk[j & 7] = big & 1 ? 16.f : 1.f; sh.fv[j & 7] = big & 2 ? 16.f : 1.f; }
-            if (j > 1) ok = warp_wait(&sh.sfull[b], (j - 2) >> 1 & 1, abort_flag);                       // the keys of page j - 2 are done with
-            if (ok) {
-#pragma unroll
-            for (int it = 0; it < 2; it++) {
-                const int jj = w >> 3 & 3, t = ((w >> 5) + 4 * it) * 8 + (w & 7);
-                unsigned kw[NG];
+            const float f = sh.big ? 16.f : 1.f;
+            stager_sync();
+            return f;
+        };
+        const __half2 down = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
+        auto do_keys = [&](int j) {
+            const uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW;
+            const float f = look(j, true);
+            if (w == 0) sh.fk[j & 7] = f;
+#pragma unroll 1
+            for (int it = w; it < 256; it += PT_ST) {        // position t, piece jj of a group's four
+                const int t = (it >> 5) * 8 + (it & 7), jj = it >> 3 & 3;
+                unsigned kw[NG], st[(NG + 1) / 2];
                 kv4_ldsw<NG>(kw, raw + t * L::KS + jj * (4 * NG));
+                kv4_ldsteps<NG>(st, raw + L::RK + t * (2 * NG));
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    __half2 d = __half2half2(__ushort_as_half(kst[t * NG + g]));
-                    if (big & 1) d = __hmul2(d, down);
+                    __half2 d = __half2half2(__ushort_as_half((unsigned short)(g & 1 ? st[g >> 1] >> 16 : st[g >> 1])));
+                    if (f != 1.f) d = __hmul2(d, down);
                     unsigned h[4], l[4];
                     kv4_values_hl(kw[g], d, h, l);
                     const int c = 4 * g + jj;
-                    uint8_t *dst = sm + L::OFF_K + 2 * b * L::K + (c >> 3) * (64 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
+                    uint8_t *dst = sm + L::OFF_K + (c >> 3) * (64 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
                     *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
                     *reinterpret_cast<uint4 *>(dst + L::K) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&sh.kfull[b]);
-            }
-            if (ok && j > 1) ok = warp_wait(&sh.pvdone[b], (j - 2) >> 1 & 1, abort_flag);                // the values of page j - 2 are done with
-            if (ok) {
-                const int o = w & 7, r = w >> 3 & 7;         // eight positions 8 o .., dims 32 g + 4 r + 0 .. 3
+            mbar_arrive(&sh.kfull);
+        };
+        auto do_values = [&](int j) {
+            const uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
+            if (w < NG) sh.nan[j & 7][w] = 0ull;
+            if (w == 4) sh.anynan[j & 7] = 0;
+            const float f = look(j, false);
+            if (w == 0) sh.fv[j & 7] = f;
+            const uint16_t *vst = reinterpret_cast<const uint16_t *>(raw + L::RV);
+#pragma unroll 1
+            for (int it = w; it < 64 * NG; it += PT_ST) {    // eight positions 8 o .., dims 32 g + 4 r + 0 .. 3
+                const int o = it & 7, r = it >> 3 & 7, g = it >> 6;
+                unsigned h[4][4], l[4][4];
 #pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    if ((g & 1) != w >> 6) continue;
-                    unsigned h[4][4], l[4][4];
+                for (int q = 0; q < 4; q++) {                // positions 8 o + 2 q, + 1
+                    const unsigned vw = *reinterpret_cast<const unsigned *>(raw + o * L::VS + (r * 4 + q) * (4 * NG) + 4 * g);
+                    const int t = 8 * o + 2 * q;
+                    __half2 d = __halves2half2(__ushort_as_half(vst[t * NG + g]), __ushort_as_half(vst[(t + 1) * NG + g]));
+                    if (f != 1.f) d = __hmul2(d, down);
+                    unsigned hh[4], ll[4];
+                    kv4_values_hl(vw, d, hh, ll);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {            // positions 8 o + 2 q, + 1
-                        const unsigned vw = *reinterpret_cast<const unsigned *>(raw + L::RK + o * L::VS + (r * 4 + q) * (4 * NG) + 4 * g);
-                        const int t = 8 * o + 2 * q;
-                        __half2 d = __halves2half2(__ushort_as_half(vst[t * NG + g]), __ushort_as_half(vst[(t + 1) * NG + g]));
-                        if (big & 2) d = __hmul2(d, down);
-                        unsigned hh[4], ll[4];
-                        kv4_values_hl(vw, d, hh, ll);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) { h[i][q] = hh[i]; l[i][q] = ll[i]; }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int dim = 32 * g + 4 * r + i;
-                        uint8_t *dst = sm + L::OFF_V + 2 * b * L::V + dim * 128 + ((o ^ (dim & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[i][0], h[i][1], h[i][2], h[i][3]);
-                        *reinterpret_cast<uint4 *>(dst + L::V) = make_uint4(l[i][0], l[i][1], l[i][2], l[i][3]);
-                    }
+                    for (int i = 0; i < 4; i++) { h[i][q] = hh[i]; l[i][q] = ll[i]; }
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&sh.vfull[b]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int dim = 32 * g + 4 * r + i;
+                    uint8_t *dst = sm + L::OFF_V + dim * 128 + ((o ^ (dim & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(h[i][0], h[i][1], h[i][2], h[i][3]);
+                    *reinterpret_cast<uint4 *>(dst + L::V) = make_uint4(l[i][0], l[i][1], l[i][2], l[i][3]);
+                }
             }
-            if (!stager_and(ok)) break;                      // everyone has read the stage
-            stage(j + 2);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&sh.vfull);
+        };
+        // groups of copies, in order: K0 V0 K1 V1 K2 V2 ...; a page's part is waited for with the two that follow it pending
+        stage(0, true); stage(0, false); stage(1, true); stage(1, false);
+        cp_async_wait<3>();
+        stager_sync();
+        if (n > 0) do_keys(0);
+        stager_sync();
+        stage(2, true);
+        bool ok = true;
+        for (int j = 0; j < n; j++) {
+            cp_async_wait<2>();                              // V of page j and K of page j + 1 are here
+            stager_sync();
+            if (j + 1 < n) {
+                ok = warp_wait(&sh.sfull[nx - 1][j & 1], j >> 1 & 1, abort_flag);                // the keys of page j are done with
+                if (!stager_and(ok)) break;
+                do_keys(j + 1);
+            }
+            if (j > 0) {
+                ok = warp_wait(&sh.pvdone[nx - 1], (j - 1) & 1, abort_flag);                     // the values of page j - 1 are done with
+                if (!stager_and(ok)) break;
+            }
+            do_values(j);
+            stager_sync();                                   // everyone has read both stages
+            stage(j + 2, false); stage(j + 3, true);
         }
         cp_async_wait<0>();
-    } else {
-        // ---- softmax: two threads a line ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFT));
-        constexpr int HO = HD / 2;                           // dims of this thread: half * HO ..
-        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
-        float m = -INFINITY, l = 0.f, o[HO];
+    } else if (x < nx) {
+        // ---- softmax: a thread a line ----
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        float m = -INFINITY, l = 0.f, o[HD];
         unsigned nanbits = 0;
 #pragma unroll
-        for (int i = 0; i < HO; i++) o[i] = 0.f;
-        float pf = 1.f;                                      // what the O of the page before is still to be multiplied by
+        for (int i = 0; i < HD; i++) o[i] = 0.f;
+        float f = 1.f;                                       // what the O of the page before is still to be multiplied by
         bool ok = true;
-        auto add_o = [&](int j) {                            // O of page j to the registers
-            const int b = j & 1;
-            ok = ok && warp_wait(&sh.pvdone[b], j >> 1 & 1, abort_flag);
-            if (!ok) return;
-            tc_after();
-            const float f = pf * sh.fv[j & 7];
-            const uint32_t at = mine + TM_O + b * 128 + half * HO;
-#pragma unroll
-            for (int c = 0; c < HO; c += 32) {
-                uint32_t v[16], w[16];
-                tm_ld16(v, at + c);
-                if (c + 16 < HO) tm_ld16(w, at + c + 16);
-                tm_wait();
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[c + i] = fmaf(__uint_as_float(v[i]), f, o[c + i]);
-                if (c + 16 < HO)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[c + 16 + i] = fmaf(__uint_as_float(w[i]), f, o[c + 16 + i]);
-            }
-            tc_before();
-            mbar_arrive(&sh.oempty[b]);
-            if (sh.anynan[j & 7]) {
-                const int t0 = list[j].y;
-                for (int g = 0; g < NG; g++)
-                    for (unsigned long long mk = sh.nan[j & 7][g]; mk; mk &= mk - 1) {
-                        const int t = t0 + __ffsll((long long)mk) - 1;
-                        if (t >= clo && t <= chi) nanbits |= 1u << g;
-                    }
-                __syncwarp();
-            }
-        };
-        for (int j = 0; j < n; j++) {
-            const int b = j & 1, t0 = list[j].y + half * 32;
-            ok = ok && warp_wait(&sh.sfull[b], j >> 1 & 1, abort_flag);
-            float v[32], mx = -INFINITY, ds = 0.f;
-            if (ok) {
+        for (int j = 0; j <= n; j++) {
+            const int t0 = j < n ? list[j].y : 0;
+            if (j < n) {
+                ok = warp_wait(&sh.sfull[x][j & 1], j >> 1 & 1, abort_flag);
+                if (!ok) break;
                 tc_after();
-                ds = desc * sh.fk[j & 7];
-                tm_ld32(v, mine + TM_S + b * 64 + half * 32);
-                if (!(t0 >= cr.lo_all && t0 + 32 <= cr.hi_all)) {
+                const float ds = desc * sh.fk[j & 7];
+                const bool inside = t0 >= cr.lo_all && t0 + KV4_PAGE <= cr.hi_all;
+                const uint32_t at = mine + TM_S + (x * 2 + (j & 1)) * 64;
+                float mx = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) if (t0 + i < clo || t0 + i > chi) v[i] = -INFINITY;
+                for (int h = 0; h < 2; h++) {
+                    float v[32];
+                    tm_ld32(v, at + h * 32);
+                    if (!inside) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) { const int t = t0 + h * 32 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, v[i]);
                 }
+                mx *= ds;                                    // (the scale is positive)
+                const bool up = mx > m + 8.f;
+                f = 1.f;
+                if (__any_sync(0xffffffffu, up)) {
+                    if (up) { f = kv4_exp2(m - mx); m = mx; }
+                    __syncwarp();
+                    l *= f;
 #pragma unroll
-                for (int i = 0; i < 32; i++) mx = fmaxf(mx, v[i]);
-                sh.mx[b][half][line] = mx;
-            }
-            ok = pair_and(quarter, ok);
-            if (!ok) break;
-            mx = fmaxf(mx, sh.mx[b][half ^ 1][line]) * ds;   // (the scale is positive)
-            float f = 1.f;
-            const bool up = mx > m + 8.f;
-            if (__any_sync(0xffffffffu, up)) {
-                if (up) { f = kv4_exp2(m - mx); m = mx; }
-                __syncwarp();
-                l *= f;
+                    for (int i = 0; i < HD; i++) o[i] *= f;
+                }
+                // weights times 2^6, as hi and lo pairs of consecutive positions, over the scores: a half's 32 columns become
+                // 16 of hi and 16 of lo (a line that has seen nothing yet: all 0)
+                const float mm = m == -INFINITY ? 0.f : m - 6.f;
+                float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                for (int i = 0; i < HO; i++) o[i] *= f;
-            }
-            // weights times 2^6, as hi and lo pairs of consecutive positions (a line that has seen nothing yet: all 0)
-            const float mm = m == -INFINITY ? 0.f : m - 6.f;
-            unsigned ph[16], pl[16];
-            float s0 = 0.f, s1 = 0.f;
+                for (int h = 0; h < 2; h++) {
+                    float v[32];
+                    tm_ld32(v, at + h * 32);
+                    if (!inside) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float p0 = kv4_exp2(fmaf(v[2 * i], ds, -mm)), p1 = kv4_exp2(fmaf(v[2 * i + 1], ds, -mm));
-                s0 += p0; s1 += p1;
-                kv4_pieces(p0, p1, ph[i], pl[i]);
+                        for (int i = 0; i < 32; i++) { const int t = t0 + h * 32 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        unsigned ph[8], pl[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float p0 = kv4_exp2(fmaf(v[16 * q + 2 * i], ds, -mm)), p1 = kv4_exp2(fmaf(v[16 * q + 2 * i + 1], ds, -mm));
+                            s0 += p0; s1 += p1;
+                            kv4_pieces(p0, p1, ph[i], pl[i]);
+                        }
+                        tm_st8(at + h * 32 + q * 8, ph);
+                        tm_st8(at + h * 32 + 16 + q * 8, pl);
+                    }
+                }
+                l += s0 + s1;
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_before();
+                mbar_arrive(&sh.pfull[x][j & 1]);
+            } else f = 1.f;
+            if (j > 0) {                                     // O of page j - 1 to the registers
+                const int i0 = j - 1;
+                ok = warp_wait(&sh.pvdone[x], i0 & 1, abort_flag);
+                if (!ok) break;
+                tc_after();
+                const float g = f * sh.fv[i0 & 7];
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    float v[32];
+                    tm_ld32(v, mine + TM_O + x * 128 + c);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[c + i] = fmaf(v[i], g, o[c + i]);
+                }
+                tc_before();
+                mbar_arrive(&sh.oempty[x]);
+                if (sh.anynan[i0 & 7]) {
+                    const int tn = list[i0].y;
+                    for (int gg = 0; gg < NG; gg++)
+                        for (unsigned long long mk = sh.nan[i0 & 7][gg]; mk; mk &= mk - 1) {
+                            const int t = tn + __ffsll((long long)mk) - 1;
+                            if (t >= clo && t <= chi) nanbits |= 1u << gg;
+                        }
+                    __syncwarp();
+                }
             }
-            l += s0 + s1;
-            tm_st16(mine + TM_P + b * 64 + half * 16, ph);
-            tm_st16(mine + TM_P + b * 64 + 32 + half * 16, pl);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            tc_before();
-            mbar_arrive(&sh.pfull[b]);
-            mbar_arrive(&sh.sempty[b]);
-            pf = f;
-            if (j > 0) add_o(j - 1);
         }
-        pf = 1.f;
-        if (n > 0 && ok) add_o(n - 1);
-        sh.mx[n & 1][half][line] = l;
-        ok = pair_and(quarter, ok);
-        l += sh.mx[n & 1][half ^ 1][line];
-        if (ok && line < ncol) {
+        if (ok && tid < ncol) {
             float *out = nsplit == 1 ? a.ctx + rh * HD : part + (rh * nsplit + split) * (HD + 4) + 4;
-            if (nsplit > 1 && half == 0) { out[-4] = m; out[-3] = l; }
+            if (nsplit > 1) { out[-4] = m; out[-3] = l; }
             const float qnan = __int_as_float(0x7fffffff);
 #pragma unroll
-            for (int c = 0; c < HO; c += 4) {
+            for (int c = 0; c < HD; c += 4) {
                 float4 v = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
                 if (nsplit == 1)
                     v = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__fdiv_rn(v.x, l), __fdiv_rn(v.y, l), __fdiv_rn(v.z, l), __fdiv_rn(v.w, l));
-                if (nanbits >> ((half * HO + c) >> 5) & 1) v = make_float4(qnan, qnan, qnan, qnan);
-                *reinterpret_cast<float4 *>(out + half * HO + c) = v;
+                if (nanbits >> (c >> 5) & 1) v = make_float4(qnan, qnan, qnan, qnan);
+                *reinterpret_cast<float4 *>(out + c) = v;
             }
         }
     }
@@ -494,7 +523,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == 12) {
+    if (warp == 11) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
