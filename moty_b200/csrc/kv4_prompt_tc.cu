@@ -12,9 +12,10 @@
 //   warps 0-3, 4-7   softmax of a tile, a thread a line: S from TMEM, running maximum (moved when passed by 8 in base-2
 //               units), weights back to TMEM over the scores as the A operand of the second product, then the O of the page
 //               before added to the registers
-//   warps 8-10  a page's codes and steps into shared memory (two pages ahead), then as k and v^T operand tiles (K-major,
-//               128-byte swizzle): eight key dims of a position, or eight positions of a value dim, are one 16-byte piece
-//   warp 11     issues the products: both S of page j + 1, then both O of page j, so that a tile's softmax of a page has the
+//   warps 8-11, 12-14   keys and values of a page: bulk copies of codes and steps into shared memory (two pages deep), then k
+//               and v^T operand tiles (K-major, 128-byte swizzle): eight key dims of a position, or eight positions of a
+//               value dim, are one 16-byte piece
+//   warp 15     issues the products: both S of page j + 1, then both O of page j, so that a tile's softmax of a page has the
 //               time of three products, and each operand tile is rebuilt during the two products that do not read it
 // TMEM (512 columns): scores / weights two buffers a tile, O one a tile.  What bounds it: the twelve products of a page and
 // two tiles, 3072 cycles of tensor core at hd = 128; with one tile a CTA the staging alone took longer than its products
@@ -24,19 +25,19 @@
 #include "kv4_frag.cuh"
 #include "kv4_attend.cuh"
 #include "tc_common.cuh"
+#include <type_traits>
 
 namespace {
 
-constexpr int PT_M = 128, PT_NP = KV4_TC_PAGES, PT_T = 384, PT_ST = 96;      // lines a tile, pages a span, threads, staging threads
-constexpr int PT_REGS = 168, PT_REGS_SOFT = 208, PT_REGS_REST = 80;
-static_assert(KV4_TC_LINES == 2 * PT_M && 256 * PT_REGS_SOFT + 128 * PT_REGS_REST <= PT_T * PT_REGS, "lines; register shares");
+constexpr int PT_M = 128, PT_NP = KV4_TC_PAGES, PT_T = 512, PT_KT = 128, PT_VT = 96;     // lines a tile, pages a span, threads: all, keys, values
+constexpr int PT_REGS = 128, PT_REGS_SOFT = 184, PT_REGS_REST = 72;
+static_assert(KV4_TC_LINES == 2 * PT_M && 256 * PT_REGS_SOFT + 256 * PT_REGS_REST <= PT_T * PT_REGS, "lines; register shares");
 constexpr uint32_t TM_S = 0, TM_O = 256;                     // TMEM columns: scores / weights [tile][page & 1] x 64, O [tile] x 128
 
 template <int NG> struct PtL {
     static constexpr int HD = NG * 32, NSUB = (NG + 1) / 2;
-    static constexpr int KS = (NG % 2 ? NG : NG + 1) * 16;   // bytes between staged key rows (an odd number of 16-byte pieces)
     static constexpr int VS = 4 * HD + 16;                   // bytes between staged value halves (eight positions)
-    static constexpr int RK = 64 * KS, RV = 8 * VS, RST = 128 * NG, RAW = RK + RV + 2 * RST;
+    static constexpr int RK = 32 * HD, RV = 8 * VS, RST = 4 * HD, RAW = RK + RV + 2 * RST;       // staged: key codes, key steps, value halves, value steps
     static constexpr int Q = NSUB * PT_M * 128, K = NSUB * 64 * 128, V = HD * 128;      // one piece (hi or lo) of an operand
     static constexpr int OFF_K = 4 * Q, OFF_V = OFF_K + 2 * K, OFF_RAW = OFF_V + 2 * V, OFF_LIST = OFF_RAW + 2 * RAW;
     static constexpr int SMEM = OFF_LIST + PT_NP * 8 + 1024;
@@ -44,12 +45,13 @@ template <int NG> struct PtL {
 
 struct PtShared {
     uint64_t kfull, vfull, sfull[2][2], pfull[2][2], pvdone[2], oempty[2];   // [tile][page & 1]; the others one phase a page
+    uint64_t rawk[2], rawv[2];                               // [page & 1]
     uint32_t tmem;
     int abort, n;
     float fk[8], fv[8];                                      // by page (the staging warps run ahead): what scores and outputs are to be multiplied by
     unsigned long long nan[8][4];                            // by page and group: positions whose value step is NaN
     int anynan[8];
-    int big;                                                 // a step of the staged page that would overflow: bit 0 keys, bit 1 values
+    int big[2];                                              // a step of the staged keys / values that would overflow
 };
 
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
@@ -88,6 +90,14 @@ __device__ __forceinline__ void tm_ld32(float (&v)[32], uint32_t addr) {
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tm_ld16(float (&v)[16], uint32_t addr) {
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tm_st8(uint32_t addr, const unsigned (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
@@ -104,13 +114,17 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     const bool ok = pt_wait(bar, parity, abort_flag);
     return __all_sync(0xffffffffu, ok);
 }
-__device__ __forceinline__ void stager_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PT_ST) : "memory"); }
-// the same, and whether all of them say yes: they go on, or leave, together
-__device__ __forceinline__ bool stager_and(bool ok) {
+// the warps of one role: a barrier of their own (1 keys, 2 values), and whether all of them say yes
+template <int ID, int N> __device__ __forceinline__ void role_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+template <int ID, int N> __device__ __forceinline__ bool role_and(bool ok) {
     int all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, 1, %2, q;\n\tselp.s32 %0, 1, 0, p;\n\t}"
-                 : "=r"(all) : "r"((int)ok), "n"(PT_ST) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, %2, %3, q;\n\tselp.s32 %0, 1, 0, p;\n\t}"
+                 : "=r"(all) : "r"((int)ok), "n"(ID), "n"(N) : "memory");
     return all != 0;
+}
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
 // the word's values times the step pair d (one step twice for keys, two positions' steps for values): 4 pairs hi, 4 pairs lo
@@ -153,7 +167,8 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
 
     if (tid == 0) {
         sh.abort = 0;
-        mbar_init(&sh.kfull, PT_ST); mbar_init(&sh.vfull, PT_ST);
+        mbar_init(&sh.kfull, PT_KT); mbar_init(&sh.vfull, PT_VT);
+        for (int i = 0; i < 2; i++) { mbar_init(&sh.rawk[i], 1); mbar_init(&sh.rawv[i], 1); }
         for (int x = 0; x < 2; x++) {
             for (int i = 0; i < 2; i++) { mbar_init(&sh.sfull[x][i], 1); mbar_init(&sh.pfull[x][i], PT_M); }
             mbar_init(&sh.pvdone[x], 1); mbar_init(&sh.oempty[x], PT_M);
@@ -161,7 +176,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 11) {
+    if (warp == 15) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -231,9 +246,9 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
     const int n = sh.n;
     volatile int *abort_flag = &sh.abort;
 
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_REST));      // (384 x 168 at launch)
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_REST));      // (512 x 128 at launch)
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFT));
-    if (warp == 11) {
+    if (warp == 15) {
         // ---- the products ----
         const uint32_t id_s = (1u << 4) | (64u >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
         const uint32_t id_o = (1u << 4) | ((uint32_t)HD >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
@@ -272,7 +287,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                     for (int term = 0; term < 3; term++)     // p lo * v hi, p hi * v lo, p hi * v hi
 #pragma unroll
                         for (int s = 0; s < 4; s++)
-                            umma_ts(d, p + (s >> 1) * 32 + (s & 1) * 8 + (term == 0 ? 16 : 0), dv + (((term == 1 ? L::V : 0) + s * 32) >> 4), id_o,
+                            umma_ts(d, p + s * 16 + (term == 0 ? 8 : 0), dv + (((term == 1 ? L::V : 0) + s * 32) >> 4), id_o,
                                     (term | s) != 0, lead);
                     if (lead) umma_commit(&sh.pvdone[y]);
                     __syncwarp();
@@ -281,130 +296,122 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         }
     } else if (warp >= 8) {
         // ---- pages into shared memory, then as operand tiles ----
-        const int w = tid - 256;
         const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
         const size_t page_bytes = kv4_page_bytes(a.geo);
-        // keys of a page are taken one page before its values: K of page j + 1 while the O of page j - 1 is formed, V of page j
-        // while the S of page j + 1 is
-        auto stage = [&](int j, bool keys) {
-            if (j < n) {
-                const uint8_t *src = base + (size_t)list[j].x * page_bytes + (keys ? 0 : kv4_v_code_off(HD));
-                uint8_t *dst = sm + L::OFF_RAW + (j & 1) * L::RAW + (keys ? 0 : L::RK + L::RST);
-                for (int c = w; c < 72 * NG; c += PT_ST)     // rows of NG pieces (keys), halves of 8 NG (values), then the steps
-                    cp_async16(dst + (c >= 64 * NG ? (keys ? L::RK : L::RV) + (c - 64 * NG) * 16
-                                      : keys ? (c / NG) * L::KS + (c % NG) * 16 : (c / (8 * NG)) * L::VS + (c % (8 * NG)) * 16), src + c * 16);
-            }
-            cp_async_commit();
-        };
-        // steps of a staged part: positions that no line sees become 0 (their memory may hold anything), steps that would
-        // overflow and NaN steps of values are noted; all of it rare, and looked for two steps at a time
-        auto look = [&](int j, bool keys) {
-            uint32_t *st = reinterpret_cast<uint32_t *>(sm + L::OFF_RAW + (j & 1) * L::RAW + (keys ? L::RK : L::RK + L::RST + L::RV));
+        const __half2 down = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
+        // Steps of a staged part: positions that no line sees become 0 (their memory may hold anything), steps that would
+        // overflow and NaN steps of values are noted; all of it rare, and looked for two steps at a time.  Returns what
+        // the part's values have been divided by.  (The barrier in it also says that all have left the page before.)
+        auto look = [&](auto keys_, int w, int j, uint32_t *st) {
+            constexpr bool keys = decltype(keys_)::value;
+            constexpr int ID = keys ? 1 : 2, N = keys ? PT_KT : PT_VT;
             const int t0 = list[j].y;
             bool odd = t0 < cr.lo_any || t0 + KV4_PAGE > cr.hi_any;
-            for (int i = w; i < 32 * NG; i += PT_ST) odd |= (((st[i] & 0x7fff7fffu) + 0x14001400u) & 0x80008000u) != 0;      // |step| >= 4096, infinity, NaN
-            if (stager_and(!odd)) return 1.f;
-            if (w == 0) sh.big = 0;
-            stager_sync();
+            for (int i = w; i < 32 * NG; i += N) odd |= (((st[i] & 0x7fff7fffu) + 0x14001400u) & 0x80008000u) != 0;      // |step| >= 4096, infinity, NaN
+            if (role_and<ID, N>(!odd)) return 1.f;
+            if (w == 0) sh.big[keys] = 0;
+            role_sync<ID, N>();
             uint16_t *h = reinterpret_cast<uint16_t *>(st);
-            for (int i = w; i < 64 * NG; i += PT_ST) {
+            for (int i = w; i < 64 * NG; i += N) {
                 const int t = i / NG, g = i - t * NG;
                 uint16_t v = h[i];
                 if (t0 + t < cr.lo_any || t0 + t >= cr.hi_any) v = 0;
                 if ((v & 0x7fff) >= 0x7c00) {
                     if (!keys) { atomicOr(&sh.nan[j & 7][g], 1ull << t); sh.anynan[j & 7] = 1; v = 0; }
-                } else if ((v & 0x7fff) >= 0x6c00) sh.big = 1;
+                } else if ((v & 0x7fff) >= 0x6c00) sh.big[keys] = 1;
                 h[i] = v;
             }
-            stager_sync();
-            const float f = sh.big ? 16.f : 1.f;
-            stager_sync();
+            role_sync<ID, N>();
+            const float f = sh.big[keys] ? 16.f : 1.f;
+            role_sync<ID, N>();
             return f;
         };
-        const __half2 down = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
-        auto do_keys = [&](int j) {
-            const uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW;
-            const float f = look(j, true);
-            if (w == 0) sh.fk[j & 7] = f;
-#pragma unroll 1
-            for (int it = w; it < 256; it += PT_ST) {        // position t, piece jj of a group's four
-                const int t = (it >> 5) * 8 + (it & 7), jj = it >> 3 & 3;
-                unsigned kw[NG], st[(NG + 1) / 2];
-                kv4_ldsw<NG>(kw, raw + t * L::KS + jj * (4 * NG));
-                kv4_ldsteps<NG>(st, raw + L::RK + t * (2 * NG));
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    __half2 d = __half2half2(__ushort_as_half((unsigned short)(g & 1 ? st[g >> 1] >> 16 : st[g >> 1])));
-                    if (f != 1.f) d = __hmul2(d, down);
-                    unsigned h[4], l[4];
-                    kv4_values_hl(kw[g], d, h, l);
-                    const int c = 4 * g + jj;
-                    uint8_t *dst = sm + L::OFF_K + (c >> 3) * (64 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4 *>(dst + L::K) = make_uint4(l[0], l[1], l[2], l[3]);
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&sh.kfull);
-        };
-        auto do_values = [&](int j) {
-            const uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
-            if (w < NG) sh.nan[j & 7][w] = 0ull;
-            if (w == 4) sh.anynan[j & 7] = 0;
-            const float f = look(j, false);
-            if (w == 0) sh.fv[j & 7] = f;
-            const uint16_t *vst = reinterpret_cast<const uint16_t *>(raw + L::RV);
-#pragma unroll 1
-            for (int it = w; it < 64 * NG; it += PT_ST) {    // eight positions 8 o .., dims 32 g + 4 r + 0 .. 3
-                const int o = it & 7, r = it >> 3 & 7, g = it >> 6;
-                unsigned h[4][4], l[4][4];
-#pragma unroll
-                for (int q = 0; q < 4; q++) {                // positions 8 o + 2 q, + 1
-                    const unsigned vw = *reinterpret_cast<const unsigned *>(raw + o * L::VS + (r * 4 + q) * (4 * NG) + 4 * g);
-                    const int t = 8 * o + 2 * q;
-                    __half2 d = __halves2half2(__ushort_as_half(vst[t * NG + g]), __ushort_as_half(vst[(t + 1) * NG + g]));
-                    if (f != 1.f) d = __hmul2(d, down);
-                    unsigned hh[4], ll[4];
-                    kv4_values_hl(vw, d, hh, ll);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) { h[i][q] = hh[i]; l[i][q] = ll[i]; }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int dim = 32 * g + 4 * r + i;
-                    uint8_t *dst = sm + L::OFF_V + dim * 128 + ((o ^ (dim & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(h[i][0], h[i][1], h[i][2], h[i][3]);
-                    *reinterpret_cast<uint4 *>(dst + L::V) = make_uint4(l[i][0], l[i][1], l[i][2], l[i][3]);
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&sh.vfull);
-        };
-        // groups of copies, in order: K0 V0 K1 V1 K2 V2 ...; a page's part is waited for with the two that follow it pending
-        stage(0, true); stage(0, false); stage(1, true); stage(1, false);
-        cp_async_wait<3>();
-        stager_sync();
-        if (n > 0) do_keys(0);
-        stager_sync();
-        stage(2, true);
         bool ok = true;
-        for (int j = 0; j < n; j++) {
-            cp_async_wait<2>();                              // V of page j and K of page j + 1 are here
-            stager_sync();
-            if (j + 1 < n) {
-                ok = warp_wait(&sh.sfull[nx - 1][j & 1], j >> 1 & 1, abort_flag);                // the keys of page j are done with
-                if (!stager_and(ok)) break;
-                do_keys(j + 1);
+        if (warp < 12) {
+            const int w = tid - 256;
+            auto load = [&](int j) {                         // key codes and steps are one run of bytes
+                mbar_expect_tx(&sh.rawk[j & 1], 36 * HD);
+                bulk_load(sm + L::OFF_RAW + (j & 1) * L::RAW, base + (size_t)list[j].x * page_bytes, 36 * HD, &sh.rawk[j & 1]);
+            };
+            if (w == 0) for (int j = 0; j < 2 && j < n; j++) load(j);
+            for (int j = 0; j < n; j++) {
+                uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW;
+                ok = warp_wait(&sh.rawk[j & 1], j >> 1 & 1, abort_flag);
+                if (!role_and<1, PT_KT>(ok)) break;
+                if (w == 0 && j > 0 && j + 1 < n) load(j + 1);
+                const float f = look(std::true_type{}, w, j, reinterpret_cast<uint32_t *>(raw + L::RK));
+                if (w == 0) sh.fk[j & 7] = f;
+                // the keys of page j - 1 are done with (a warp that gives up goes on to the next barrier, where all leave)
+                if (j > 0 && !warp_wait(&sh.sfull[nx - 1][(j - 1) & 1], (j - 1) >> 1 & 1, abort_flag)) continue;
+#pragma unroll
+                for (int it = w; it < 256; it += PT_KT) {    // position t, piece jj of a group's four
+                    const int t = (it >> 5) * 8 + (it & 7), jj = it >> 3 & 3;
+                    unsigned kw[NG], st[(NG + 1) / 2];
+                    kv4_ldsw<NG>(kw, raw + t * (HD / 2) + jj * (4 * NG));
+                    kv4_ldsteps<NG>(st, raw + L::RK + t * (2 * NG));
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        __half2 d = __half2half2(__ushort_as_half((unsigned short)(g & 1 ? st[g >> 1] >> 16 : st[g >> 1])));
+                        if (f != 1.f) d = __hmul2(d, down);
+                        unsigned h[4], l[4];
+                        kv4_values_hl(kw[g], d, h, l);
+                        const int c = 4 * g + jj;
+                        uint8_t *dst = sm + L::OFF_K + (c >> 3) * (64 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4 *>(dst + L::K) = make_uint4(l[0], l[1], l[2], l[3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&sh.kfull);
             }
-            if (j > 0) {
-                ok = warp_wait(&sh.pvdone[nx - 1], (j - 1) & 1, abort_flag);                     // the values of page j - 1 are done with
-                if (!stager_and(ok)) break;
+        } else {
+            const int w = tid - 384;
+            auto load = [&](int j) {
+                uint8_t *dst = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
+                const uint8_t *src = base + (size_t)list[j].x * page_bytes + kv4_v_code_off(HD);
+                mbar_expect_tx(&sh.rawv[j & 1], 36 * HD);
+                for (int o = 0; o < 8; o++) bulk_load(dst + o * L::VS, src + o * (4 * HD), 4 * HD, &sh.rawv[j & 1]);     // apart by 16 bytes: eight halves, eight bank groups
+                bulk_load(dst + L::RV, src + 32 * HD, 4 * HD, &sh.rawv[j & 1]);
+            };
+            if (w == 0) for (int j = 0; j < 2 && j < n; j++) load(j);
+            for (int j = 0; j < n; j++) {
+                uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
+                ok = warp_wait(&sh.rawv[j & 1], j >> 1 & 1, abort_flag);
+                if (!role_and<2, PT_VT>(ok)) break;
+                if (w == 0 && j > 0 && j + 1 < n) load(j + 1);
+                if (w < NG) sh.nan[j & 7][w] = 0ull;
+                if (w == 4) sh.anynan[j & 7] = 0;
+                const float f = look(std::false_type{}, w, j, reinterpret_cast<uint32_t *>(raw + L::RV));
+                if (w == 0) sh.fv[j & 7] = f;
+                if (j > 0 && !warp_wait(&sh.pvdone[nx - 1], (j - 1) & 1, abort_flag)) continue;  // the values of page j - 1 are done with
+                const uint16_t *vst = reinterpret_cast<const uint16_t *>(raw + L::RV);
+#pragma unroll 1
+                for (int it = w; it < 64 * NG; it += PT_VT) {        // eight positions 8 o .., dims 32 g + 4 r + 0 .. 3
+                    const int o = it & 7, r = it >> 3 & 7, g = it >> 6;
+                    unsigned h[4][4], l[4][4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {            // positions 8 o + 2 q, + 1
+                        const unsigned vw = *reinterpret_cast<const unsigned *>(raw + o * L::VS + (r * 4 + q) * (4 * NG) + 4 * g);
+                        const int t = 8 * o + 2 * q;
+                        __half2 d = __halves2half2(__ushort_as_half(vst[t * NG + g]), __ushort_as_half(vst[(t + 1) * NG + g]));
+                        if (f != 1.f) d = __hmul2(d, down);
+                        unsigned hh[4], ll[4];
+                        kv4_values_hl(vw, d, hh, ll);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) { h[i][q] = hh[i]; l[i][q] = ll[i]; }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int dim = 32 * g + 4 * r + i;
+                        uint8_t *dst = sm + L::OFF_V + dim * 128 + ((o ^ (dim & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[i][0], h[i][1], h[i][2], h[i][3]);
+                        *reinterpret_cast<uint4 *>(dst + L::V) = make_uint4(l[i][0], l[i][1], l[i][2], l[i][3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&sh.vfull);
             }
-            do_values(j);
-            stager_sync();                                   // everyone has read both stages
-            stage(j + 2, false); stage(j + 3, true);
         }
-        cp_async_wait<0>();
     } else if (x < nx) {
         // ---- softmax: a thread a line ----
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -445,30 +452,27 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
 #pragma unroll
                     for (int i = 0; i < HD; i++) o[i] *= f;
                 }
-                // weights times 2^6, as hi and lo pairs of consecutive positions, over the scores: a half's 32 columns become
-                // 16 of hi and 16 of lo (a line that has seen nothing yet: all 0)
+                // weights times 2^6, as hi and lo pairs of consecutive positions, over the scores: 16 columns become 8 of hi
+                // and 8 of lo (a line that has seen nothing yet: all 0)
                 const float mm = m == -INFINITY ? 0.f : m - 6.f;
                 float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float v[32];
-                    tm_ld32(v, at + h * 32);
+                for (int q = 0; q < 4; q++) {
+                    float v[16];
+                    tm_ld16(v, at + q * 16);
                     if (!inside) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) { const int t = t0 + h * 32 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
+                        for (int i = 0; i < 16; i++) { const int t = t0 + q * 16 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
                     }
+                    unsigned ph[8], pl[8];
 #pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        unsigned ph[8], pl[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float p0 = kv4_exp2(fmaf(v[16 * q + 2 * i], ds, -mm)), p1 = kv4_exp2(fmaf(v[16 * q + 2 * i + 1], ds, -mm));
-                            s0 += p0; s1 += p1;
-                            kv4_pieces(p0, p1, ph[i], pl[i]);
-                        }
-                        tm_st8(at + h * 32 + q * 8, ph);
-                        tm_st8(at + h * 32 + 16 + q * 8, pl);
+                    for (int i = 0; i < 8; i++) {
+                        const float p0 = kv4_exp2(fmaf(v[2 * i], ds, -mm)), p1 = kv4_exp2(fmaf(v[2 * i + 1], ds, -mm));
+                        s0 += p0; s1 += p1;
+                        kv4_pieces(p0, p1, ph[i], pl[i]);
                     }
+                    tm_st8(at + q * 16, ph);
+                    tm_st8(at + q * 16 + 8, pl);
                 }
                 l += s0 + s1;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == 11) {
+    if (warp == 15) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
