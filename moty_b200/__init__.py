@@ -41,6 +41,12 @@ def lib() -> C.CDLL:
         _lib.moty_cuda_last_error.restype = C.c_char_p
         _lib.moty_cuda_mat_bytes.restype = C.c_int64
         _lib.moty_cuda_kv4_page_bytes.restype = C.c_int64
+        # the calls of a decode step take plain numbers: converted once by signature, not object by object
+        P, I, F = C.c_void_p, C.c_int, C.c_float
+        for name, args in (("append_dev", (P, I, P, P, I, P, P)), ("append_rope_dev", (P, I, I, P, I, P, P, I, P, P, P)),
+                           ("fetch_dev", (P, I, P, P, P, P)), ("attend_dev", (P, I, P, P, I, I, I, F, P, P)),
+                           ("fork_dev", (P, I, P, P, P, I, P, P, I, P)), ("compact_dev", (P, I, P, P, C.c_int64, P, P, P))):
+            getattr(_lib, "moty_cuda_kv4_" + name).argtypes = args
     return _lib
 
 
@@ -391,6 +397,7 @@ class Kv4Batch:
     def __init__(self, nseq, rows, row0_ptr, len_ptr, table_ptr, table_ld, max_rows=None, max_len=None):
         self.c = _Kv4BatchC(nseq, rows, rows if max_rows is None else max_rows, table_ld * Kv4.PAGE if max_len is None else max_len,
                             table_ld, row0_ptr, len_ptr, table_ptr)
+        self.ptr = C.addressof(self.c)
 
 
 class Kv4:
@@ -444,33 +451,41 @@ class Kv4:
 
     # -- device entries --
     def append_dev(self, layer, k_ptr, v_ptr, batch, stream=0, ld=0):
-        _ck(lib().moty_cuda_kv4_append_dev(self.h, layer, C.c_void_p(k_ptr), C.c_void_p(v_ptr), ld, C.byref(batch.c), C.c_void_p(stream)))
+        rc = _lib.moty_cuda_kv4_append_dev(self.h, layer, k_ptr, v_ptr, ld, batch.ptr, stream)
+        if rc:
+            _ck(rc)
 
     def append_rope_dev(self, layer, H, q_ptr, k_ptr, v_ptr, batch, rot, theta, eps, qn_ptr=0, kn_ptr=0, vn_ptr=0, gemma=False,
                         stream=0, q_ld=0, kv_ld=0):
         """Norm and rotate q and k in place at their rows' positions (as ``Attn.core_dev`` does), then store k and v."""
         r = _Kv4RopeC(rot, 1 if gemma else 0, theta, eps, qn_ptr or None, kn_ptr or None, vn_ptr or None)
-        _ck(lib().moty_cuda_kv4_append_rope_dev(self.h, layer, H, C.c_void_p(q_ptr), q_ld, C.c_void_p(k_ptr), C.c_void_p(v_ptr), kv_ld,
-                                                C.byref(r), C.byref(batch.c), C.c_void_p(stream)))
+        rc = _lib.moty_cuda_kv4_append_rope_dev(self.h, layer, H, q_ptr, q_ld, k_ptr, v_ptr, kv_ld, C.addressof(r), batch.ptr, stream)
+        if rc:
+            _ck(rc)
 
     def fetch_dev(self, layer, k_ptr, v_ptr, batch, stream=0):
         """The values held for the batch's rows, f32 [rows][KV * hd]."""
-        _ck(lib().moty_cuda_kv4_fetch_dev(self.h, layer, C.c_void_p(k_ptr), C.c_void_p(v_ptr), C.byref(batch.c), C.c_void_p(stream)))
+        rc = _lib.moty_cuda_kv4_fetch_dev(self.h, layer, k_ptr, v_ptr, batch.ptr, stream)
+        if rc:
+            _ck(rc)
 
     def attend_dev(self, layer, ctx_ptr, q_ptr, H, batch, window=0, scale=0.0, stream=0, q_ld=0):
         """ctx [rows][H * hd] = softmax(scale q k^T) v over each row's own sequence up to its position."""
-        _ck(lib().moty_cuda_kv4_attend_dev(self.h, layer, C.c_void_p(ctx_ptr), C.c_void_p(q_ptr), q_ld, H, window, C.c_float(scale),
-                                           C.byref(batch.c), C.c_void_p(stream)))
+        rc = _lib.moty_cuda_kv4_attend_dev(self.h, layer, ctx_ptr, q_ptr, q_ld, H, window, scale, batch.ptr, stream)
+        if rc:
+            _ck(rc)
 
     def fork_dev(self, n, src_ptr, dst_ptr, fresh_ptr, nseq, len_ptr, table_ptr, table_ld, stream=0):
         """Sequences dst[f] become copies of src[f]: full pages shared, a partial last page copied to fresh[f]."""
-        _ck(lib().moty_cuda_kv4_fork_dev(self.h, n, C.c_void_p(src_ptr), C.c_void_p(dst_ptr), C.c_void_p(fresh_ptr), nseq,
-                                         C.c_void_p(len_ptr), C.c_void_p(table_ptr), table_ld, C.c_void_p(stream)))
+        rc = _lib.moty_cuda_kv4_fork_dev(self.h, n, src_ptr, dst_ptr, fresh_ptr, nseq, len_ptr, table_ptr, table_ld, stream)
+        if rc:
+            _ck(rc)
 
     def compact_dev(self, n, src_ptr, dst_ptr, count, table_ptr, out_ptr, stream=0):
         """Pages src[i] -> dst[i], and the table's ``count`` entries renamed into out (which may be the table)."""
-        _ck(lib().moty_cuda_kv4_compact_dev(self.h, n, C.c_void_p(src_ptr), C.c_void_p(dst_ptr), C.c_int64(count), C.c_void_p(table_ptr),
-                                            C.c_void_p(out_ptr), C.c_void_p(stream)))
+        rc = _lib.moty_cuda_kv4_compact_dev(self.h, n, src_ptr, dst_ptr, count, table_ptr, out_ptr, stream)
+        if rc:
+            _ck(rc)
 
     def close(self):
         if self.h:

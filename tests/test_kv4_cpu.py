@@ -184,11 +184,11 @@ def test_refusals_without_a_gpu():
         mb.Kv4(1, 1, 64, 4, mem_ptr=64)
     L = mb.lib()
     b = mb.Kv4Batch(1, 1, 16, 16, 16, 1)
-    assert L.moty_cuda_kv4_append_dev(None, 0, 16, 16, 0, C.byref(b.c), None) == -2
-    assert L.moty_cuda_kv4_fetch_dev(None, 0, 16, 16, C.byref(b.c), None) == -2
-    assert L.moty_cuda_kv4_attend_dev(None, 0, 16, 16, 0, 1, 0, C.c_float(0), C.byref(b.c), None) == -2
+    assert L.moty_cuda_kv4_append_dev(None, 0, 16, 16, 0, b.ptr, None) == -2
+    assert L.moty_cuda_kv4_fetch_dev(None, 0, 16, 16, b.ptr, None) == -2
+    assert L.moty_cuda_kv4_attend_dev(None, 0, 16, 16, 0, 1, 0, 0.0, b.ptr, None) == -2
     assert L.moty_cuda_kv4_fork_dev(None, 1, 16, 16, 16, 1, 16, 16, 1, None) == -2
-    assert L.moty_cuda_kv4_compact_dev(None, 1, 16, 16, C.c_int64(0), None, None, None) == -2
+    assert L.moty_cuda_kv4_compact_dev(None, 1, 16, 16, 0, None, None, None) == -2
     n = C.c_int()
     assert L.moty_cuda_kv4_alloc(None, 1, C.byref(n)) == -2 and L.moty_cuda_kv4_compact_plan(None, 0, None, None, C.byref(n)) == -2
     assert L.moty_cuda_kv4_free(None) == 0
