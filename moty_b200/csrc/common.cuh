@@ -63,6 +63,7 @@ struct DevCtx {
     // FFN / MoE intermediates
     Buf g, u, h, hq, hs, hxs, hxsum, pair, misc;
     Buf rec;                         // per (token, group) records of the Q4R4 batch kernel
+    Buf kv4n;                        // attention over the paged 4-bit cache: counts of finished spans, zero between launches
     Buf attn;                        // partial results of an attention call whose positions are split over CTAs
     Buf ffn1;                        // the constant logit and the index/weight outputs of a dense FFN run as a one-expert MoE block
     Buf mmak;                        // split-K scratch of the Q8_0 MMA kernel: tile counters + int32 partials, zero between calls
@@ -83,14 +84,17 @@ struct DevCtx {
 // Every entry point that makes a GPU current puts the caller's device back before it returns.
 struct MotyDevGuard {
     int prev = -1;
+    bool moved = false;
     cudaError_t set(int device) {
         if (prev < 0) {
             cudaError_t e = cudaGetDevice(&prev);
             if (e != cudaSuccess) { prev = -1; return e; }
         }
+        if (device == prev && !moved) return cudaSuccess;
+        moved = true;
         return cudaSetDevice(device);
     }
-    ~MotyDevGuard() { if (prev >= 0) cudaSetDevice(prev); }
+    ~MotyDevGuard() { if (moved) cudaSetDevice(prev); }
 };
 #define MOTY_CAT2(a, b) a##b
 #define MOTY_CAT(a, b) MOTY_CAT2(a, b)

@@ -27,7 +27,8 @@ int launch_kv4_append_rope(const Kv4Geom &geo, uint8_t *mem, int layer, int H, f
 int launch_kv4_fetch(const Kv4Geom &geo, const uint8_t *mem, int layer, float *k, float *v, const Kv4Batch &b, int *err, cudaStream_t st);
 // ---- kv4_attend.cu ----
 size_t kv4_attend_scratch_bytes(const Kv4Attend &a, int sms);
-int launch_kv4_attend(const Kv4Attend &a, float *part, int sms, cudaStream_t st);
+size_t kv4_attend_counters(const Kv4Attend &a, int sms);
+int launch_kv4_attend(const Kv4Attend &a, float *part, int *count, int sms, cudaStream_t st);
 // ---- kv4_pages.cu ----
 int launch_kv4_fork(const Kv4Geom &geo, uint8_t *mem, int n, const int *src, const int *dst, const int *fresh, int nseq, int *len,
                     int *table, int ld, int *err, cudaStream_t st);

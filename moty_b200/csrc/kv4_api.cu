@@ -203,8 +203,10 @@ extern "C" int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_d
     a.H = n_heads; a.G = n_heads / kv->geo.KV; a.q = q_dev; a.ctx = ctx_dev; a.max_rows = batch->max_rows; a.max_len = batch->max_len;
     a.window = window; a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)kv->geo.hd); a.err = c->err_dev + 4;
     const size_t sb = kv4_attend_scratch_bytes(a, c->sms);
+    const size_t nc = kv4_attend_counters(a, c->sms) * 4;
     if (sb) CKR(moty_grow(c, &c->attn, sb));
-    return launch_kv4_attend(a, sb ? (float *)c->attn.p : nullptr, c->sms, kv4_stream(c, stream));
+    if (nc) CKR(moty_grow_zero(c, &c->kv4n, nc));
+    return launch_kv4_attend(a, sb ? (float *)c->attn.p : nullptr, nc ? (int *)c->kv4n.p : nullptr, c->sms, kv4_stream(c, stream));
 }
 
 extern "C" int moty_cuda_kv4_fork_dev(MotyCudaKv4 *kv, int n, const int *src_dev, const int *dst_dev, const int *fresh_dev, int nseq,

@@ -12,31 +12,31 @@ namespace {
 // ---- few rows a sequence (decode) ------------------------------------------------------------------------------------
 // A CTA takes one KV head of one sequence, up to 4 or 8 (row, query head) pairs of it ("columns"), and a span of pages.
 // Warp w owns positions 16 w .. 16 w + 15 of every page of the span: it brings their codes and steps to its own ring in
-// shared memory (DEC_ST pages deep, 16-byte asynchronous copies, no barrier beyond the warp) and multiplies
+// shared memory (three or four pages deep, 16-byte asynchronous copies, no barrier beyond the warp) and multiplies
 //     scores  [16 positions x columns] = codes [16 x 32] (a group) * q pieces, times the position's step, group by group
 //     output  [32 dims x columns]     += codes [dims x 16 positions] * (weight * value step) pieces
 // PAIR (up to four columns): hi and lo piece of a column are neighbouring columns of one product and land in the same
 // thread, which adds them.  Otherwise eight columns, and hi and lo are two products into the same sums: the same matrix
 // work a column, half the piece arithmetic.  Every warp keeps its own running maximum (moved only when a score passes it by
-// 8 in base-2 units, so weights stay below 256) and exponent of the largest value step (so that weight * step fits f16:
-// a value 2^9 times smaller than the largest of its 16 positions still has all 22 bits).  Warps join in shared memory, spans
+// 8 in base-2 units, so weights stay below 256) and exponent of the largest value step.  Warps join in shared memory, spans
 // through `part` ({m, l, acc[hd]} per (row, head, split)) and kv4_merge_kernel.
-constexpr int DEC_W = 4, DEC_ST = 4, DEC_NP = 256;           // warps a CTA, ring depth in pages, the most pages of a span
+constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 16, DEC_WK = 7;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, weights' exponent
 
 // CTAs an SM holds (registers)
-constexpr int kv4_decode_ctas(int NG, bool pair) { return NG <= 2 ? 4 : NG <= 4 ? (pair ? 4 : 3) : NG <= 6 ? (pair ? 3 : 2) : 2; }
+constexpr int kv4_decode_ctas(int NG, bool pair) { return NG <= 2 ? 4 : NG <= 4 ? (pair ? 4 : 3) : NG <= 6 ? (pair ? 3 : 2) : pair ? 3 : 2; }
 template <int NG, bool PAIR> struct DecL {
     static constexpr int HD = NG * 32, NC = PAIR ? 4 : 8, STAGE = 18 * HD;       // bytes of 16 positions: codes 2 x 8 HD, steps 2 x HD
     static constexpr int CTAS = kv4_decode_ctas(NG, PAIR);
-    static constexpr int RING = DEC_W * DEC_ST * STAGE, JOIN = DEC_W * NC * HD * 4;
+    static constexpr int ST = NG >= 7 ? 3 : 4;               // ring depth in pages
+    static constexpr int RING = DEC_W * ST * STAGE, JOIN = DEC_W * NC * HD * 4;
     static constexpr int BODY = RING > JOIN ? RING : JOIN;
     static constexpr int SMEM = BODY + NC * HD * 4 + (2 * DEC_W * NC + 4 * NC + DEC_NP) * 4;
 };
 
 template <int NG, bool PAIR>
-__global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
+__global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part, int *count) {
     using Lay = DecL<NG, PAIR>;
-    constexpr int HD = NG * 32, NC = Lay::NC, UNIT = 72 * HD, STAGE = Lay::STAGE, NS = PAIR ? 1 : 2, NCP = (36 * NG + 31) / 32;
+    constexpr int HD = NG * 32, NC = Lay::NC, UNIT = 72 * HD, STAGE = Lay::STAGE, NS = PAIR ? 1 : 2, NCP = (36 * NG + 31) / 32, DEC_ST = Lay::ST;
     extern __shared__ __align__(128) uint8_t sm_kv4[];
     float *js = reinterpret_cast<float *>(sm_kv4);           // the ring, then acc[DEC_W][NC][HD]
     float *qs = reinterpret_cast<float *>(sm_kv4 + Lay::BODY);   // the query rows [NC][HD]
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
     pdl_wait();
     const Kv4Seq sq = kv4_load_seq(a, seq);
     if (!sq.ok) {
-        if (nsplit == 1 && tile == 0) kv4_zero_rows(a, sq, head);
+        if ((nsplit == 1 || (count && split == 0)) && tile == 0) kv4_zero_rows(a, sq, head);
         return;
     }
     const int c0 = tile * NC, ncol = sq.n * a.G - c0 < NC ? sq.n * a.G - c0 : NC;
@@ -153,9 +153,10 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
     }
     const int phi = col[2 * NC + (PAIR ? r >> 1 : r)], plo = a.window > 0 ? phi - a.window + 1 : 0;      // limits of operand column r
     float m[NS], l[NS], acc[NG][2][4];
-    float vth = 0.f, vn = 1.f, vl = 0.f;                     // 2^(e + 1), 64 * 2^-e and its base-2 log, for the exponent e of the largest value step so far
+    float vth = 0.f;                                         // 2^(e + 1) for the exponent e of the largest value step so far
+    int dk = 0;                                              // exponent of the steps' factor; see below
 #pragma unroll
-    for (int k = 0; k < NS; k++) { m[k] = -INFINITY; l[k] = 0.f; }   // m: the running maximum less vl; l and acc: sums of weights times vn
+    for (int k = 0; k < NS; k++) { m[k] = -INFINITY; l[k] = 0.f; }   // m: the running maximum less DEC_WK; l: weights times 2^DEC_WK; acc: times 2^(DEC_WK + dk)
 #pragma unroll
     for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -225,7 +226,9 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                     if (t < clo[k] || t > chi[k]) { see &= ~(1u << (2 * k + h)); s[k][h] = 0.f; }
                 }
         }
-        // the largest value step (NaN left aside) decides the power of two that weight * step is scaled by
+        // Weights (below 256) are scaled by 2^DEC_WK, to below 2^15.  Where the largest value step so far (NaN left aside), of
+        // exponent e, is 1 or more or below 2^-8, steps are scaled by 2^dk, dk = -1 - e: weight * step stays below 2^15 and its
+        // pieces keep their bits.
         {
             __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
 #pragma unroll
@@ -242,12 +245,11 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             }
             const float big = fmaxf(__low2float(mx), __high2float(mx));
             if (__any_sync(0xffffffffu, big >= vth)) {
-                const unsigned b = __reduce_max_sync(0xffffffffu, __float_as_uint(big)) & 0x7f800000u;   // 2^e
+                const unsigned b = __reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23;           // e + 127
                 if (b) {                                     // (f16 subnormals are normal f32; all steps 0: nothing to add, any scale does)
-                    const float nn = 64.f / __uint_as_float(b), f = nn / vn, d = (float)(133 - (int)(b >> 23)) - vl;
-                    vth = 2.f * __uint_as_float(b); vn = nn; vl += d;
-#pragma unroll
-                    for (int k = 0; k < NS; k++) { m[k] -= d; l[k] *= f; }
+                    const int e = (int)b - 127, k = e > -1 || e < -8 ? -1 - e : 0;                       // -16 .. 23
+                    const float f = kv4_pow2(k - dk);
+                    vth = kv4_pow2(e + 1); dk = k;
 #pragma unroll
                     for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         }
         float e[NS][2];                                      // base-2 exponents of the scaled weights
         bool up = false;
-        const float thr = 8.f + vl;
+        constexpr float thr = 8.f + DEC_WK;
 #pragma unroll
         for (int k = 0; k < NS; k++)
 #pragma unroll
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             for (int k = 0; k < NS; k++) {
                 float mx = m[k];
 #pragma unroll
-                for (int h = 0; h < 2; h++) if (see >> (2 * k + h) & 1) mx = fmaxf(mx, s[k][h] * desc[k] - vl);
+                for (int h = 0; h < 2; h++) if (see >> (2 * k + h) & 1) mx = fmaxf(mx, s[k][h] * desc[k] - (float)DEC_WK);
                 for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                 float f = mx == -INFINITY ? 1.f : kv4_exp2(m[k] - mx);
                 m[k] = mx; l[k] *= f;
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                     }
             }
         }
-        // scaled weights (weight * step * vn < 256 * 2 * 64 = 2^15) of positions 2 j, 2 j + 1, 2 j + 8, 2 j + 9 for column r
+        // scaled weights of positions 2 j, 2 j + 1, 2 j + 8, 2 j + 9 for column r
         float y[4];
         bool hide[4];
         {
@@ -328,22 +330,34 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             kv4_ldsw<NG>(vb, sg + 12 * HD + lane * (4 * NG));
             kv4_ldsw<NG>(wa, sg + 17 * HD + 2 * j * (2 * NG));
             kv4_ldsw<NG>(wb, sg + 17 * HD + (8 + 2 * j) * (2 * NG));
+            if (dk) {                                        // (f16 ends at 2^15: the rest in a second step)
+                const __half2 f1 = __float2half2_rn(kv4_pow2(dk < 15 ? dk : 15)), f2 = __float2half2_rn(kv4_pow2(dk < 15 ? 0 : dk - 15));
+                const unsigned u1 = *reinterpret_cast<const unsigned *>(&f1), u2 = *reinterpret_cast<const unsigned *>(&f2);
+#pragma unroll
+                for (int g = 0; g < NG; g++) { wa[g] = kv4_hmul2(kv4_hmul2(wa[g], u1), u2); wb[g] = kv4_hmul2(kv4_hmul2(wb[g], u1), u2); }
+            }
+            // weight * step in f16 pairs of positions: with y = yh + yl, hi = round(yh d), lo = round(yl d + (yh d - hi)); the
+            // remainder of hi is exact, lo's rounding is 2^-22 of the product
+            unsigned yh[2], yl[2];
+            kv4_pieces(y[0], y[1], yh[0], yl[0]);
+            kv4_pieces(y[2], y[3], yh[1], yl[1]);
             unsigned b[NS][NG][2];                           // operand columns: PAIR: this lane's piece; else hi and lo
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                float x[4] = {y[0] * kv4_half_of(wa[g >> 1], g & 1), y[1] * kv4_half_of(wa[(NG + g) >> 1], (NG + g) & 1),
-                              y[2] * kv4_half_of(wb[g >> 1], g & 1), y[3] * kv4_half_of(wb[(NG + g) >> 1], (NG + g) & 1)};
-                if (!inside) {                               // a position that is not seen adds nothing, whatever its step holds
+            for (int g = 0; g < NG; g++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) if (hide[i]) x[i] = 0.f;
+                for (int q = 0; q < 2; q++) {
+                    const unsigned *w = q ? wb : wa;
+                    const int i1 = NG + g;                   // steps of positions 2 j (+ 8 q) and the next: halves g and NG + g
+                    const unsigned d = __byte_perm(w[g >> 1], w[i1 >> 1], (g & 1 ? 0x32 : 0x10) | (i1 & 1 ? 0x7600 : 0x5400));
+                    unsigned hi, lo;
+                    kv4_scaled_pieces(yh[q], yl[q], d, hi, lo);
+                    if (!inside) {                           // a position that is not seen adds nothing, whatever its step holds
+                        const unsigned keep = (hide[2 * q] ? 0u : 0xffffu) | (hide[2 * q + 1] ? 0u : 0xffff0000u);
+                        hi &= keep; lo &= keep;
+                    }
+                    if (PAIR) b[0][g][q] = r & 1 ? lo : hi;
+                    else { b[0][g][q] = hi; b[NS - 1][g][q] = lo; }
                 }
-                if (PAIR) {
-                    b[0][g][0] = kv4_piece(x[0], x[1], sel); b[0][g][1] = kv4_piece(x[2], x[3], sel);
-                } else {
-                    kv4_pieces(x[0], x[1], b[0][g][0], b[NS - 1][g][0]);
-                    kv4_pieces(x[2], x[3], b[0][g][1], b[NS - 1][g][1]);
-                }
-            }
             constexpr int GB = NG % 2 == 0 ? 2 : NG == 3 ? 3 : 1;
 #pragma unroll
             for (int g0 = 0; g0 < NG; g0 += GB) {
@@ -366,7 +380,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
     // join the warps: a thread holds dims 32 g + 4 r + 0 .. 3 of its score columns
     cp_async_wait<0>();
     __syncthreads();
-    const float vs = 1.f / vn;                               // (a power of two)
+    const float vs = kv4_pow2(-DEC_WK - dk), ls = kv4_pow2(-DEC_WK);
 #pragma unroll
     for (int k = 0; k < NS; k++) {
         for (int o = 4; o < 32; o <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], o);
@@ -378,7 +392,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             for (int i = 0; i < 4; i++) o[i] = (PAIR ? acc[g][i >> 1][(i & 1) * 2] + acc[g][i >> 1][(i & 1) * 2 + 1] : acc[g][i >> 1][(i & 1) * 2 + k]) * vs;
             *reinterpret_cast<float4 *>(js + ((size_t)warp * NC + c) * HD + g * 32 + 4 * r) = make_float4(o[0], o[1], o[2], o[3]);
         }
-        if (r == 0) { ml[warp * NC + c] = m[k] + vl; ml[DEC_W * NC + warp * NC + c] = l[k] * vs; }
+        if (r == 0) { ml[warp * NC + c] = m[k] + (float)DEC_WK; ml[DEC_W * NC + warp * NC + c] = l[k] * ls; }
     }
     __syncthreads();
     if (warp == 0 && lane < NC) {                            // the factor of each warp's sums; m and l of all
@@ -416,6 +430,42 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             if (d == 0) { p[0] = ml[2 * DEC_W * NC + c]; p[1] = L; }
         }
     }
+    if (!count) return;
+    // few spans: the CTA that finishes last joins them, in the spans' order (the same sums whichever it is)
+    int live = (cr.hi_any - (cr.lo_any & ~(KV4_PAGE - 1)) + span - 1) / span;
+    if (live > nsplit) live = nsplit;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) col[0] = atomicAdd(&count[u], 1) == live - 1 ? col[0] : -1;
+    __syncthreads();
+    if (col[0] < 0) return;
+    __threadfence();
+    for (int c = warp; c < ncol; c += DEC_W) {               // a warp a column, lane k the span k's {m, l}
+        const size_t rh = (size_t)col[c] * a.H + col[NC + c];
+        const float *p = part + rh * nsplit * (HD + 4);
+        const float2 e = lane < live ? __ldcg(reinterpret_cast<const float2 *>(p + (size_t)lane * (HD + 4))) : make_float2(-INFINITY, 0.f);
+        float M = e.x;
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float f = e.y == 0.f ? 0.f : kv4_exp2(e.x - M);
+        float L = e.y * f;
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+#pragma unroll
+        for (int d0 = 0; d0 < HD / 4; d0 += 32) {
+            const int d = 4 * (d0 + lane);
+            const bool mine = d < HD;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int k = 0; k < live; k++) {
+                const float fk = __shfl_sync(0xffffffffu, f, k);
+                const float4 v = mine ? __ldcg(reinterpret_cast<const float4 *>(p + (size_t)k * (HD + 4) + 4 + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (fk != 0.f) { o.x = fmaf(v.x, fk, o.x); o.y = fmaf(v.y, fk, o.y); o.z = fmaf(v.z, fk, o.z); o.w = fmaf(v.w, fk, o.w); }
+            }
+            if (mine)
+                *reinterpret_cast<float4 *>(a.ctx + rh * HD + d) = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                    : make_float4(__fdiv_rn(o.x, L), __fdiv_rn(o.y, L), __fdiv_rn(o.z, L), __fdiv_rn(o.w, L));
+        }
+    }
+    if (tid == 0) count[u] = 0;                              // as the next launch finds it
 }
 
 // joins the spans of one (row, head): the same sums over {m, l, acc} with the maximum over all spans
@@ -527,7 +577,7 @@ size_t kv4_attend_scratch_bytes(const Kv4Attend &a, int sms) {
 }
 
 template <int NG, bool PAIR>
-static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st) {
+static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *count, cudaStream_t st) {
     constexpr size_t smem = DecL<NG, PAIR>::SMEM;
     static bool attr[MOTY_MAX_DEV];
     int dev = 0;
@@ -539,32 +589,39 @@ static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, cuda
     }
     const long long grid = (long long)a.b.nseq * a.geo.KV * p.ntile * p.nsplit;
     if (grid > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend: %lld CTAs", grid);
-    CK(moty_launch_pdl(kv4_decode_kernel<NG, PAIR>, dim3((unsigned)grid), dim3(DEC_W * 32), smem, st, a, p.ntile, p.nsplit, p.span, part));
+    CK(moty_launch_pdl(kv4_decode_kernel<NG, PAIR>, dim3((unsigned)grid), dim3(DEC_W * 32), smem, st, a, p.ntile, p.nsplit, p.span, part, count));
     return 0;
 }
 template <int NG>
-static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st) {
-    return p.cols == 4 ? kv4_decode_go<NG, true>(a, p, part, st) : kv4_decode_go<NG, false>(a, p, part, st);
+static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *count, cudaStream_t st) {
+    return p.cols == 4 ? kv4_decode_go<NG, true>(a, p, part, count, st) : kv4_decode_go<NG, false>(a, p, part, count, st);
 }
 
-int launch_kv4_attend(const Kv4Attend &a, float *part, int sms, cudaStream_t st) {
+// CTAs that count their spans' ends, when few spans are joined in the launch itself
+size_t kv4_attend_counters(const Kv4Attend &a, int sms) {
+    const Kv4Plan p = kv4_plan(a, sms);
+    return p.decode && p.nsplit > 1 && p.nsplit <= DEC_JOIN ? (size_t)a.b.nseq * a.geo.KV * p.ntile : 0;
+}
+
+// part: scratch of kv4_attend_scratch_bytes; count: kv4_attend_counters ints, all zero (and left so)
+int launch_kv4_attend(const Kv4Attend &a, float *part, int *count, int sms, cudaStream_t st) {
     const Kv4Plan p = kv4_plan(a, sms);
     if (p.nsplit > 1 && !part) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: scratch for %d spans missing", p.nsplit);
     int rc = 0;
     if (p.tc) rc = launch_kv4_prompt_tc(a, p, part, st);
     else if (!p.decode) rc = launch_kv4_prompt(a, p, part, st);
     else switch (a.geo.hd / 32) {
-        case 1: rc = kv4_decode_go<1>(a, p, part, st); break;
-        case 2: rc = kv4_decode_go<2>(a, p, part, st); break;
-        case 3: rc = kv4_decode_go<3>(a, p, part, st); break;
-        case 4: rc = kv4_decode_go<4>(a, p, part, st); break;
-        case 5: rc = kv4_decode_go<5>(a, p, part, st); break;
-        case 6: rc = kv4_decode_go<6>(a, p, part, st); break;
-        case 7: rc = kv4_decode_go<7>(a, p, part, st); break;
-        default: rc = kv4_decode_go<8>(a, p, part, st); break;
+        case 1: rc = kv4_decode_go<1>(a, p, part, count, st); break;
+        case 2: rc = kv4_decode_go<2>(a, p, part, count, st); break;
+        case 3: rc = kv4_decode_go<3>(a, p, part, count, st); break;
+        case 4: rc = kv4_decode_go<4>(a, p, part, count, st); break;
+        case 5: rc = kv4_decode_go<5>(a, p, part, count, st); break;
+        case 6: rc = kv4_decode_go<6>(a, p, part, count, st); break;
+        case 7: rc = kv4_decode_go<7>(a, p, part, count, st); break;
+        default: rc = kv4_decode_go<8>(a, p, part, count, st); break;
     }
     CKR(rc);
-    if (p.nsplit > 1)
+    if (p.nsplit > 1 && !count)
         CK(moty_launch_pdl(kv4_merge_kernel, dim3(a.b.rows, a.H), dim3(MG_T), (size_t)0, st, a, p, (const float *)part));
     return 0;
 }

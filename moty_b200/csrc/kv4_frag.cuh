@@ -119,6 +119,17 @@ __device__ __forceinline__ void kv4_pieces(float x0, float x1, unsigned &h, unsi
     kv4_rest(x0, x1, h, KV4_HM1);
     lo = kv4_pack_f16(x0, x1);
 }
+__device__ __forceinline__ unsigned kv4_hmul2(unsigned a, unsigned b) {
+    const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+// (yh + yl) d as hi + lo, pairs of f16
+__device__ __forceinline__ void kv4_scaled_pieces(unsigned yh, unsigned yl, unsigned d, unsigned &hi, unsigned &lo) {
+    const __half2 a = *reinterpret_cast<const __half2 *>(&yh), b = *reinterpret_cast<const __half2 *>(&yl), c = *reinterpret_cast<const __half2 *>(&d);
+    const __half2 h = __hmul2(a, c), l = __hfma2(b, c, __hfma2(a, c, __hneg2(h)));
+    hi = *reinterpret_cast<const unsigned *>(&h);
+    lo = *reinterpret_cast<const unsigned *>(&l);
+}
 // 2^k for -126 <= k <= 127, and x 2^k for any k of the f32 range (two factors, each a normal number)
 __device__ __forceinline__ float kv4_pow2(int k) { return __int_as_float((k + 127) << 23); }
 __device__ __forceinline__ float kv4_scale2(float x, int k) { const int h = k >> 1; return x * kv4_pow2(h) * kv4_pow2(k - h); }
