@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                 if (w == 0) sh.fk[j & 7] = f;
                 // the keys of page j - 1 are done with (a warp that gives up goes on to the next barrier, where all leave)
                 if (j > 0 && !warp_wait(&sh.sfull[nx - 1][(j - 1) & 1], (j - 1) >> 1 & 1, abort_flag)) continue;
-#pragma unroll
+#pragma unroll 1
                 for (int it = w; it < 256; it += PT_KT) {    // position t, piece jj of a group's four
                     const int t = (it >> 5) * 8 + (it & 7), jj = it >> 3 & 3;
                     unsigned kw[NG], st[(NG + 1) / 2];
@@ -431,16 +431,17 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                 const bool inside = t0 >= cr.lo_all && t0 + KV4_PAGE <= cr.hi_all;
                 const uint32_t at = mine + TM_S + (x * 2 + (j & 1)) * 64;
                 float mx = -INFINITY;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float v[32];
-                    tm_ld32(v, at + h * 32);
+                // (loops kept rolled: unrolled, the roles' code together outgrew the instruction cache)
+#pragma unroll 1
+                for (int q = 0; q < 4; q++) {
+                    float v[16];
+                    tm_ld16(v, at + q * 16);
                     if (!inside) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) { const int t = t0 + h * 32 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
+                        for (int i = 0; i < 16; i++) { const int t = t0 + q * 16 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, v[i]);
+                    for (int i = 0; i < 16; i++) mx = fmaxf(mx, v[i]);
                 }
                 mx *= ds;                                    // (the scale is positive)
                 const bool up = mx > m + 8.f;
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                 // and 8 of lo (a line that has seen nothing yet: all 0)
                 const float mm = m == -INFINITY ? 0.f : m - 6.f;
                 float s0 = 0.f, s1 = 0.f;
-#pragma unroll
+#pragma unroll 1
                 for (int q = 0; q < 4; q++) {
                     float v[16];
                     tm_ld16(v, at + q * 16);
