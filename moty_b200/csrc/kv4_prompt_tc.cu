@@ -433,15 +433,15 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                 float mx = -INFINITY;
                 // (loops kept rolled: unrolled, the roles' code together outgrew the instruction cache)
 #pragma unroll 1
-                for (int q = 0; q < 4; q++) {
-                    float v[16];
-                    tm_ld16(v, at + q * 16);
+                for (int q = 0; q < 2; q++) {
+                    float v[32];
+                    tm_ld32(v, at + q * 32);
                     if (!inside) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) { const int t = t0 + q * 16 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
+                        for (int i = 0; i < 32; i++) { const int t = t0 + q * 32 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; i++) mx = fmaxf(mx, v[i]);
+                    for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(v[i], v[i + 1]));
                 }
                 mx *= ds;                                    // (the scale is positive)
                 const bool up = mx > m + 8.f;
