@@ -132,21 +132,27 @@ __global__ void __launch_bounds__(ST_T) kv4_append_kernel(Kv4Geom geo, uint8_t *
     const int tid = threadIdx.x, hd = geo.hd, NG = hd >> 5, row0 = blockIdx.x * ST_ROWS, head = blockIdx.y;
     pdl_trigger();
     pdl_wait();
-    kv4_rows(rs, geo, mem, b, row0, layer, head, err, false);
     const int per = hd >> 3, items = ST_ROWS * per;            // eight dims an item; a quad never leaves its group
-    for (int it = tid; it < (items + ST_T - 1) / ST_T * ST_T; it += ST_T) {
-        const int i = it / per, d8 = it - i * per, g = d8 >> 2, j = d8 & 3;
-        uint8_t *unit = it < items ? rs.unit[i] : nullptr;
-        float kx[8], vx[8];
+    const unsigned nth = 65535u / (unsigned)NG + 1;            // n / NG = n nth >> 16 for n < 65536 / NG: here n <= 1024
+    float kx[8], vx[8];
+    auto load = [&](int it) {
+        const int i = (int)((unsigned)(it >> 2) * nth >> 16), d8 = it - i * per;
 #pragma unroll
         for (int e = 0; e < 8; e++) kx[e] = vx[e] = 0.f;
-        if (unit) {
+        if (it < items && row0 + i < b.rows) {
             const size_t at = (size_t)(row0 + i) * ld + (size_t)head * hd + d8 * 8;
             *reinterpret_cast<float4 *>(kx) = *reinterpret_cast<const float4 *>(k + at);
             *reinterpret_cast<float4 *>(kx + 4) = *reinterpret_cast<const float4 *>(k + at + 4);
             *reinterpret_cast<float4 *>(vx) = *reinterpret_cast<const float4 *>(v + at);
             *reinterpret_cast<float4 *>(vx + 4) = *reinterpret_cast<const float4 *>(v + at + 4);
         }
+    };
+    load(tid);                                                 // on its way while the rows are looked up
+    kv4_rows(rs, geo, mem, b, row0, layer, head, err, false);
+    for (int it = tid; it < (items + ST_T - 1) / ST_T * ST_T; it += ST_T) {
+        const int i = (int)((unsigned)(it >> 2) * nth >> 16), d8 = it - i * per, g = d8 >> 2, j = d8 & 3;
+        uint8_t *unit = it < items ? rs.unit[i] : nullptr;
+        if (it != tid) load(it);
         unsigned short kd, vd;
         const float ks = kv4_quad_step(kx, &kd), vs = kv4_quad_step(vx, &vd);
         if (unit) {
@@ -160,7 +166,7 @@ __global__ void __launch_bounds__(ST_T) kv4_append_kernel(Kv4Geom geo, uint8_t *
     }
     __syncthreads();
     for (int it = tid; it < ST_ROWS * NG * 8; it += ST_T) {    // [r][row][g]: consecutive threads, consecutive bytes of a block
-        const int g = it % NG, q = it / NG, i = q % ST_ROWS, r = q / ST_ROWS;
+        const int q = (int)((unsigned)it * nth >> 16), g = it - q * NG, i = q % ST_ROWS, r = q / ST_ROWS;
         uint8_t *unit = rs.unit[i];
         if (!unit) continue;
         const int t = rs.t[i];
