@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
 #pragma unroll
         for (int w = 0; w < DEC_W; w++) {
             const float lw = ml[DEC_W * NC + w * NC + lane];
-            f[w] = lw == 0.f ? 0.f : kv4_exp2(ml[w * NC + lane] - M);
+            f[w] = kv4_factor(lw, ml[w * NC + lane], M);
             L = fmaf(lw, f[w], L);
         }
 #pragma unroll
@@ -422,8 +422,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         const float L = ml[DEC_W * NC + c];
         const size_t rh = (size_t)col[c] * a.H + col[NC + c];
         if (nsplit == 1) {
-            *reinterpret_cast<float4 *>(a.ctx + rh * HD + d) = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                : make_float4(__fdiv_rn(o.x, L), __fdiv_rn(o.y, L), __fdiv_rn(o.z, L), __fdiv_rn(o.w, L));
+            *reinterpret_cast<float4 *>(a.ctx + rh * HD + d) = kv4_times(o, kv4_over(L));
         } else {
             float *p = part + (rh * nsplit + split) * (HD + 4);
             *reinterpret_cast<float4 *>(p + 4 + d) = o;
@@ -446,7 +445,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         const float2 e = lane < live ? __ldcg(reinterpret_cast<const float2 *>(p + (size_t)lane * (HD + 4))) : make_float2(-INFINITY, 0.f);
         float M = e.x;
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float f = e.y == 0.f ? 0.f : kv4_exp2(e.x - M);
+        const float f = kv4_factor(e.y, e.x, M);
         float L = e.y * f;
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
 #pragma unroll
@@ -461,37 +460,72 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                 if (fk != 0.f) { o.x = fmaf(v.x, fk, o.x); o.y = fmaf(v.y, fk, o.y); o.z = fmaf(v.z, fk, o.z); o.w = fmaf(v.w, fk, o.w); }
             }
             if (mine)
-                *reinterpret_cast<float4 *>(a.ctx + rh * HD + d) = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                    : make_float4(__fdiv_rn(o.x, L), __fdiv_rn(o.y, L), __fdiv_rn(o.z, L), __fdiv_rn(o.w, L));
+                *reinterpret_cast<float4 *>(a.ctx + rh * HD + d) = kv4_times(o, kv4_over(L));
         }
     }
     if (tid == 0) count[u] = 0;                              // as the next launch finds it
 }
 
-// joins the spans of one (row, head): the same sums over {m, l, acc} with the maximum over all spans
+// What the join of a (row, head) needs: how many of its spans hold something (the row's column tile decides), 0: the row is
+// refused and reads as zeros, -1: no sequence has the row.
+__device__ __forceinline__ int kv4_live_spans(const Kv4Attend &a, const Kv4Plan &pl, int row, int h) {
+    int seq, pos;
+    const int st = kv4_row(a.b, row, &seq, &pos);
+    if (st == KV4_ROW_NONE) return -1;
+    if (st == KV4_ROW_BAD) return 0;
+    const int n = a.b.row0[seq + 1] - a.b.row0[seq], len = a.b.len[seq];
+    if (n > a.max_rows || len > a.max_len) return 0;
+    const long long c = (long long)(row - a.b.row0[seq]) * a.G + h % a.G, c0 = c / pl.cols * pl.cols, last = (long long)n * a.G - 1;
+    const long long cz = c0 + pl.cols - 1 < last ? c0 + pl.cols - 1 : last;
+    const Kv4Range cr = kv4_range(a, len - n + (int)(c0 / a.G), len - n + (int)(cz / a.G));
+    const int live = (cr.hi_any - (cr.lo_any & ~(KV4_PAGE - 1)) + pl.span - 1) / pl.span;
+    return live < pl.nsplit ? live : pl.nsplit;
+}
+// joins up to 32 spans of one (row, head), a warp each, a span's {m, l} a lane
 constexpr int MG_T = 256;
+__global__ void __launch_bounds__(MG_T) kv4_merge_few_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
+    const int hd = a.geo.hd, lane = threadIdx.x & 31, q4 = hd >> 2;
+    const long long item = (long long)blockIdx.x * (MG_T / 32) + (threadIdx.x >> 5);
+    pdl_trigger();
+    pdl_wait();
+    const int row = (int)(item / a.H), h = (int)(item - (long long)row * a.H);
+    if (row >= a.b.rows) return;
+    const int live = kv4_live_spans(a, pl, row, h);
+    if (live < 0) return;
+    const float *p = part + (size_t)item * pl.nsplit * (hd + 4);
+    const bool mine = lane < live;
+    const float2 ml = mine ? *reinterpret_cast<const float2 *>(p + (size_t)lane * (hd + 4)) : make_float2(-INFINITY, 0.f);
+    const float M = warp_max_f32(ml.x), f = kv4_factor(ml.y, ml.x, M);
+    float L = ml.y * f;
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    const unsigned some = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    for (int d0 = 0; d0 < q4; d0 += 32) {
+        const int d = d0 + lane < q4 ? d0 + lane : d0;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < live; i0 += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = reinterpret_cast<const float4 *>(p + (size_t)(i0 + u < live ? i0 + u : i0) * (hd + 4) + 4)[d];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float fi = __shfl_sync(0xffffffffu, f, i0 + u);
+                if (some >> (i0 + u) & 1) { o.x = fmaf(v[u].x, fi, o.x); o.y = fmaf(v[u].y, fi, o.y); o.z = fmaf(v[u].z, fi, o.z); o.w = fmaf(v[u].w, fi, o.w); }
+            }
+        }
+        if (d0 + lane < q4) reinterpret_cast<float4 *>(a.ctx + (size_t)item * hd)[d] = kv4_times(o, kv4_over(L));
+    }
+}
+
+// joins the many spans of one (row, head): the same sums over {m, l, acc}, a CTA each
 __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
     __shared__ float red[MG_T / 32], ls[MG_T / 8];
     __shared__ float4 os[MG_T];
     const int row = blockIdx.x, h = blockIdx.y, hd = a.geo.hd, tid = threadIdx.x;
     pdl_trigger();
     pdl_wait();
-    int seq, pos;
-    const int st = kv4_row(a.b, row, &seq, &pos);
-    if (st == KV4_ROW_NONE) return;
+    const int live = kv4_live_spans(a, pl, row, h);
+    if (live < 0) return;
     float *out = a.ctx + ((size_t)row * a.H + h) * hd;
-    const int n = st == KV4_ROW_OK ? a.b.row0[seq + 1] - a.b.row0[seq] : 0;
-    if (st == KV4_ROW_BAD || n > a.max_rows || a.b.len[seq] > a.max_len) {
-        if (tid < hd) out[tid] = 0.f;
-        return;
-    }
-    // the spans that hold anything for this row's column tile
-    const long long c = (long long)(row - a.b.row0[seq]) * a.G + h % a.G, c0 = c / pl.cols * pl.cols, last = (long long)n * a.G - 1;
-    const long long cz = c0 + pl.cols - 1 < last ? c0 + pl.cols - 1 : last;
-    const int pos0 = a.b.len[seq] - n;
-    const Kv4Range cr = kv4_range(a, pos0 + (int)(c0 / a.G), pos0 + (int)(cz / a.G));
-    int live = (cr.hi_any - (cr.lo_any & ~(KV4_PAGE - 1)) + pl.span - 1) / pl.span;
-    if (live > pl.nsplit) live = pl.nsplit;
     const float *p = part + ((size_t)row * a.H + h) * pl.nsplit * (hd + 4);
     float M = -INFINITY;
     for (int i = tid; i < live; i += MG_T) M = fmaxf(M, p[(size_t)i * (hd + 4)]);
@@ -507,7 +541,7 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
     if (k < ng)
         for (int i = k; i < live; i += ng) {
             const float *pi = p + (size_t)i * (hd + 4);
-            const float li = pi[1], f = li == 0.f ? 0.f : kv4_exp2(pi[0] - M);
+            const float li = pi[1], f = kv4_factor(li, pi[0], M);
             const float4 v = *reinterpret_cast<const float4 *>(pi + 4 + 4 * d);
             L = fmaf(li, f, L);
             if (li != 0.f) { o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w); }
@@ -519,8 +553,7 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
             const float4 v = os[i * q4 + d];
             L += ls[i]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
         }
-        *reinterpret_cast<float4 *>(out + 4 * d) = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-            : make_float4(__fdiv_rn(o.x, L), __fdiv_rn(o.y, L), __fdiv_rn(o.z, L), __fdiv_rn(o.w, L));
+        *reinterpret_cast<float4 *>(out + 4 * d) = kv4_times(o, kv4_over(L));
     }
 }
 
@@ -538,8 +571,9 @@ static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     Kv4Plan p{};
     const long long cols = (long long)a.max_rows * a.G;
     const int NG = a.geo.hd / 32;
-    p.decode = cols <= 32;
-    p.tc = cols > KV4_LINES && NG >= 2 && NG <= 4;
+    p.decode = cols <= (NG == 3 || NG == 4 ? 48 : 64);
+    const long long pages64 = (long long)a.b.nseq * a.geo.KV * ((cols + 63) / 64) * ((a.max_len + KV4_PAGE - 1) / KV4_PAGE);
+    p.tc = cols > KV4_LINES && NG >= 2 && NG <= 4 && pages64 > 6LL * sms;
     p.cols = p.tc ? KV4_TC_LINES : !p.decode ? KV4_LINES : cols > 4 ? 8 : 4;
     p.ntile = (int)((cols + p.cols - 1) / p.cols);
     if (p.ntile < 1) p.ntile = 1;
@@ -621,7 +655,10 @@ int launch_kv4_attend(const Kv4Attend &a, float *part, int *count, int sms, cuda
         default: rc = kv4_decode_go<8>(a, p, part, count, st); break;
     }
     CKR(rc);
-    if (p.nsplit > 1 && !count)
-        CK(moty_launch_pdl(kv4_merge_kernel, dim3(a.b.rows, a.H), dim3(MG_T), (size_t)0, st, a, p, (const float *)part));
+    if (p.nsplit > 1 && !count) {
+        if (p.nsplit <= 32)
+            CK(moty_launch_pdl(kv4_merge_few_kernel, dim3((unsigned)(((long long)a.b.rows * a.H + MG_T / 32 - 1) / (MG_T / 32))), dim3(MG_T), (size_t)0, st, a, p, (const float *)part));
+        else CK(moty_launch_pdl(kv4_merge_kernel, dim3(a.b.rows, a.H), dim3(MG_T), (size_t)0, st, a, p, (const float *)part));
+    }
     return 0;
 }

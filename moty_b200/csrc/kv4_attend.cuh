@@ -30,6 +30,13 @@ __device__ __forceinline__ void kv4_zero_rows(const Kv4Attend &a, const Kv4Seq &
     for (long long r = lo; r < hi; r++)
         for (int i = threadIdx.x; i < w; i += blockDim.x) a.ctx[r * a.H * a.geo.hd + (size_t)head * w + i] = 0.f;
 }
+// a finished row: its sums over the weights' total l, zeros where nothing was seen (times a reciprocal: half a step of f32
+// more than the quotient, and a prompt's CTA spends 3 us less on its rows)
+__device__ __forceinline__ float kv4_over(float l) { return l == 0.f ? 0.f : __frcp_rn(l); }
+__device__ __forceinline__ float4 kv4_times(const float4 &o, float f) { return make_float4(o.x * f, o.y * f, o.z * f, o.w * f); }
+// What sums over a part with maximum m count where the whole's is M; never 0 where the part saw anything (l > 0), for a NaN
+// among its values has to stay one however small its weight.
+__device__ __forceinline__ float kv4_factor(float l, float m, float M) { return l == 0.f ? 0.f : fmaxf(kv4_exp2(m - M), 1.17549435e-38f); }
 // rows at positions p_a .. p_z: [lo_any, hi_any) is seen by some of them, [lo_all, hi_all) by all
 struct Kv4Range { int lo_any, hi_any, lo_all, hi_all; };
 __device__ __forceinline__ Kv4Range kv4_range(const Kv4Attend &a, int p_a, int p_z) {

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
         float f = vs;
         if (nsplit == 1) {
             out = a.ctx + rh * HD;
-            f = l[hlf] == 0.f ? 0.f : vs;
+            f = vs * kv4_over(l[hlf]);
         } else {
             out = part + (rh * nsplit + split) * (HD + 4) + 4;
             if (j == 0) { out[-4] = m[hlf]; out[-3] = l[hlf]; }
@@ -304,10 +304,7 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
             for (int k = 0; k < 2; k++) {
                 float o[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    o[i] = acc[g][i][2 * hlf + k] * f;
-                    if (nsplit == 1) o[i] = l[hlf] == 0.f ? 0.f : __fdiv_rn(o[i], l[hlf]);
-                }
+                for (int i = 0; i < 4; i++) o[i] = acc[g][i][2 * hlf + k] * f;
                 *reinterpret_cast<float4 *>(out + g * 32 + 8 * j + 4 * k) = make_float4(o[0], o[1], o[2], o[3]);
             }
     }

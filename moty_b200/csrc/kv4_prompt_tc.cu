@@ -168,7 +168,6 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
     if (tid == 0) {
         sh.abort = 0;
         mbar_init(&sh.kfull, PT_KT); mbar_init(&sh.vfull, PT_VT);
-        for (int i = 0; i < 2; i++) { mbar_init(&sh.rawk[i], 1); mbar_init(&sh.rawv[i], 1); }
         for (int x = 0; x < 2; x++) {
             for (int i = 0; i < 2; i++) { mbar_init(&sh.sfull[x][i], 1); mbar_init(&sh.pfull[x][i], PT_M); }
             mbar_init(&sh.pvdone[x], 1); mbar_init(&sh.oempty[x], PT_M);
@@ -180,6 +179,20 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // pages as they lie in memory, two in flight
+    const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
+    const size_t page_bytes = kv4_page_bytes(a.geo);
+    auto load_k = [&](int j) {                               // key codes and steps are one run of bytes
+        mbar_expect_tx(&sh.rawk[j & 1], 36 * HD);
+        bulk_load(sm + L::OFF_RAW + (j & 1) * L::RAW, base + (size_t)list[j].x * page_bytes, 36 * HD, &sh.rawk[j & 1]);
+    };
+    auto load_v = [&](int j) {
+        uint8_t *dst = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
+        const uint8_t *src = base + (size_t)list[j].x * page_bytes + kv4_v_code_off(HD);
+        mbar_expect_tx(&sh.rawv[j & 1], 36 * HD);
+        for (int o = 0; o < 8; o++) bulk_load(dst + o * L::VS, src + o * (4 * HD), 4 * HD, &sh.rawv[j & 1]);     // apart by 16 bytes: eight halves, eight bank groups
+        bulk_load(dst + L::RV, src + 32 * HD, 4 * HD, &sh.rawv[j & 1]);
+    };
     if (warp == 8) {                                         // the pages of the span that are there, in order
         const int np = t_hi > t_lo ? (t_hi - t_lo + KV4_PAGE - 1) / KV4_PAGE : 0;
         const int *tab = a.b.table + (size_t)seq * a.b.ld + t_lo / KV4_PAGE;
@@ -192,7 +205,14 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
             if (ok) list[n + __popc(m & ((1u << lane) - 1))] = make_int2(id, t_lo + i * KV4_PAGE);
             n += __popc(m);
         }
-        if (lane == 0) sh.n = n;
+        __syncwarp();
+        if (lane == 0) {
+            sh.n = n;
+            for (int i = 0; i < 2; i++) { mbar_init(&sh.rawk[i], 1); mbar_init(&sh.rawv[i], 1); }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            for (int j = 0; j < 2 && j < n; j++) { load_k(j); load_v(j); }         // on their way while the queries are prepared
+        }
     }
     // a softmax thread's line: its query row, limits, scale; the row goes to shared memory in two pieces
     float desc = 0.f;
@@ -210,33 +230,41 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
             chi = p;
             clo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
         }
+        // LPR lanes bring a row (a lane the eight dims of a piece), so that a warp's loads touch few lines of memory
+        constexpr int LPR = NG == 2 ? 8 : 16, RPI = 32 / LPR;
+        const int c = lane % LPR, sub = lane / LPR;          // piece c = 4 g + j: dims 8 c + 0, 4, 1, 5, 2, 6, 3, 7 (the order of a code word's pairs)
         unsigned mb = 0;
-        if (have)
-#pragma unroll 8
-            for (int i = 0; i < HD / 4; i++) {
-                const uint4 v = reinterpret_cast<const uint4 *>(src)[i];
-                mb = max(max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu)), mb);
+#pragma unroll 4
+        for (int i0 = 0; i0 < 32; i0 += RPI) {
+            const int line = (warp & 3) * 32 + i0 + sub;     // of the tile
+            const float *from = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), i0 + sub));
+            float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+            if (x * PT_M + line < ncol && c < 4 * NG) {
+                v0 = reinterpret_cast<const float4 *>(from)[2 * c];
+                v1 = reinterpret_cast<const float4 *>(from)[2 * c + 1];
             }
-        const bool fin = mb < 0x7f800000u;
-        const int k = fin ? kv4_q_shift(mb) : 0;
-        // (not below the smallest normal number: -infinity times it has to stay -infinity)
-        desc = fin ? fmaxf(kv4_scale2(a.scale * 1.44269504f, -k), 1.17549435e-38f) : __int_as_float(0x7fffffff);
-#pragma unroll 2
-        for (int c = 0; c < NG * 4; c++) {                   // piece c = 4 g + j: dims 8 c + 0, 4, 1, 5, 2, 6, 3, 7 (the order of a code word's pairs)
-            float y[8];
+            const float y[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+            unsigned m = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = 0.f;
-            if (have && fin) {
-                const float4 v0 = reinterpret_cast<const float4 *>(src)[2 * c], v1 = reinterpret_cast<const float4 *>(src)[2 * c + 1];
-                y[0] = v0.x; y[1] = v0.y; y[2] = v0.z; y[3] = v0.w; y[4] = v1.x; y[5] = v1.y; y[6] = v1.z; y[7] = v1.w;
-            }
+            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(y[i]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const unsigned own = __shfl_sync(0xffffffffu, m, lane % RPI * LPR);
+            if (lane / RPI * RPI == i0) mb = own;
+            const bool fin = m < 0x7f800000u;
+            const int k = fin ? kv4_q_shift(m) : 0;
             unsigned h[4], l[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) kv4_pieces(kv4_scale2(y[i], k), kv4_scale2(y[i + 4], k), h[i], l[i]);
-            uint8_t *dst = sm + 2 * x * L::Q + (c >> 3) * (PT_M * 128) + (tid & 127) * 128 + (((c & 7) ^ (tid & 7)) << 4);
-            *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4 *>(dst + L::Q) = make_uint4(l[0], l[1], l[2], l[3]);
+            for (int i = 0; i < 4; i++) kv4_pieces(fin ? kv4_scale2(y[i], k) : 0.f, fin ? kv4_scale2(y[i + 4], k) : 0.f, h[i], l[i]);
+            if (c < 4 * NG) {
+                uint8_t *dst = sm + 2 * x * L::Q + (c >> 3) * (PT_M * 128) + line * 128 + (((c & 7) ^ (line & 7)) << 4);
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(dst + L::Q) = make_uint4(l[0], l[1], l[2], l[3]);
+            }
         }
+        const bool fin = mb < 0x7f800000u;
+        // (not below the smallest normal number: -infinity times it has to stay -infinity)
+        desc = fin ? fmaxf(kv4_scale2(a.scale * 1.44269504f, -kv4_q_shift(mb)), 1.17549435e-38f) : __int_as_float(0x7fffffff);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     tc_before();
@@ -296,8 +324,6 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         }
     } else if (warp >= 8) {
         // ---- pages into shared memory, then as operand tiles ----
-        const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
-        const size_t page_bytes = kv4_page_bytes(a.geo);
         const __half2 down = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
         // Steps of a staged part: positions that no line sees become 0 (their memory may hold anything), steps that would
         // overflow and NaN steps of values are noted; all of it rare, and looked for two steps at a time.  Returns what
@@ -329,16 +355,11 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         bool ok = true;
         if (warp < 12) {
             const int w = tid - 256;
-            auto load = [&](int j) {                         // key codes and steps are one run of bytes
-                mbar_expect_tx(&sh.rawk[j & 1], 36 * HD);
-                bulk_load(sm + L::OFF_RAW + (j & 1) * L::RAW, base + (size_t)list[j].x * page_bytes, 36 * HD, &sh.rawk[j & 1]);
-            };
-            if (w == 0) for (int j = 0; j < 2 && j < n; j++) load(j);
             for (int j = 0; j < n; j++) {
                 uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW;
                 ok = warp_wait(&sh.rawk[j & 1], j >> 1 & 1, abort_flag);
                 if (!role_and<1, PT_KT>(ok)) break;
-                if (w == 0 && j > 0 && j + 1 < n) load(j + 1);
+                if (w == 0 && j > 0 && j + 1 < n) load_k(j + 1);
                 const float f = look(std::true_type{}, w, j, reinterpret_cast<uint32_t *>(raw + L::RK));
                 if (w == 0) sh.fk[j & 7] = f;
                 // the keys of page j - 1 are done with (a warp that gives up goes on to the next barrier, where all leave)
@@ -366,19 +387,11 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
             }
         } else {
             const int w = tid - 384;
-            auto load = [&](int j) {
-                uint8_t *dst = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
-                const uint8_t *src = base + (size_t)list[j].x * page_bytes + kv4_v_code_off(HD);
-                mbar_expect_tx(&sh.rawv[j & 1], 36 * HD);
-                for (int o = 0; o < 8; o++) bulk_load(dst + o * L::VS, src + o * (4 * HD), 4 * HD, &sh.rawv[j & 1]);     // apart by 16 bytes: eight halves, eight bank groups
-                bulk_load(dst + L::RV, src + 32 * HD, 4 * HD, &sh.rawv[j & 1]);
-            };
-            if (w == 0) for (int j = 0; j < 2 && j < n; j++) load(j);
             for (int j = 0; j < n; j++) {
                 uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
                 ok = warp_wait(&sh.rawv[j & 1], j >> 1 & 1, abort_flag);
                 if (!role_and<2, PT_VT>(ok)) break;
-                if (w == 0 && j > 0 && j + 1 < n) load(j + 1);
+                if (w == 0 && j > 0 && j + 1 < n) load_v(j + 1);
                 if (w < NG) sh.nan[j & 7][w] = 0ull;
                 if (w == 4) sh.anynan[j & 7] = 0;
                 const float f = look(std::false_type{}, w, j, reinterpret_cast<uint32_t *>(raw + L::RV));
@@ -506,17 +519,24 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                 }
             }
         }
-        if (ok && tid < ncol) {
-            float *out = nsplit == 1 ? a.ctx + rh * HD : part + (rh * nsplit + split) * (HD + 4) + 4;
-            if (nsplit > 1) { out[-4] = m; out[-3] = l; }
-            const float qnan = __int_as_float(0x7fffffff);
+        // out through the tile's query rows (their products are done), so that a warp writes whole lines: a thread puts its
+        // line there in pieces of four dims, turned by the line so that eight lanes meet eight bank groups
+        if (__all_sync(0xffffffffu, ok)) {
+            float4 *box = reinterpret_cast<float4 *>(sm + 2 * x * L::Q) + (warp & 3) * (32 * HD / 4);
+            if (tid < ncol && nsplit > 1) *reinterpret_cast<float2 *>(part + (rh * nsplit + split) * (HD + 4)) = make_float2(m, l);
+            const float over = nsplit > 1 ? 1.f : kv4_over(l);
 #pragma unroll
-            for (int c = 0; c < HD; c += 4) {
-                float4 v = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-                if (nsplit == 1)
-                    v = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(__fdiv_rn(v.x, l), __fdiv_rn(v.y, l), __fdiv_rn(v.z, l), __fdiv_rn(v.w, l));
-                if (nanbits >> (c >> 5) & 1) v = make_float4(qnan, qnan, qnan, qnan);
-                *reinterpret_cast<float4 *>(out + c) = v;
+            for (int c = 0; c < HD / 4; c++) {
+                const float no = nanbits >> (c >> 3) & 1 ? __int_as_float(0x7fffffff) : 0.f;
+                box[lane * (HD / 4) + (c ^ (lane & 7))] = make_float4(fmaf(o[4 * c], over, no), fmaf(o[4 * c + 1], over, no), fmaf(o[4 * c + 2], over, no), fmaf(o[4 * c + 3], over, no));
+            }
+            __syncwarp();
+            float *const to = nsplit == 1 ? a.ctx + rh * HD : part + (rh * nsplit + split) * (HD + 4) + 4;
+#pragma unroll 8
+            for (int i = 0; i < HD / 4; i++) {
+                const int at = i * 32 + lane, line = at / (HD / 4), c = at - line * (HD / 4);
+                float4 *dst = reinterpret_cast<float4 *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), line));
+                if ((warp & 3) * 32 + line + x * PT_M < ncol) dst[c] = box[line * (HD / 4) + (c ^ (line & 7))];
             }
         }
     }

@@ -22,7 +22,7 @@ __device__ __forceinline__ unsigned kv4_quant_lane(float x, int lane, unsigned s
     const int src = __ffs(__ballot_sync(0xffffffffu, ab == m)) - 1;
     const float big = __shfl_sync(0xffffffffu, x, src);
     const float other = warp_max_f32(((x > 0.f) != (big > 0.f)) ? a : 0.f);
-    const float step = fminf(fmaxf(__fdiv_rn(fabsf(big), 8.f), __fdiv_rn(other, 7.f)), 65504.f);
+    const float step = fminf(fmaxf(__fmul_rn(fabsf(big), 0.125f), __fdiv_rn(other, 7.f)), 65504.f);
     const __half h = __float2half_rn(big > 0.f ? -step : step);
     const float df = __half2float(h);
     *d = __half_as_ushort(h);
@@ -81,7 +81,7 @@ __device__ __forceinline__ float kv4_quad_step(const float (&x)[8], unsigned sho
         if (pb == nb) neg = first & 1;
     }
     const float big = __int_as_float(neg ? nb : pb), other = __int_as_float(neg ? pb : nb);
-    const float step = fminf(fmaxf(__fdiv_rn(big, 8.f), __fdiv_rn(other, 7.f)), 65504.f);
+    const float step = fminf(fmaxf(__fmul_rn(big, 0.125f), __fdiv_rn(other, 7.f)), 65504.f);
     const __half h = __float2half_rn(neg || big == 0.f ? step : -step);
     *d = bad ? (unsigned short)0x7fff : __half_as_ushort(h);
     return bad ? 0.f : __half2float(h);                        // codes of a bad group are 0, as with a step of 0

@@ -356,6 +356,98 @@ def test_attend_strided_queries_and_another_stream(gpu, t):
     gpu.sync(0)
     assert ctx.cpu().numpy().tobytes() == plain.tobytes()
 
+# A table with room for much longer sequences than there are: the cut of the work follows the limits, so that the same small
+# batch also runs through the kernels and the many short spans of large ones.
+ROOM = [0, 150]
+
+
+@pytest.mark.parametrize("H,KV,hd,rows,lens,window", [c for c in CASES if max(c[3]) > 1])
+def test_attend_with_room(gpu, t, H, KV, hd, rows, lens, window):
+    p = Pool(gpu, t, KV, hd, lens, seed=H * hd + len(lens), scale=2.0, extra_ld=500)
+    q = p.rng.standard_normal((sum(rows), H, hd)).astype(np.float32)
+    got = p.attend(q, H, rows, window=window, max_len=p.ld * 64)
+    assert got.tobytes() == p.attend(q, H, rows, window=window, max_len=p.ld * 64).tobytes()
+    at = 0
+    for s, (r, L) in enumerate(zip(rows, lens)):
+        want, tol = attend64(quant(p.k[s])[0], quant(p.v[s])[0], q[at:at + r], np.arange(L - r, L), H // KV, window)
+        check(got[at:at + r], want, tol)
+        at += r
+    p.status()
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("rows", [1, 3, 20, 70])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
+def test_attend_values_and_keys_that_are_not_finite(gpu, t, hd, rows, room):
+    """A NaN value reaches the rows that see its position, in its group's 32 dims, however small its weight; an infinite key
+    makes the rows that see it NaN altogether; no other row or head changes."""
+    H, KV, L, G = 8, 2, 300, 4
+    p = Pool(gpu, t, KV, hd, [L], seed=hd + rows, scale=2.0, extra_ld=1 + room)
+    q = p.rng.standard_normal((rows, H, hd)).astype(np.float32)
+    pos, scale = np.arange(L - rows, L), 4.0                 # (weights from 1 down to what underflows)
+    clean = p.v[0].copy()
+    g = hd // 64                                             # a group of 32 dims
+    # one that all see, one that half of the rows see, in different heads
+    at = [(70, 0), (L - 1 - rows // 2, 1)]
+    for w, h in at:
+        p.v[0][w, h, 32 * g + 5] = np.nan
+    p.store()
+    got = p.attend(q, H, [rows], scale=scale, max_len=p.ld * 64).reshape(rows, H, hd)
+    ql = clean.copy()
+    for w, h in at:
+        ql[w, h, 32 * g:32 * g + 32] = 0
+    want, tol = attend64(quant(p.k[0])[0], quant(ql)[0], q, pos, G, scale=scale)
+    for w, h in at:
+        want[pos >= w, h * G:(h + 1) * G, 32 * g:32 * g + 32] = np.nan
+    check(got, want, tol)
+    # keys
+    p.v[0] = clean
+    for w, h in at:
+        p.k[0][w, h, 3] = np.inf
+    p.store()
+    got = p.attend(q, H, [rows], scale=scale, max_len=p.ld * 64).reshape(rows, H, hd)
+    kl = np.where(np.isfinite(p.k[0]), p.k[0], 0)
+    want, tol = attend64(quant(kl)[0], quant(clean)[0], q, pos, G, scale=scale)
+    for w, h in at:
+        want[pos >= w, h * G:(h + 1) * G] = np.nan
+    check(got, want, tol)
+    p.status()
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("rows", [1, 3, 70])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kmag,vmag", [(3e4, 1.0), (1.0, 9e4), (1e-6, 1e-6), (3e4, 9e4)])
+def test_attend_step_range(gpu, t, hd, rows, kmag, vmag, room):
+    """Steps from the smallest f16 numbers to nearly the largest."""
+    H, KV, L = 8, 2, 200
+    p = Pool(gpu, t, KV, hd, [L], seed=hd + rows, scale=kmag, extra_ld=1 + room)
+    p.v[0] *= np.float32(vmag)
+    p.store()
+    q = p.rng.standard_normal((rows, H, hd)).astype(np.float32)
+    scale = float(np.float32(1 / (kmag * math.sqrt(hd))))
+    got = p.attend(q, H, [rows], scale=scale, max_len=p.ld * 64)
+    want, tol = attend64(quant(p.k[0])[0], quant(p.v[0])[0], q, np.arange(L - rows, L), H // KV, scale=scale)
+    check(got, want, tol)
+    p.status()
+
+
+@pytest.mark.parametrize("nseq,rows,H,KV,hd,L", [(5, 40, 128, 16, 64, 33285), (90, 1, 16, 8, 32, 17001), (3, 20, 64, 32, 160, 9000)])
+def test_attend_one_long_sequence_among_short_ones(gpu, t, nseq, rows, H, KV, hd, L):
+    """More units than the GPU holds CTAs, and more pages in one sequence than a CTA's list of pages has room for."""
+    lens = [rows + 3 * s for s in range(nseq)]
+    lens[1] = L
+    p = Pool(gpu, t, KV, hd, lens, seed=7)
+    q = p.rng.standard_normal((nseq * rows, H, hd)).astype(np.float32)
+    got = p.attend(q, H, [rows] * nseq).reshape(-1, H, hd)
+    for s in (0, 1, 2, nseq - 1):
+        k, v = quant(p.k[s])[0], quant(p.v[s])[0]
+        for i, h in ((0, 0), (rows - 1, H - 1), (rows // 2, H // 2)):
+            g, row = h // (H // KV), s * rows + i
+            want, tol = attend64(k[:, g:g + 1], v[:, g:g + 1], q[row:row + 1, h:h + 1], np.array([lens[s] - rows + i]), 1)
+            check(got[row:row + 1, h:h + 1], want, tol)
+    p.status()
+
 
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attend_does_not_depend_on_the_neighbours(gpu, t, rows):
