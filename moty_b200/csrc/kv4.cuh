@@ -26,9 +26,14 @@ int launch_kv4_append_rope(const Kv4Geom &geo, uint8_t *mem, int layer, int H, f
                            const Kv4Rope &rope, const Kv4Batch &b, int *err, cudaStream_t st);
 int launch_kv4_fetch(const Kv4Geom &geo, const uint8_t *mem, int layer, float *k, float *v, const Kv4Batch &b, int *err, cudaStream_t st);
 // ---- kv4_attend.cu ----
-size_t kv4_attend_scratch_bytes(const Kv4Attend &a, int sms);
-size_t kv4_attend_counters(const Kv4Attend &a, int sms);
-int launch_kv4_attend(const Kv4Attend &a, float *part, int *count, int sms, cudaStream_t st);
+// how an attention call is cut.  decode: the kernel for few rows; tc: the tensor-memory prompt kernel; a CTA takes `cols`
+// (row, query head) pairs of one KV head of one sequence, ntile such tiles a sequence at most, and one of nsplit spans of
+// `span` positions
+struct Kv4Plan { bool decode, tc; int cols, ntile, nsplit, span; };
+Kv4Plan kv4_plan(const Kv4Attend &a, int sms);
+size_t kv4_attend_scratch_bytes(const Kv4Attend &a, const Kv4Plan &p);
+size_t kv4_attend_counters(const Kv4Attend &a, const Kv4Plan &p);
+int launch_kv4_attend(const Kv4Attend &a, const Kv4Plan &p, float *part, int *count, cudaStream_t st);
 // ---- kv4_pages.cu ----
 int launch_kv4_fork(const Kv4Geom &geo, uint8_t *mem, int n, const int *src, const int *dst, const int *fresh, int nseq, int *len,
                     int *table, int ld, int *err, cudaStream_t st);

@@ -193,6 +193,8 @@ extern "C" int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_d
     if (batch->max_rows < 0 || batch->max_rows > batch->rows || batch->max_len < 0 || batch->max_len > (long long)batch->table_ld * KV4_PAGE)
         return moty_set_error(MOTY_CUDA_EARG, "kv4_attend_dev: max_rows=%d of %d rows, max_len=%d with %d pages a sequence", batch->max_rows, batch->rows,
                               batch->max_len, batch->table_ld);
+    if ((long long)batch->rows * n_heads > 0x7fffff00LL)       // (512 GB of context rows)
+        return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend_dev: %d rows of %d heads", batch->rows, n_heads);
     CKR(kv4_ld("kv4_attend_dev", q_ld, (long long)n_heads * kv->geo.hd, &a.q_ld));
     if (!ctx_dev || !q_dev || !kv4_aligned(ctx_dev, 16) || !kv4_aligned(q_dev, 16))
         return moty_set_error(MOTY_CUDA_EARG, "kv4_attend_dev: ctx or q null or not 16-byte aligned");
@@ -202,11 +204,11 @@ extern "C" int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_d
     MOTY_USE_DEVICE(kv->device);
     a.H = n_heads; a.G = n_heads / kv->geo.KV; a.q = q_dev; a.ctx = ctx_dev; a.max_rows = batch->max_rows; a.max_len = batch->max_len;
     a.window = window; a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)kv->geo.hd); a.err = c->err_dev + 4;
-    const size_t sb = kv4_attend_scratch_bytes(a, c->sms);
-    const size_t nc = kv4_attend_counters(a, c->sms) * 4;
+    const Kv4Plan p = kv4_plan(a, c->sms);
+    const size_t sb = kv4_attend_scratch_bytes(a, p), nc = kv4_attend_counters(a, p) * 4;
     if (sb) CKR(moty_grow(c, &c->attn, sb));
     if (nc) CKR(moty_grow_zero(c, &c->kv4n, nc));
-    return launch_kv4_attend(a, sb ? (float *)c->attn.p : nullptr, nc ? (int *)c->kv4n.p : nullptr, c->sms, kv4_stream(c, stream));
+    return launch_kv4_attend(a, p, sb ? (float *)c->attn.p : nullptr, nc ? (int *)c->kv4n.p : nullptr, kv4_stream(c, stream));
 }
 
 extern "C" int moty_cuda_kv4_fork_dev(MotyCudaKv4 *kv, int n, const int *src_dev, const int *dst_dev, const int *fresh_dev, int nseq,

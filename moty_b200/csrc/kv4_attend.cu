@@ -466,35 +466,46 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
     if (tid == 0) count[u] = 0;                              // as the next launch finds it
 }
 
-// What the join of a (row, head) needs: how many of its spans hold something (the row's column tile decides), 0: the row is
-// refused and reads as zeros, -1: no sequence has the row.
-__device__ __forceinline__ int kv4_live_spans(const Kv4Attend &a, const Kv4Plan &pl, int row, int h) {
+// What the join of a row's heads needs of its sequence: r0 < 0: no sequence has the row; n == 0: the row is refused and
+// reads as zeros.
+struct Kv4Join { int r0, n, len; };
+__device__ __forceinline__ Kv4Join kv4_join_row(const Kv4Attend &a, int row) {
     int seq, pos;
     const int st = kv4_row(a.b, row, &seq, &pos);
-    if (st == KV4_ROW_NONE) return -1;
-    if (st == KV4_ROW_BAD) return 0;
-    const int n = a.b.row0[seq + 1] - a.b.row0[seq], len = a.b.len[seq];
-    if (n > a.max_rows || len > a.max_len) return 0;
-    const long long c = (long long)(row - a.b.row0[seq]) * a.G + h % a.G, c0 = c / pl.cols * pl.cols, last = (long long)n * a.G - 1;
-    const long long cz = c0 + pl.cols - 1 < last ? c0 + pl.cols - 1 : last;
-    const Kv4Range cr = kv4_range(a, len - n + (int)(c0 / a.G), len - n + (int)(cz / a.G));
+    Kv4Join r{-1, 0, 0};
+    if (st == KV4_ROW_NONE) return r;
+    r.r0 = 0;
+    if (st == KV4_ROW_BAD) return r;
+    const int r0 = a.b.row0[seq], n = a.b.row0[seq + 1] - r0, len = a.b.len[seq];
+    if (n <= a.max_rows && len <= a.max_len) r = {r0, n, len};
+    return r;
+}
+// how many spans of a (row, head) hold something (the row's column tile decides)
+__device__ __forceinline__ int kv4_live_spans(const Kv4Attend &a, const Kv4Plan &pl, const Kv4Join &j, int row, int h) {
+    if (j.n == 0) return 0;
+    const int c0 = ((row - j.r0) * a.G + h % a.G) & -pl.cols, last = j.n * a.G - 1;      // (cols: a power of two)
+    const int cz = c0 + pl.cols - 1 < last ? c0 + pl.cols - 1 : last;
+    const Kv4Range cr = kv4_range(a, j.len - j.n + c0 / a.G, j.len - j.n + cz / a.G);
     const int live = (cr.hi_any - (cr.lo_any & ~(KV4_PAGE - 1)) + pl.span - 1) / pl.span;
     return live < pl.nsplit ? live : pl.nsplit;
 }
-// joins up to 32 spans of one (row, head), a warp each, a span's {m, l} a lane
+
+// Joins up to 32 spans of a (row, head): a warp each, a span's {m, l} a lane.  A chain of loads (the row's sequence, {m, l},
+// sums), so what counts is how many warps wait at once: 1568 rows x 20 heads x 96 dims in two spans 22 us, 130 us when a CTA
+// took a (row, head); with more spans than lanes a CTA does (kv4_merge_kernel).
 constexpr int MG_T = 256;
-__global__ void __launch_bounds__(MG_T) kv4_merge_few_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
+__global__ void __launch_bounds__(MG_T, 4) kv4_merge_few_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
     const int hd = a.geo.hd, lane = threadIdx.x & 31, q4 = hd >> 2;
-    const long long item = (long long)blockIdx.x * (MG_T / 32) + (threadIdx.x >> 5);
+    const unsigned item = blockIdx.x * (MG_T / 32) + (threadIdx.x >> 5);
     pdl_trigger();
     pdl_wait();
-    const int row = (int)(item / a.H), h = (int)(item - (long long)row * a.H);
+    const int row = (int)(item / (unsigned)a.H), h = (int)item - row * a.H;
     if (row >= a.b.rows) return;
-    const int live = kv4_live_spans(a, pl, row, h);
-    if (live < 0) return;
+    const Kv4Join j = kv4_join_row(a, row);
+    if (j.r0 < 0) return;
+    const int live = kv4_live_spans(a, pl, j, row, h);
     const float *p = part + (size_t)item * pl.nsplit * (hd + 4);
-    const bool mine = lane < live;
-    const float2 ml = mine ? *reinterpret_cast<const float2 *>(p + (size_t)lane * (hd + 4)) : make_float2(-INFINITY, 0.f);
+    const float2 ml = lane < live ? *reinterpret_cast<const float2 *>(p + (size_t)lane * (hd + 4)) : make_float2(-INFINITY, 0.f);
     const float M = warp_max_f32(ml.x), f = kv4_factor(ml.y, ml.x, M);
     float L = ml.y * f;
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
@@ -505,7 +516,8 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_few_kernel(Kv4Attend a, Kv4Pla
         for (int i0 = 0; i0 < live; i0 += 8) {
             float4 v[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++) v[u] = reinterpret_cast<const float4 *>(p + (size_t)(i0 + u < live ? i0 + u : i0) * (hd + 4) + 4)[d];
+            for (int u = 0; u < 8; u++)
+                if (i0 + u < live) v[u] = reinterpret_cast<const float4 *>(p + (size_t)(i0 + u) * (hd + 4) + 4)[d];
 #pragma unroll
             for (int u = 0; u < 8; u++) {
                 const float fi = __shfl_sync(0xffffffffu, f, i0 + u);
@@ -523,8 +535,9 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
     const int row = blockIdx.x, h = blockIdx.y, hd = a.geo.hd, tid = threadIdx.x;
     pdl_trigger();
     pdl_wait();
-    const int live = kv4_live_spans(a, pl, row, h);
-    if (live < 0) return;
+    const Kv4Join j = kv4_join_row(a, row);
+    if (j.r0 < 0) return;
+    const int live = kv4_live_spans(a, pl, j, row, h);
     float *out = a.ctx + ((size_t)row * a.H + h) * hd;
     const float *p = part + ((size_t)row * a.H + h) * pl.nsplit * (hd + 4);
     float M = -INFINITY;
@@ -560,19 +573,27 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
 }  // namespace
 
 // How a call is cut.  Host numbers only (the limits the caller gave), so a captured call stays valid for any batch within
-// them.  Decode or prompt kernel: the decode kernel re-reads the pages for every 8 columns, the prompt kernel fills 16
-// lines a warp: 32 columns (Q_DEC) is where they meet at 4096 positions of 128-wide heads.
-// Spans: with `units` (sequence, KV head, tile) triples of P pages on `slots` resident CTAs, a CTA costs its pages plus
-// about FIX pages' time of set-up and join.  When all CTAs are resident at once the longest one counts; otherwise the total
-// work over the slots plus a last CTA (lengths of a ragged batch are taken as 0.6 of the limit).  The cut with the least of
-// that: 64 sequences of up to 8192 positions 136 us uncut, 108 us with 5 spans of 26 pages, 113 us with 3; one sequence of
-// 131072 positions 62 us on 148 CTAs, 38 us on 444 (one full set), 55 us on 1184.
-static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
+// them.  Which kernel, by (row, query head) pairs of a KV head ("columns"):
+//   decode, which re-reads the pages for every 8 columns, up to 64 of them, up to 48 where the tensor-memory kernel has the
+//     heads' width and their dims are many (8 sequences of 4096, 8 KV heads, hd 128: 72 us against 91 / 88 us of the prompt
+//     kernels at 48 columns, 108 against 95 / 90 us at 64; hd 64, 64 columns: 59 against 75 / 72 us; hd 256: 186 against
+//     191 us);
+//   tensor memory above 64 columns at hd 64, 96, 128 when there are more than six pages of 64 columns an SM: below that its
+//     set-up (15 us) is more than the matrix work it saves (one sequence of 1024, 8 KV heads, hd 128, 256 columns: 24 us
+//     against 21 us of the other; of 4096: 32 us against 52 us; 8 of 4096: 125 us against 330 us).
+// Spans of decode: with `units` (sequence, KV head, tile) triples of P pages on `slots` resident CTAs, a CTA costs its pages
+// plus about FIX pages' time of set-up and join.  When all CTAs are resident at once the longest one counts; otherwise the
+// total work over the slots plus a last CTA (lengths of a ragged batch are taken as 0.6 of the limit).  The cut with the
+// least of that (64 sequences of up to 8192 positions, 32 heads on 8: 104 us).  A prompt is cut only to fill the GPU: the
+// joins move rows x heads x hd x spans f32 values (4096 rows at 4096 positions, 16 heads: 176 us whole, 277 us in two spans;
+// nine ragged sequences of up to 333 rows and 2900 positions 108 us whole, 129 us in two).
+Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     Kv4Plan p{};
     const long long cols = (long long)a.max_rows * a.G;
     const int NG = a.geo.hd / 32;
     p.decode = cols <= (NG == 3 || NG == 4 ? 48 : 64);
-    const long long pages64 = (long long)a.b.nseq * a.geo.KV * ((cols + 63) / 64) * ((a.max_len + KV4_PAGE - 1) / KV4_PAGE);
+    const long long seen = a.window > 0 && a.window + 2LL * KV4_PAGE < a.max_len ? a.window + 2LL * KV4_PAGE : a.max_len;
+    const long long pages64 = (long long)a.b.nseq * a.geo.KV * ((cols + 63) / 64) * ((seen + KV4_PAGE - 1) / KV4_PAGE);
     p.tc = cols > KV4_LINES && NG >= 2 && NG <= 4 && pages64 > 6LL * sms;
     p.cols = p.tc ? KV4_TC_LINES : !p.decode ? KV4_LINES : cols > 4 ? 8 : 4;
     p.ntile = (int)((cols + p.cols - 1) / p.cols);
@@ -582,19 +603,18 @@ static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     const long long rows_a_tile = p.cols / a.G + 2 < a.max_rows ? p.cols / a.G + 2 : a.max_rows;
     if (a.window > 0 && (long long)a.window + rows_a_tile + KV4_PAGE < range) range = (long long)a.window + rows_a_tile + KV4_PAGE;
     const int occ = p.tc ? 1 : !p.decode ? 2 : p.cols == 4 ? kv4_decode_ctas(NG, true) : kv4_decode_ctas(NG, false);
-    const double units = (double)a.b.nseq * a.geo.KV * p.ntile, slots = (double)sms * occ, FIX = p.decode ? 6 : 2;
+    const double units = (double)a.b.nseq * a.geo.KV * p.ntile, slots = (double)sms * occ, FIX = 6;
     const long long P = (range + KV4_PAGE - 1) / KV4_PAGE, least = p.decode ? (P + DEC_NP - 1) / DEC_NP : p.tc ? (P + KV4_TC_PAGES - 1) / KV4_TC_PAGES : 1;
     const double w = a.b.nseq > 1 ? 0.6 : 1.0;
     long long best = least > 0 ? least : 1;
     double cost = 1e300;
-    for (long long n = best; n <= P && n <= 1024 + best; n++) {
+    for (long long n = best; n <= P && n <= 1024 + best;) {
         const long long pages = (P + n - 1) / n;
-        if (n > best && (P + n - 2) / (n - 1) == pages) continue;            // the same spans with fewer cuts
         const double c = (units * n <= slots ? pages + FIX : units * (w * P + FIX * n) / slots + pages + FIX) + (n > 1 ? 2 : 0);
         if (c < cost) { cost = c; best = n; }
+        if (pages == 1) break;
+        n = (P + pages - 2) / (pages - 1);                     // the next that makes the spans shorter
     }
-    // a prompt is cut only to fill the GPU (4096 rows at 4096 positions: 587 us whole, 820 us in two spans, whose joins move
-    // rows x heads x hd x spans f32 values)
     if (!p.decode) best = units < slots ? (long long)(slots / units) : 1;
     if (best < least) best = least;
     if (best > P) best = P > 0 ? P : 1;
@@ -605,9 +625,12 @@ static Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     return p;
 }
 
-size_t kv4_attend_scratch_bytes(const Kv4Attend &a, int sms) {
-    const Kv4Plan p = kv4_plan(a, sms);
+size_t kv4_attend_scratch_bytes(const Kv4Attend &a, const Kv4Plan &p) {
     return p.nsplit > 1 ? (size_t)a.b.rows * a.H * p.nsplit * (a.geo.hd + 4) * 4 : 0;
+}
+// CTAs that count their spans' ends, when few spans are joined in the launch itself
+size_t kv4_attend_counters(const Kv4Attend &a, const Kv4Plan &p) {
+    return p.decode && p.nsplit > 1 && p.nsplit <= DEC_JOIN ? (size_t)a.b.nseq * a.geo.KV * p.ntile : 0;
 }
 
 template <int NG, bool PAIR>
@@ -631,15 +654,8 @@ static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, int 
     return p.cols == 4 ? kv4_decode_go<NG, true>(a, p, part, count, st) : kv4_decode_go<NG, false>(a, p, part, count, st);
 }
 
-// CTAs that count their spans' ends, when few spans are joined in the launch itself
-size_t kv4_attend_counters(const Kv4Attend &a, int sms) {
-    const Kv4Plan p = kv4_plan(a, sms);
-    return p.decode && p.nsplit > 1 && p.nsplit <= DEC_JOIN ? (size_t)a.b.nseq * a.geo.KV * p.ntile : 0;
-}
-
 // part: scratch of kv4_attend_scratch_bytes; count: kv4_attend_counters ints, all zero (and left so)
-int launch_kv4_attend(const Kv4Attend &a, float *part, int *count, int sms, cudaStream_t st) {
-    const Kv4Plan p = kv4_plan(a, sms);
+int launch_kv4_attend(const Kv4Attend &a, const Kv4Plan &p, float *part, int *count, cudaStream_t st) {
     if (p.nsplit > 1 && !part) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: scratch for %d spans missing", p.nsplit);
     int rc = 0;
     if (p.tc) rc = launch_kv4_prompt_tc(a, p, part, st);

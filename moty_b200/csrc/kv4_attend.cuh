@@ -2,12 +2,8 @@
 #pragma once
 #include "kv4.cuh"
 
-// A CTA takes `cols` (row, query head) pairs of one KV head of one sequence, ntile such
-// tiles a sequence at most, and one of nsplit spans of `span` positions.
 constexpr int KV4_LINES = 64;             // (row, query head) pairs a CTA of the prompt kernel takes
 constexpr int KV4_TC_LINES = 256, KV4_TC_PAGES = 512;       // the same of the tensor-memory prompt kernel, and the most pages of its spans
-// decode: the kernel for few rows; tc: the tensor-memory prompt kernel
-struct Kv4Plan { bool decode, tc; int cols, ntile, nsplit, span; };
 int launch_kv4_prompt(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st);
 int launch_kv4_prompt_tc(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st);
 

@@ -38,26 +38,25 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
         if (nsplit == 1 && tile == 0) kv4_zero_rows(a, sq, head);
         return;
     }
-    const long long lines = (long long)sq.n * a.G;
-    const long long c0 = (long long)tile * NL;
+    const int lines = sq.n * a.G, c0 = tile * NL;            // (rows * heads of a call stay below 2^31)
     if (c0 >= lines) return;
-    const int ncol = lines - c0 < NL ? (int)(lines - c0) : NL;
-    const int pos0 = sq.len - sq.n, row_a = (int)(c0 / a.G), row_z = (int)((c0 + ncol - 1) / a.G);
+    const int ncol = lines - c0 < NL ? lines - c0 : NL;
+    const int pos0 = sq.len - sq.n, row_a = c0 / a.G, row_z = (c0 + ncol - 1) / a.G;
     const Kv4Range cr = kv4_range(a, pos0 + row_a, pos0 + row_z);
     const int t_lo = (cr.lo_any & ~(KV4_PAGE - 1)) + split * span, t_hi = cr.hi_any - t_lo < span ? cr.hi_any : t_lo + span;
     if (t_lo >= cr.hi_any && nsplit > 1) return;
     // the warp's own lines
     const int w0 = warp * 16, wn = ncol - w0 < 16 ? ncol - w0 : 16;          // valid lines of the warp (may be <= 0)
     Kv4Range wr = kv4_range(a, 0, 0);
-    if (wn > 0) wr = kv4_range(a, pos0 + (int)((c0 + w0) / a.G), pos0 + (int)((c0 + w0 + wn - 1) / a.G));
+    if (wn > 0) wr = kv4_range(a, pos0 + (c0 + w0) / a.G, pos0 + (c0 + w0 + wn - 1) / a.G);
     float desc[2];
     int clo[2], chi[2];
 #pragma unroll
     for (int hlf = 0; hlf < 2; hlf++) {
         const int line = r + 8 * hlf;
-        const long long cc = c0 + w0 + line;
+        const int cc = c0 + w0 + line;
         const bool have = line < wn;
-        const int row = have ? (int)(cc / a.G) : 0, g0 = have ? (int)(cc % a.G) : 0;
+        const int row = have ? cc / a.G : 0, g0 = have ? cc % a.G : 0;
         const float *src = a.q + (size_t)(sq.r0 + row) * a.q_ld + (size_t)(head * a.G + g0) * HD;
         unsigned mb = 0;
         if (have) {
@@ -287,8 +286,8 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
         l[hlf] += __shfl_xor_sync(0xffffffffu, l[hlf], 2);
         const int line = r + 8 * hlf;
         if (line >= wn) continue;
-        const long long cc = c0 + w0 + line;
-        const size_t rh = (size_t)(sq.r0 + (int)(cc / a.G)) * a.H + head * a.G + (int)(cc % a.G);
+        const int cc = c0 + w0 + line;
+        const size_t rh = (size_t)(sq.r0 + cc / a.G) * a.H + head * a.G + cc % a.G;
         float *out;
         float f = vs;
         if (nsplit == 1) {

@@ -157,11 +157,11 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         if (nsplit == 1 && tile == 0) kv4_zero_rows(a, sq, head);
         return;
     }
-    const long long lines = (long long)sq.n * a.G, c0 = (long long)tile * KV4_TC_LINES;
+    const int lines = sq.n * a.G, c0 = tile * KV4_TC_LINES;  // (rows * heads of a call stay below 2^31)
     if (c0 >= lines) return;
-    const int ncol = lines - c0 < KV4_TC_LINES ? (int)(lines - c0) : KV4_TC_LINES, nx = ncol > PT_M ? 2 : 1;      // lines, tiles
+    const int ncol = lines - c0 < KV4_TC_LINES ? lines - c0 : KV4_TC_LINES, nx = ncol > PT_M ? 2 : 1;      // lines, tiles
     const int pos0 = sq.len - sq.n;
-    const Kv4Range cr = kv4_range(a, pos0 + (int)(c0 / a.G), pos0 + (int)((c0 + ncol - 1) / a.G));
+    const Kv4Range cr = kv4_range(a, pos0 + c0 / a.G, pos0 + (c0 + ncol - 1) / a.G);
     const int t_lo = (cr.lo_any & ~(KV4_PAGE - 1)) + split * span, t_hi = cr.hi_any - t_lo < span ? cr.hi_any : t_lo + span;
     if (t_lo >= cr.hi_any && nsplit > 1) return;
 
@@ -223,8 +223,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         const bool have = tid < ncol;
         const float *src = a.q;
         if (have) {
-            const long long cc = c0 + tid;
-            const int row = (int)(cc / a.G), g0 = (int)(cc - (long long)row * a.G), p = pos0 + row;
+            const int cc = c0 + tid, row = cc / a.G, g0 = cc - row * a.G, p = pos0 + row;
             src = a.q + (size_t)(sq.r0 + row) * a.q_ld + (size_t)(head * a.G + g0) * HD;
             rh = (size_t)(sq.r0 + row) * a.H + head * a.G + g0;
             chi = p;

@@ -526,6 +526,15 @@ def test_refused_arguments(gpu, t):
     p.status()
 
 
+def test_attend_of_more_pairs_than_it_counts_is_refused(gpu, t):
+    p = Pool(gpu, t, 2, 64, [10])
+    a, ok = t.zeros(4096, device="cuda").data_ptr(), p.batch([1])
+    for rows, H in ((1 << 29, 4), (1 << 20, 2048), (0x7fffffff, 2)):
+        b = gpu.Kv4Batch(1, rows, ok.c.row0_dev, ok.c.len_dev, ok.c.table_dev, p.ld, max_rows=1, max_len=10)
+        with pytest.raises(gpu.MotyCudaError):
+            p.kv.attend_dev(0, a, a, H, b)
+
+
 @pytest.mark.parametrize("what", ["len_past_table", "len_past_max", "rows_more_than_len", "row0_negative", "row0_past_rows", "row0_back",
                                   "rows_past_max", "page_past_pool", "page_negative"])
 @pytest.mark.parametrize("big", [False, True])
