@@ -477,9 +477,9 @@ int moty_cuda_kv4_compact_plan(MotyCudaKv4 *kv, int cap, int *src, int *dst, int
 /* A ragged batch.  All arrays are device int32 and are read when the kernels run, so a captured graph follows them:
  * rows row0[s] .. row0[s + 1] - 1 of the row buffers belong to sequence s and stand for the LAST positions of its len[s]
  * (which counts them); position t lies in page table[s][t / 64].  A table entry of -1 is an absent page (freed in front
- * of a sliding window, say): its positions are not there.  rows: height of the row buffers; rows from row0[nseq] on are
- * neither read nor written.  max_rows / max_len: no sequence has more rows / positions (attend_dev sizes its launch by
- * them; append and fetch do not use them).  Arrays that do not describe a batch (offsets outside the buffers, more rows
+ * of a sliding window, say): its positions are not there.  rows: height of the row buffers; rows from row0[nseq] on have
+ * no effect and are not written.  max_rows / max_len: no sequence has more rows / positions (attend_dev sizes its launch by
+ * them, max_len 2^30 at most and rows * n_heads below 2^31; append and fetch do not use them).  Arrays that do not describe a batch (offsets outside the buffers, more rows
  * than positions, a length past the table or max_len, page ids outside the pool) never move an access out of bounds: the
  * rows concerned are skipped (attend_dev: set to 0; positions of a bad page are left out) and moty_cuda_kernel_status reports it. */
 typedef struct {

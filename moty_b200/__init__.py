@@ -395,7 +395,7 @@ class Kv4Batch:
     are the last of sequence s's len[s] positions, position t lies in page table[s][t // 64] (-1: absent)."""
 
     def __init__(self, nseq, rows, row0_ptr, len_ptr, table_ptr, table_ld, max_rows=None, max_len=None):
-        self.c = _Kv4BatchC(nseq, rows, rows if max_rows is None else max_rows, table_ld * Kv4.PAGE if max_len is None else max_len,
+        self.c = _Kv4BatchC(nseq, rows, rows if max_rows is None else max_rows, min(table_ld * Kv4.PAGE, 1 << 30) if max_len is None else max_len,
                             table_ld, row0_ptr, len_ptr, table_ptr)
         self.ptr = C.addressof(self.c)
 

@@ -193,6 +193,7 @@ extern "C" int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_d
     if (batch->max_rows < 0 || batch->max_rows > batch->rows || batch->max_len < 0 || batch->max_len > (long long)batch->table_ld * KV4_PAGE)
         return moty_set_error(MOTY_CUDA_EARG, "kv4_attend_dev: max_rows=%d of %d rows, max_len=%d with %d pages a sequence", batch->max_rows, batch->rows,
                               batch->max_len, batch->table_ld);
+    if (batch->max_len > 1 << 30) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend_dev: max_len=%d (2^30 at most)", batch->max_len);
     if ((long long)batch->rows * n_heads > 0x7fffff00LL)       // (512 GB of context rows)
         return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend_dev: %d rows of %d heads", batch->rows, n_heads);
     CKR(kv4_ld("kv4_attend_dev", q_ld, (long long)n_heads * kv->geo.hd, &a.q_ld));

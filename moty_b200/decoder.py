@@ -447,6 +447,8 @@ class PagedDecoder(DenseDecoder):
     def fork(self, sid, n=1) -> list:
         """n copies of a sequence: they share its full pages, the last partial page is copied on the device."""
         self._check(sid)
+        if n < 1:
+            raise MotyCudaError(f"{n} forks")
         self._drop_graph()
         L = int(self.lens[sid]); full = L // Kv4.PAGE
         free = np.flatnonzero(~self.used)[:n]
@@ -486,6 +488,11 @@ class PagedDecoder(DenseDecoder):
         if not (0 <= sid < self.max_seqs and self.used[sid]):
             raise MotyCudaError(f"sequence {sid} is not in use")
 
+    def _check_tokens(self, toks):
+        for i in toks:
+            if i.min() < 0 or i.max() >= self.head.O:
+                raise MotyCudaError(f"a token id outside the vocabulary of {self.head.O}")
+
     def _reserve(self, sids, more):
         """Pages for `more[i]` further positions of each sequence: all of them or none."""
         grow = []
@@ -510,6 +517,7 @@ class PagedDecoder(DenseDecoder):
             self._check(s)
         if len(set(sids)) != len(sids) or any(not i.size for i in toks):
             raise MotyCudaError("each sequence of a batch once, with at least one token")
+        self._check_tokens(toks)
         counts = [i.size for i in toks]
         S, n = sum(counts), len(sids)
         self._reserve(sids, counts)
@@ -543,6 +551,10 @@ class PagedDecoder(DenseDecoder):
         if len(set(sids)) != len(sids) or not sids or n < 1:
             raise MotyCudaError("each sequence once, at least one, and at least one token")
         k = len(sids)
+        tokens = np.ascontiguousarray(tokens, np.int32).ravel()
+        if tokens.size != k:
+            raise MotyCudaError(f"{tokens.size} tokens for {k} sequences")
+        self._check_tokens([tokens])
         self._reserve(sids, [n] * k)
         if k > self.cap:
             self._alloc(k)

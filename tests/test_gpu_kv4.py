@@ -535,6 +535,16 @@ def test_attend_of_more_pairs_than_it_counts_is_refused(gpu, t):
             p.kv.attend_dev(0, a, a, H, b)
 
 
+def test_attend_of_a_length_past_2_30_is_refused(gpu, t):
+    p = Pool(gpu, t, 2, 64, [10])
+    a, ok = t.zeros(4096, device="cuda").data_ptr(), p.batch([1])
+    mk = lambda **kw: gpu.Kv4Batch(1, 1, ok.c.row0_dev, ok.c.len_dev, ok.c.table_dev, 1 << 25, max_rows=1, **kw)
+    for n in ((1 << 30) + 1, 0x7fffffff):
+        with pytest.raises(gpu.MotyCudaError):
+            p.kv.attend_dev(0, a, a, 4, mk(max_len=n))
+    assert mk().c.max_len == 1 << 30                        # what the binding gives a table of that width
+
+
 @pytest.mark.parametrize("what", ["len_past_table", "len_past_max", "rows_more_than_len", "row0_negative", "row0_past_rows", "row0_back",
                                   "rows_past_max", "page_past_pool", "page_negative"])
 @pytest.mark.parametrize("big", [False, True])

@@ -167,3 +167,19 @@ def test_replayed_loop_equals_steps(gpu):
         one.append(tok)
     assert np.array_equal(np.array(one).T, g)
     dec.close()
+
+
+def test_forks_and_tokens_that_are_none(gpu):
+    rng = np.random.default_rng(4)
+    from moty_b200.decoder import PagedDecoder
+    W, layers, head = _model(gpu, rng, 4, 2, 32, 128, 256, 300, 1, True)
+    dec = PagedDecoder(layers, head, W["final_norm"], 4, 2, 32, pages=8, max_seqs=3, max_pages=4)
+    s = dec.new()
+    dec.run([(s, rng.integers(0, 300, 70))])
+    table, lens, free = dec.table.copy(), dec.lens.copy(), dec.kv.free_pages()
+    for bad in (lambda: dec.fork(s, 0), lambda: dec.fork(s, -1), lambda: dec.run([(s, [300])]), lambda: dec.run([(s, [5, -1])]),
+                lambda: dec.run([(s, [])]), lambda: dec.greedy([s], [300], 3), lambda: dec.greedy([s], [1, 2], 3), lambda: dec.greedy([s], [1], 0)):
+        with pytest.raises(gpu.MotyCudaError):
+            bad()
+        assert np.array_equal(table, dec.table) and np.array_equal(lens, dec.lens) and dec.kv.free_pages() == free
+    dec.close()
