@@ -450,24 +450,29 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         const size_t rh = (size_t)col[c] * a.H + col[NC + c];
         const float *p = part + rh * nsplit * (HD + 4);
         const float2 e = lane < live ? __ldcg(reinterpret_cast<const float2 *>(p + (size_t)lane * (HD + 4))) : make_float2(-INFINITY, 0.f);
-        float M = e.x;
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float f = kv4_factor(e.y, e.x, M);
+        float4 v[DEC_JOIN];                                  // (on their way beside the {m, l}: every value of a span at a lane's first four dims)
+#pragma unroll
+        for (int k = 0; k < DEC_JOIN; k++)
+            if (k < live && 4 * lane < HD) v[k] = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)k * (HD + 4) + 4 + 4 * lane));
+        const float M = warp_max_f32(e.x), f = kv4_factor(e.y, e.x, M);
         float L = e.y * f;
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        const float over = kv4_over(L);
 #pragma unroll
-        for (int d0 = 0; d0 < HD / 4; d0 += 32) {
-            const int d = 4 * (d0 + lane);
-            const bool mine = d < HD;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int k = 0; k < live; k++) {
-                const float fk = __shfl_sync(0xffffffffu, f, k);
-                const float4 v = mine ? __ldcg(reinterpret_cast<const float4 *>(p + (size_t)k * (HD + 4) + 4 + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                if (fk != 0.f) { o.x = fmaf(v.x, fk, o.x); o.y = fmaf(v.y, fk, o.y); o.z = fmaf(v.z, fk, o.z); o.w = fmaf(v.w, fk, o.w); }
+        for (int d0 = 0; d0 < HD; d0 += 128) {
+            const bool mine = d0 + 4 * lane < HD;
+            if (d0 > 0) {
+#pragma unroll
+                for (int k = 0; k < DEC_JOIN; k++)
+                    if (k < live && mine) v[k] = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)k * (HD + 4) + 4 + d0 + 4 * lane));
             }
-            if (mine)
-                *reinterpret_cast<float4 *>(a.ctx + rh * HD + d) = kv4_times(o, kv4_over(L));
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < DEC_JOIN; k++) {
+                const float fk = __shfl_sync(0xffffffffu, f, k);
+                if (k < live && fk != 0.f) { o.x = fmaf(v[k].x, fk, o.x); o.y = fmaf(v[k].y, fk, o.y); o.z = fmaf(v[k].z, fk, o.z); o.w = fmaf(v[k].w, fk, o.w); }
+            }
+            if (mine) *reinterpret_cast<float4 *>(a.ctx + rh * HD + d0 + 4 * lane) = kv4_times(o, over);
         }
     }
     if (tid == 0) count[u] = 0;                              // as the next launch finds it
