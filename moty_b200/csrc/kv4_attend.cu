@@ -27,7 +27,7 @@ namespace {
 // 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 104 us, 3.5 TB/s; one sequence of 131072, 32 heads on 4: 39 us;
 // 13 sequences, window 1024, hd 256: 19 us.  The steps measured at the first of these: codes straight from memory to
 // fragments 188 us, the ring 107 us, weight * step in f16 pairs and the joins in the launch 104 us.
-constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 16, DEC_WK = 7;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, weights' exponent
+constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_WK = 7;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, weights' exponent
 
 // CTAs an SM holds (registers)
 constexpr int kv4_decode_ctas(int NG, bool pair) { return NG <= 2 ? 4 : NG <= 4 ? (pair ? 4 : 3) : NG <= 6 ? (pair ? 3 : 2) : pair ? 3 : 2; }
@@ -450,29 +450,30 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         const size_t rh = (size_t)col[c] * a.H + col[NC + c];
         const float *p = part + rh * nsplit * (HD + 4);
         const float2 e = lane < live ? __ldcg(reinterpret_cast<const float2 *>(p + (size_t)lane * (HD + 4))) : make_float2(-INFINITY, 0.f);
-        float4 v[DEC_JOIN];                                  // (on their way beside the {m, l}: every value of a span at a lane's first four dims)
+        float4 v[16];                                        // the first spans' values on their way beside the {m, l}
+        auto fetch = [&](int k0, int d) {
 #pragma unroll
-        for (int k = 0; k < DEC_JOIN; k++)
-            if (k < live && 4 * lane < HD) v[k] = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)k * (HD + 4) + 4 + 4 * lane));
+            for (int k = 0; k < 16; k++)
+                if (k0 + k < live && d < HD) v[k] = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)(k0 + k) * (HD + 4) + 4 + d));
+        };
+        fetch(0, 4 * lane);
         const float M = warp_max_f32(e.x), f = kv4_factor(e.y, e.x, M);
         float L = e.y * f;
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         const float over = kv4_over(L);
-#pragma unroll
+#pragma unroll 1
         for (int d0 = 0; d0 < HD; d0 += 128) {
-            const bool mine = d0 + 4 * lane < HD;
-            if (d0 > 0) {
-#pragma unroll
-                for (int k = 0; k < DEC_JOIN; k++)
-                    if (k < live && mine) v[k] = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)k * (HD + 4) + 4 + d0 + 4 * lane));
-            }
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int k0 = 0; k0 < live; k0 += 16) {
+                if (d0 + k0 > 0) fetch(k0, d0 + 4 * lane);
 #pragma unroll
-            for (int k = 0; k < DEC_JOIN; k++) {
-                const float fk = __shfl_sync(0xffffffffu, f, k);
-                if (k < live && fk != 0.f) { o.x = fmaf(v[k].x, fk, o.x); o.y = fmaf(v[k].y, fk, o.y); o.z = fmaf(v[k].z, fk, o.z); o.w = fmaf(v[k].w, fk, o.w); }
+                for (int k = 0; k < 16; k++) {
+                    const float fk = __shfl_sync(0xffffffffu, f, k0 + k);
+                    if (k0 + k < live && fk != 0.f) { o.x = fmaf(v[k].x, fk, o.x); o.y = fmaf(v[k].y, fk, o.y); o.z = fmaf(v[k].z, fk, o.z); o.w = fmaf(v[k].w, fk, o.w); }
+                }
             }
-            if (mine) *reinterpret_cast<float4 *>(a.ctx + rh * HD + d0 + 4 * lane) = kv4_times(o, over);
+            if (d0 + 4 * lane < HD) *reinterpret_cast<float4 *>(a.ctx + rh * HD + d0 + 4 * lane) = kv4_times(o, over);
         }
     }
     if (tid == 0) count[u] = 0;                              // as the next launch finds it
@@ -552,25 +553,35 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
     const int live = kv4_live_spans(a, pl, j, row, h);
     float *out = a.ctx + ((size_t)row * a.H + h) * hd;
     const float *p = part + ((size_t)row * a.H + h) * pl.nsplit * (hd + 4);
+    // thread group k takes spans k, k + ng, ...: four dims a thread, group order fixed; the first eight of its spans are
+    // fetched beside the maxima
+    const int q4 = hd / 4, ng = MG_T / q4, k = tid / q4, d = tid - k * q4, mine = k < ng ? live : 0;
+    auto span = [&](int i) { return p + (size_t)i * (hd + 4); };
+    float2 e[8];
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+        if (k + u * ng < mine) {
+            e[u] = *reinterpret_cast<const float2 *>(span(k + u * ng));
+            v[u] = reinterpret_cast<const float4 *>(span(k + u * ng) + 4)[d];
+        }
     float M = -INFINITY;
-    for (int i = tid; i < live; i += MG_T) M = fmaxf(M, p[(size_t)i * (hd + 4)]);
+    for (int i = tid; i < live; i += MG_T) M = fmaxf(M, span(i)[0]);
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     if ((tid & 31) == 0) red[tid >> 5] = M;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < MG_T / 32; w++) M = fmaxf(M, red[w]);
-    // thread group k takes spans k, k + ng, ...: four dims a thread, group order fixed
-    const int q4 = hd / 4, ng = MG_T / q4, k = tid / q4, d = tid - k * q4;
     float L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (k < ng)
-        for (int i = k; i < live; i += ng) {
-            const float *pi = p + (size_t)i * (hd + 4);
-            const float li = pi[1], f = kv4_factor(li, pi[0], M);
-            const float4 v = *reinterpret_cast<const float4 *>(pi + 4 + 4 * d);
-            L = fmaf(li, f, L);
-            if (li != 0.f) { o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w); }
-        }
+    auto add = [&](const float2 &ml, const float4 &x) {
+        const float f = kv4_factor(ml.y, ml.x, M);
+        L = fmaf(ml.y, f, L);
+        if (ml.y != 0.f) { o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w); }
+    };
+#pragma unroll
+    for (int u = 0; u < 8; u++) if (k + u * ng < mine) add(e[u], v[u]);
+    for (int i = k + 8 * ng; i < mine; i += ng) add(*reinterpret_cast<const float2 *>(span(i)), reinterpret_cast<const float4 *>(span(i) + 4)[d]);
     if (k < ng) { os[k * q4 + d] = o; if (d == 0) ls[k] = L; }
     __syncthreads();
     if (k == 0) {
