@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         float L = e.y * f;
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         const float over = kv4_over(L);
-#pragma unroll 1
+#pragma unroll
         for (int d0 = 0; d0 < HD; d0 += 128) {
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
@@ -507,7 +507,7 @@ __device__ __forceinline__ int kv4_live_spans(const Kv4Attend &a, const Kv4Plan 
 // sums), so what counts is how many warps wait at once: 1568 rows x 20 heads x 96 dims in two spans 22 us, 130 us when a CTA
 // took a (row, head); with more spans than lanes a CTA does (kv4_merge_kernel).
 constexpr int MG_T = 256;
-__global__ void __launch_bounds__(MG_T, 4) kv4_merge_few_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
+__global__ void __launch_bounds__(MG_T, 3) kv4_merge_few_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
     const int hd = a.geo.hd, lane = threadIdx.x & 31, q4 = hd >> 2;
     const unsigned item = blockIdx.x * (MG_T / 32) + (threadIdx.x >> 5);
     pdl_trigger();
@@ -519,25 +519,30 @@ __global__ void __launch_bounds__(MG_T, 4) kv4_merge_few_kernel(Kv4Attend a, Kv4
     const int live = kv4_live_spans(a, pl, j, row, h);
     const float *p = part + (size_t)item * pl.nsplit * (hd + 4);
     const float2 ml = lane < live ? *reinterpret_cast<const float2 *>(p + (size_t)lane * (hd + 4)) : make_float2(-INFINITY, 0.f);
+    float4 v[8];                                             // the first spans' values on their way beside the {m, l}
+    auto fetch = [&](int i0, int d) {
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (i0 + u < live && d < q4) v[u] = reinterpret_cast<const float4 *>(p + (size_t)(i0 + u) * (hd + 4) + 4)[d];
+    };
+    fetch(0, lane);
     const float M = warp_max_f32(ml.x), f = kv4_factor(ml.y, ml.x, M);
     float L = ml.y * f;
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    const unsigned some = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    const float over = kv4_over(L);
+#pragma unroll 1
     for (int d0 = 0; d0 < q4; d0 += 32) {
-        const int d = d0 + lane < q4 ? d0 + lane : d0;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
         for (int i0 = 0; i0 < live; i0 += 8) {
-            float4 v[8];
-#pragma unroll
-            for (int u = 0; u < 8; u++)
-                if (i0 + u < live) v[u] = reinterpret_cast<const float4 *>(p + (size_t)(i0 + u) * (hd + 4) + 4)[d];
+            if (d0 + i0 > 0) fetch(i0, d0 + lane);
 #pragma unroll
             for (int u = 0; u < 8; u++) {
                 const float fi = __shfl_sync(0xffffffffu, f, i0 + u);
-                if (some >> (i0 + u) & 1) { o.x = fmaf(v[u].x, fi, o.x); o.y = fmaf(v[u].y, fi, o.y); o.z = fmaf(v[u].z, fi, o.z); o.w = fmaf(v[u].w, fi, o.w); }
+                if (fi != 0.f) { o.x = fmaf(v[u].x, fi, o.x); o.y = fmaf(v[u].y, fi, o.y); o.z = fmaf(v[u].z, fi, o.z); o.w = fmaf(v[u].w, fi, o.w); }
             }
         }
-        if (d0 + lane < q4) reinterpret_cast<float4 *>(a.ctx + (size_t)item * hd)[d] = kv4_times(o, kv4_over(L));
+        if (d0 + lane < q4) reinterpret_cast<float4 *>(a.ctx + (size_t)item * hd)[d0 + lane] = kv4_times(o, over);
     }
 }
 
