@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
 struct Kv4Join { int r0, n, len; };
 __device__ __forceinline__ Kv4Join kv4_join_row(const Kv4Attend &a, int row) {
     int seq, pos;
-    const int st = kv4_row(a.b, row, &seq, &pos);
+    const int st = kv4_row<32>(a.b, row, &seq, &pos);
     Kv4Join r{-1, 0, 0};
     if (st == KV4_ROW_NONE) return r;
     r.r0 = 0;

@@ -109,12 +109,16 @@ __device__ __forceinline__ unsigned kv4_quant8(const float (&x)[8], float d) {
 struct Kv4Rows { uint8_t *unit[ST_ROWS]; int t[ST_ROWS], seq[ST_ROWS]; };
 __device__ __forceinline__ void kv4_rows(Kv4Rows &s, const Kv4Geom &geo, uint8_t *mem, const Kv4Batch &b, int row0, int layer, int head, int *err,
                                          bool absent_ok) {
-    const int i = threadIdx.x, r = row0 + i;
-    if (i < ST_ROWS) {
+    // 16 lanes look for a row where there are many sequences (64: 6.7 us for their rows stored and fetched, 7.5 us with four
+    // lanes), else four, which is two warps instead of all (3 prompts of up to 4096 rows: 75.0 us, 76.6 us with 16)
+    const int w = b.nseq > 16 ? 4 : 2, i = threadIdx.x >> w, r = row0 + i;
+    int seq, pos, st = KV4_ROW_NONE;
+    if (w == 4) st = kv4_row<16>(b, r, &seq, &pos);
+    else if (i < ST_ROWS) st = kv4_row<4>(b, r, &seq, &pos);   // (whole warps)
+    if (i < ST_ROWS && (threadIdx.x & ((1 << w) - 1)) == 0) {
         uint8_t *unit = nullptr;
-        int seq = -1, pos = 0;
-        if (r < b.rows) {
-            const int st = kv4_row(b, r, &seq, &pos);
+        if (r >= b.rows) { seq = -1; pos = 0; }
+        else {
             if (st == KV4_ROW_BAD) atomicExch(err, 1);
             if (st == KV4_ROW_OK) {
                 const int page = b.table[(size_t)seq * b.ld + pos / KV4_PAGE];
@@ -207,7 +211,7 @@ __global__ void __launch_bounds__(256) kv4_append_rope_kernel(Kv4Geom geo, uint8
     const bool isq = slot < H;
     const int hh = isq ? slot : slot - H;
     int seq, pos;
-    const int st = kv4_row(b, r, &seq, &pos);
+    const int st = kv4_row<32>(b, r, &seq, &pos);
     if (st != KV4_ROW_OK) { if (st == KV4_ROW_BAD && i == 0) atomicExch(err, 1); return; }       // (the whole CTA)
     float *row = (isq ? q + (size_t)r * q_ld : k + (size_t)r * ld) + (size_t)hh * hd;
     const float *nw = isq ? a.qn : a.kn;

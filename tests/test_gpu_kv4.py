@@ -154,6 +154,22 @@ def test_append_and_fetch(gpu, t, hd, KV, rows, lens):
     p.status()
 
 
+@pytest.mark.parametrize("nseq", [16, 17, 40, 300])
+def test_append_and_fetch_many_sequences(gpu, t, nseq):
+    """Rows of many sequences in one batch, some with none."""
+    rng = np.random.default_rng(nseq)
+    lens = [int(x) for x in rng.integers(1, 90, nseq)]
+    p = Pool(gpu, t, 2, 64, lens, seed=nseq)
+    rows = [int(min(L, r)) for L, r in zip(lens, rng.choice([0, 0, 1, 1, 3, 20, 90], nseq))]
+    n = sum(rows)
+    k = t.full((n, 2 * 64), 7.0, device="cuda"); v = k.clone()
+    p.kv.fetch_dev(0, k.data_ptr(), v.data_ptr(), p.batch(rows), stream=p.sh())
+    for got, held in ((k, p.k), (v, p.v)):
+        want = np.concatenate([quant(x[L - r:])[0] for x, L, r in zip(held, lens, rows) if r]).reshape(n, -1)
+        assert np.array_equal(got.cpu().numpy(), want.astype(np.float32))
+    p.status()
+
+
 def test_append_strides_and_single_positions(gpu, t):
     """Rows inside wider rows; positions stored one call at a time leave their neighbours as they were."""
     KV, hd, L = 2, 96, 70

@@ -126,6 +126,34 @@ def test_rows_of_arrays_that_are_no_batch(h):
                 assert 0 <= r0.value and n.value > 0 and r0.value + n.value <= rows and n.value <= L.value <= ld * 64
 
 
+@pytest.mark.parametrize("nseq", [1, 2, 15, 16, 17, 64, 255, 256, 257, 5000])
+def test_rows_of_many_sequences(h, nseq):
+    """Every row finds its sequence among many, empty ones among them; offsets that do not ascend stay inside the arrays."""
+    rng = random.Random(nseq)
+    n = [rng.choice([0, 0, 1, 1, 2, 5]) for _ in range(nseq)]
+    off = [0]
+    for x in n:
+        off.append(off[-1] + x)
+    rows, ld = off[-1] + 3, 4
+    row0, pr = _i(off); ln, pl = _i([x + rng.randint(0, 200) for x in n])
+    s, p = C.c_int(), C.c_int()
+    at = 0
+    for r in range(rows):
+        while at < nseq and r >= off[at + 1]:
+            at += 1
+        st = h.row(nseq, rows, ld, pr, pl, r, C.byref(s), C.byref(p))
+        if at == nseq:
+            assert st == 0
+        else:
+            assert st == 1 and s.value == at and p.value == ln[at] - n[at] + r - off[at]
+    wild, pw = _i([rng.choice([-7, 0, 1, rows, 1 << 30, rng.randint(0, rows)]) for _ in range(nseq + 1)])
+    for r in range(rows):
+        st = h.row(nseq, rows, ld, pw, pl, r, C.byref(s), C.byref(p))
+        assert 0 <= s.value < nseq
+        if st == 1:
+            assert wild[s.value] <= r < wild[s.value + 1] and 0 <= p.value < ld * 64
+
+
 def test_page_books(h):
     rng = random.Random(1)
     N = 40
