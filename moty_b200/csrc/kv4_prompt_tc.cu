@@ -231,6 +231,8 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
             const int cc = c0 + tid, row = cc / a.G, g0 = cc - row * a.G, p = pos0 + row;
             src = a.q + (size_t)(sq.r0 + row) * a.q_ld + (size_t)(head * a.G + g0) * HD;
             rh = (size_t)(sq.r0 + row) * a.H + head * a.G + g0;
+#pragma unroll
+            for (int i = 0; i < NG; i++) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 32 * i));       // all of the tile's rows at once
             chi = p;
             clo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
         }
