@@ -20,13 +20,14 @@ namespace {
 // work a column, half the piece arithmetic.  Every warp keeps its own running maximum (moved only when a score passes it by
 // 8 in base-2 units, so weights stay below 256) and exponent of the largest value step.  Warps join in shared memory, spans
 // through `part` ({m, l, acc[hd]} per (row, head, split)): up to DEC_JOIN of them by the CTA of a tile that ends last
-// (1000 positions, 16 heads on 8: 7.8 us, 8.9 us with a second launch; 4 sequences of 4000, 32 heads: 12.7 and 14.2 us; 32
-// instead of 16 gained nothing more), others by the merge kernels below.
+// (1000 positions, 16 heads on 8: 6.8 us, with a second launch a microsecond more; 2 sequences of 8000 at hd 64, 17 to 32
+// spans: 9.7 us, 13.3 us with a second launch), others by the merge kernels below.  A join is a chain of waits, so it asks
+// for the sums of its spans before it knows their weights (7.8 -> 6.8 us; one sequence of 131072 39.8 -> 33.7 us).
 // What bounds it: instructions.  A warp's 16 positions of 128 dims against 4 columns take about 400 (32 matrix products,
 // the rest unpacking codes, the two pieces of weight * step, softmax), issued in 68 of 100 cycles; memory is not the limit:
-// 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 104 us, 3.5 TB/s; one sequence of 131072, 32 heads on 4: 39 us;
-// 13 sequences, window 1024, hd 256: 19 us.  The steps measured at the first of these: codes straight from memory to
-// fragments 188 us, the ring 107 us, weight * step in f16 pairs and the joins in the launch 104 us.
+// 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 103 us, 3.6 TB/s; one sequence of 131072, 32 heads on 4: 34 us;
+// 13 sequences, window 1024, hd 256: 17.7 us.  The steps measured at the first of these: codes straight from memory to
+// fragments 188 us, the ring 107 us, weight * step in f16 pairs and the joins in the launch 103 us.
 constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_WK = 7;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, weights' exponent
 
 // CTAs an SM holds (registers)
@@ -504,8 +505,8 @@ __device__ __forceinline__ int kv4_live_spans(const Kv4Attend &a, const Kv4Plan 
 }
 
 // Joins up to 32 spans of a (row, head): a warp each, a span's {m, l} a lane.  A chain of loads (the row's sequence, {m, l},
-// sums), so what counts is how many warps wait at once: 1568 rows x 20 heads x 96 dims in two spans 22 us, 130 us when a CTA
-// took a (row, head); with more spans than lanes a CTA does (kv4_merge_kernel).
+// sums), so what counts is how many warps wait at once: 1568 rows x 20 heads x 96 dims in two spans 22 us, 34 us with half the
+// warps, and 1024 rows x 32 heads x 128 dims in two 140 us when a CTA took a (row, head); with more spans than lanes a CTA does (kv4_merge_kernel).
 constexpr int MG_T = 256;
 __global__ void __launch_bounds__(MG_T, 3) kv4_merge_few_kernel(Kv4Attend a, Kv4Plan pl, const float *part) {
     const int hd = a.geo.hd, lane = threadIdx.x & 31, q4 = hd >> 2;
@@ -603,18 +604,18 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
 // How a call is cut.  Host numbers only (the limits the caller gave), so a captured call stays valid for any batch within
 // them.  Which kernel, by (row, query head) pairs of a KV head ("columns"):
 //   decode, which re-reads the pages for every 8 columns, up to 64 of them, up to 48 where the tensor-memory kernel has the
-//     heads' width and their dims are many (8 sequences of 4096, 8 KV heads, hd 128: 72 us against 91 / 88 us of the prompt
-//     kernels at 48 columns, 108 against 95 / 90 us at 64; hd 64, 64 columns: 59 against 75 / 72 us; hd 256: 186 against
-//     191 us);
+//     heads' width and their dims are many (8 sequences of 4096, 8 KV heads, hd 128: 72 us against 89 / 85 us of the prompt
+//     kernels at 48 columns, 107 against 92 / 87 us at 64; hd 64, 64 columns: 59 against 74 / 65 us; hd 256: 185 against
+//     179 us, and one sequence of 1024 16 against 31 us);
 //   tensor memory above 64 columns at hd 64, 96, 128 when there are more than six pages of 64 columns an SM: below that its
-//     set-up (15 us) is more than the matrix work it saves (one sequence of 1024, 8 KV heads, hd 128, 256 columns: 24 us
-//     against 21 us of the other; of 4096: 32 us against 52 us; 8 of 4096: 125 us against 330 us).
+//     set-up (13 us) is more than the matrix work it saves (one sequence of 1024, 8 KV heads, hd 128, 256 columns: 25 us
+//     against 20 us of the other; of 4096: 33 us against 51 us; 8 of 4096: 119 us against 327 us).
 // Spans of decode: with `units` (sequence, KV head, tile) triples of P pages on `slots` resident CTAs, a CTA costs its pages
 // plus about FIX pages' time of set-up and join.  When all CTAs are resident at once the longest one counts; otherwise the
 // total work over the slots plus a last CTA (lengths of a ragged batch are taken as 0.6 of the limit).  The cut with the
-// least of that (64 sequences of up to 8192 positions, 32 heads on 8: 104 us).  A prompt is cut only to fill the GPU: the
-// joins move rows x heads x hd x spans f32 values (4096 rows at 4096 positions, 16 heads: 176 us whole, 277 us in two spans;
-// nine ragged sequences of up to 333 rows and 2900 positions 108 us whole, 129 us in two).
+// least of that (64 sequences of up to 8192 positions, 32 heads on 8: 103 us).  A prompt is cut only to fill the GPU: the
+// joins move rows x heads x hd x spans f32 values (4096 rows at 4096 positions, 16 heads: 174 us whole, 250 us in two spans;
+// nine ragged sequences of up to 333 rows and 2900 positions 105 us whole, 124 us in two).
 Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     Kv4Plan p{};
     const long long cols = (long long)a.max_rows * a.G;

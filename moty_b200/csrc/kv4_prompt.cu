@@ -11,8 +11,8 @@
 // units) and the exponent of the largest value step as in the decode kernel.
 // It serves the head widths that the tensor-memory kernel has no operand tiles for, and calls too short for that kernel's
 // set-up.  What bounds it: two pieces make two matrix instructions of half the rate a product, and turning codes into
-// operands is done by every warp for itself; 4096 rows at 4096 positions, 16 heads on 8, hd 128: 587 us (tensor memory:
-// 176 us), one sequence of 1024, 64 rows, 32 heads on 8: 21 us (24 us).
+// operands is done by every warp for itself; 4096 rows at 4096 positions, 16 heads on 8, hd 128: 573 us (tensor memory:
+// 174 us), one sequence of 1024, 64 rows, 32 heads on 8: 20 us (25 us).
 #include "kv4_frag.cuh"
 #include "kv4_attend.cuh"
 
