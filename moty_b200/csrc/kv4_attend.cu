@@ -28,8 +28,10 @@ namespace {
 // 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 103 us, 3.6 TB/s; one sequence of 131072, 32 heads on 4: 34 us;
 // 13 sequences, window 1024, hd 256: 17.7 us.  The steps measured at the first of these: codes straight from memory to
 // fragments 188 us, the ring 107 us, weight * step in f16 pairs and the joins in the launch 103 us.
-constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_WK = 7;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, weights' exponent
+constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_WK = 7, DEC_F = 16;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, weights' exponent, pages of a matrix unit's sum
 
+// the most pages of a span whose sums stay in the matrix unit (one or two products a page)
+constexpr int kv4_decode_long(bool pair) { return pair ? 32 : 20; }
 // CTAs an SM holds (registers)
 constexpr int kv4_decode_ctas(int NG, bool pair) { return NG <= 2 ? 4 : NG <= 4 ? (pair ? 4 : 3) : NG <= 6 ? (pair ? 3 : 2) : pair ? 3 : 2; }
 template <int NG, bool PAIR> struct DecL {
@@ -41,7 +43,8 @@ template <int NG, bool PAIR> struct DecL {
     static constexpr int SMEM = BODY + NC * HD * 4 + (2 * DEC_W * NC + 4 * NC + DEC_NP) * 4;
 };
 
-template <int NG, bool PAIR>
+// LONG: spans of more pages than the matrix unit's own sums are good for (see tot below).
+template <int NG, bool PAIR, bool LONG>
 __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part, int *count) {
     using Lay = DecL<NG, PAIR>;
     constexpr int HD = NG * 32, NC = Lay::NC, UNIT = 72 * HD, STAGE = Lay::STAGE, NS = PAIR ? 1 : 2, NCP = (36 * NG + 31) / 32, DEC_ST = Lay::ST;
@@ -169,6 +172,12 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
     for (int g = 0; g < NG; g++)
 #pragma unroll
         for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] = 0.f;
+    // The matrix unit cuts its sums off, it does not round them, 1.6e-8 of a result a product: with 99 pages to a span and two
+    // products a page results were 3.2e-6 off, with kv4_decode_long pages 0.6e-6 at most.  Of longer spans what acc holds is
+    // added to rounded sums every DEC_F pages.  These lie in local memory, and the code beside the loop costs 10 % (64
+    // sequences of up to 8192: 114 us), so shorter spans have a kernel without.
+    volatile float tot[LONG ? NG * 8 : 1];
+    int pages = 0;                                           // (tot holds nothing before DEC_F of them)
     for (int it = 0, slot = 0; it < np; it++) {
         cp_async_wait<DEC_ST - 2>();
         __syncwarp();                                        // everyone's pieces of page `it` are here, and page it - 1 is done with
@@ -262,6 +271,9 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                     for (int g = 0; g < NG; g++)
 #pragma unroll
                         for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] *= f;
+                    if (LONG && pages >= DEC_F)
+#pragma unroll
+                        for (int i = 0; i < NG * 8; i++) tot[LONG ? i : 0] *= f;
                 }
             }
         }
@@ -291,9 +303,14 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                 for (int g = 0; g < NG; g++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {            // the thread's output columns are its score columns
-                        acc[g][i >> 1][PAIR ? (i & 1) * 2 : (i & 1) * 2 + k] *= f;
-                        if (PAIR) acc[g][i >> 1][(i & 1) * 2 + 1] *= f;
+                        const int at = PAIR ? (i & 1) * 2 : (i & 1) * 2 + k;
+                        acc[g][i >> 1][at] *= f;
+                        if (PAIR) acc[g][i >> 1][at + 1] *= f;
                     }
+                if (LONG && pages >= DEC_F)
+#pragma unroll
+                    for (int i = 0; i < NG * 8; i++) if (PAIR || (i & 1) == k) tot[LONG ? i : 0] *= f;
+
             }
         }
         // scaled weights of positions 2 j, 2 j + 1, 2 j + 8, 2 j + 9 for column r
@@ -384,7 +401,23 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         };
         if (t0 >= cr.lo_all && t0 + 15 < cr.hi_all) body(std::true_type{});
         else body(std::false_type{});
+        if (LONG && ++pages % DEC_F == 0) {
+            const bool first = pages == DEC_F;
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    volatile float &s = tot[LONG ? 8 * g + i : 0];
+                    s = first ? acc[g][i >> 2][i & 3] : s + acc[g][i >> 2][i & 3];
+                    acc[g][i >> 2][i & 3] = 0.f;
+                }
+        }
     }
+    if (LONG && pages >= DEC_F)
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] += tot[LONG ? 8 * g + i : 0];
     // join the warps: a thread holds dims 32 g + 4 r + 0 .. 3 of its score columns
     cp_async_wait<0>();
     __syncthreads();
@@ -662,7 +695,7 @@ size_t kv4_attend_counters(const Kv4Attend &a, const Kv4Plan &p) {
     return p.decode && p.nsplit > 1 && p.nsplit <= DEC_JOIN ? (size_t)a.b.nseq * a.geo.KV * p.ntile : 0;
 }
 
-template <int NG, bool PAIR>
+template <int NG, bool PAIR, bool LONG>
 static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *count, cudaStream_t st) {
     constexpr size_t smem = DecL<NG, PAIR>::SMEM;
     static bool attr[MOTY_MAX_DEV];
@@ -670,17 +703,19 @@ static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, int 
     CK(cudaGetDevice(&dev));
     if (dev < 0 || dev >= MOTY_MAX_DEV) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: device %d", dev);
     if (!attr[dev]) {
-        CK(cudaFuncSetAttribute(kv4_decode_kernel<NG, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        CK(cudaFuncSetAttribute(kv4_decode_kernel<NG, PAIR, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         attr[dev] = true;
     }
     const long long grid = (long long)a.b.nseq * a.geo.KV * p.ntile * p.nsplit;
     if (grid > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend: %lld CTAs", grid);
-    CK(moty_launch_pdl(kv4_decode_kernel<NG, PAIR>, dim3((unsigned)grid), dim3(DEC_W * 32), smem, st, a, p.ntile, p.nsplit, p.span, part, count));
+    CK(moty_launch_pdl(kv4_decode_kernel<NG, PAIR, LONG>, dim3((unsigned)grid), dim3(DEC_W * 32), smem, st, a, p.ntile, p.nsplit, p.span, part, count));
     return 0;
 }
 template <int NG>
 static int kv4_decode_go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *count, cudaStream_t st) {
-    return p.cols == 4 ? kv4_decode_go<NG, true>(a, p, part, count, st) : kv4_decode_go<NG, false>(a, p, part, count, st);
+    const bool pair = p.cols == 4;
+    if (p.span / KV4_PAGE > kv4_decode_long(pair)) return pair ? kv4_decode_go<NG, true, true>(a, p, part, count, st) : kv4_decode_go<NG, false, true>(a, p, part, count, st);
+    return pair ? kv4_decode_go<NG, true, false>(a, p, part, count, st) : kv4_decode_go<NG, false, false>(a, p, part, count, st);
 }
 
 // part: scratch of kv4_attend_scratch_bytes; count: kv4_attend_counters ints, all zero (and left so)

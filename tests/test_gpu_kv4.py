@@ -465,6 +465,31 @@ def test_attend_one_long_sequence_among_short_ones(gpu, t, nseq, rows, H, KV, hd
     p.status()
 
 
+@pytest.mark.parametrize("H,KV,nseq", [(128, 16, 7), (64, 16, 8), (16, 16, 40)])
+def test_attend_long_sums_of_one_sign(gpu, t, H, KV, nseq):
+    """Flat weights and positive values: all sums grow evenly.  The matrix unit cuts each of its sums off by at most 2^-23 of the
+    sum so far.  Of at most 20 pages of two products, 16 where sums are passed on, or 32 of one, that is 20 x 2^-23 of the
+    whole at most and half of that on the average; passing on (31 times at most), four warps, the spans (fewer than 32) and
+    the quotient round to nearest, half a 2^-23 each at most, the earlier ones of smaller sums: another 20 x 2^-23 at most
+    and nothing on the average.  A score (below 2 in magnitude) is off by less than 2 x 2^-23 x 8, its weight by that much
+    and the exponential's 2 x 2^-23: another 20."""
+    hd, L = 32, 31680
+    p = Pool(gpu, t, KV, hd, [L], seed=H)
+    p.v[0] = np.abs(p.v[0]) + np.float32(0.5)
+    p.store()
+    q = p.rng.standard_normal((nseq, H, hd)).astype(np.float32)
+    got = p.attend(q, H, [1] * nseq, lens=[L] * nseq, table=np.repeat(p.table, nseq, 0), scale=0.05).reshape(nseq, H, hd)
+    k, v = quant(p.k[0])[0], quant(p.v[0])[0]
+    rel = []
+    for s, h in [(0, 0), (0, H - 1), (nseq - 1, H // 2), (nseq // 2, 1)]:
+        want, _ = attend64(k[:, h // (H // KV)][:, None], v[:, h // (H // KV)][:, None], q[s:s + 1, h:h + 1], np.array([L - 1]), 1, scale=0.05)
+        rel.append((got[s, h] - want[0, 0]) / want[0, 0])
+    rel = np.array(rel)
+    assert np.max(np.abs(rel)) <= 60 * 2.0**-23
+    assert abs(np.mean(rel)) <= 10 * 2.0**-23
+    p.status()
+
+
 @pytest.mark.parametrize("rows", [1, 20])
 def test_attend_does_not_depend_on_the_neighbours(gpu, t, rows):
     """A sequence's result is the same bits alone with the same limits and beside others."""
