@@ -51,7 +51,7 @@ __device__ __forceinline__ void kv4_put_v(uint8_t *unit, int hd, int t, int g, i
 // two positions of a pair leave as one word and neighbouring threads write neighbouring bytes.  A warp a group, a value a
 // lane (as the single-row kernel below has it) spent 188 us on 3 sequences' 4096-row prompts of 16 heads, hd 128 (append and
 // fetch: 248 MB, 38 us at the copy rate); this 75 us, 47 of them the append, which issues instructions four cycles of five:
-// two exact maxima, a correctly rounded step and eight codes a thread.  64 single rows: 6.9 us both, launch and look-up latency.
+// two exact maxima, a correctly rounded step and eight codes a thread.  64 single rows: 6.6 us both, launch and look-up latency.
 constexpr int ST_ROWS = 16, ST_T = 256;
 
 // The quad's step for x[8] a thread: *d = its bits, returns it (0 for a group of zeros, NaN for one that is not finite).
