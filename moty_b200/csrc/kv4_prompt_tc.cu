@@ -119,6 +119,11 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     const bool ok = pt_wait(bar, parity, abort_flag);
     return __all_sync(0xffffffffu, ok);
 }
+// a warpgroup's registers a thread (all four warps run it)
+template <bool MORE, int N> __device__ __forceinline__ void role_registers() {
+    if constexpr (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 // the warps of one role: a barrier of their own (1 keys, 2 values), and whether all of them say yes
 template <int ID, int N> __device__ __forceinline__ void role_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
 template <int ID, int N> __device__ __forceinline__ bool role_and(bool ok) {
@@ -280,118 +285,88 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
     const int n = sh.n;
     volatile int *abort_flag = &sh.abort;
 
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_REST));      // (512 x 128 at launch)
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFT));
-    if (warp == 15) {
-        // ---- the products ----
-        const uint32_t id_s = (1u << 4) | (64u >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
-        const uint32_t id_o = (1u << 4) | ((uint32_t)HD >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
-        const uint32_t q0 = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint32_t dq = desc_lo(q0), dk = desc_lo(q0 + L::OFF_K), dv = desc_lo(q0 + L::OFF_V);     // (offsets below do not leave 14 bits)
-        const uint32_t lead = elect_one();
-        bool ok = true;
-        for (int j = 0; j <= n && ok; j++) {
-            if (j < n) {                                     // S of page j (its buffer: the O of page j - 2 was issued before)
-                ok = warp_wait(&sh.kfull, j & 1, abort_flag);
-                if (!ok) break;
-                tc_after();
-#pragma unroll 1
-                for (int y = 0; y < nx; y++) {
-                    const uint32_t d = tm + TM_S + (y * 2 + (j & 1)) * 64, q = dq + y * (2 * L::Q >> 4);
-#pragma unroll
-                    for (int term = 0; term < 3; term++)     // q lo * k hi, q hi * k lo, q hi * k hi
-#pragma unroll
-                        for (int s = 0; s < 2 * NG; s++)
-                            umma_ss(d, q + (((term == 0 ? L::Q : 0) + (s >> 2) * (PT_M * 128) + (s & 3) * 32) >> 4),
-                                    dk + (((term == 1 ? L::K : 0) + (s >> 2) * (64 * 128) + (s & 3) * 32) >> 4), id_s, (term | s) != 0, lead);
-                    if (lead) umma_commit(&sh.sfull[y][j & 1]);
-                    __syncwarp();
-                }
-            }
-            if (j > 0) {                                     // O of page j - 1
-                const int i = j - 1;
-                ok = warp_wait(&sh.vfull, i & 1, abort_flag);
-#pragma unroll 1
-                for (int y = 0; y < nx && ok; y++) {
-                    ok = warp_wait(&sh.pfull[y][i & 1], i >> 1 & 1, abort_flag) && warp_wait(&sh.oempty[y], (i & 1) ^ 1, abort_flag);
+    // ---- pages into shared memory, then as operand tiles ----
+    const __half2 down = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
+    // Steps of a staged part: positions that no line sees become 0 (their memory may hold anything), steps that would
+    // overflow and NaN steps of values are noted; all of it rare, and looked for two steps at a time.  Returns what
+    // the part's values have been divided by.  (The barrier in it also says that all have left the page before.)
+    auto look = [&](auto keys_, int w, int j, uint32_t *st) {
+        constexpr bool keys = decltype(keys_)::value;
+        constexpr int ID = keys ? 1 : 2, N = keys ? PT_KT : PT_VT;
+        const int t0 = list[j].y;
+        bool odd = t0 < cr.lo_any || t0 + KV4_PAGE > cr.hi_any;
+        for (int i = w; i < 32 * NG; i += N) odd |= (((st[i] & 0x7fff7fffu) + 0x14001400u) & 0x80008000u) != 0;      // |step| >= 4096, infinity, NaN
+        if (role_and<ID, N>(!odd)) return 1.f;
+        if (w == 0) sh.big[keys] = 0;
+        role_sync<ID, N>();
+        uint16_t *h = reinterpret_cast<uint16_t *>(st);
+        for (int i = w; i < 64 * NG; i += N) {
+            const int t = i / NG, g = i - t * NG;
+            uint16_t v = h[i];
+            if (t0 + t < cr.lo_any || t0 + t >= cr.hi_any) v = 0;
+            if ((v & 0x7fff) >= 0x7c00) {
+                if (!keys) { atomicOr(&sh.nan[j & 7][g], 1ull << t); sh.anynan[j & 7] = 1; v = 0; }
+            } else if ((v & 0x7fff) >= 0x6c00) sh.big[keys] = 1;
+            h[i] = v;
+        }
+        role_sync<ID, N>();
+        const float f = sh.big[keys] ? 16.f : 1.f;
+        role_sync<ID, N>();
+        return f;
+    };
+    // The roles by warpgroup; each takes its registers first thing in its own branch, so that what the compiler gives a role's
+    // code is bounded by the number the role holds (512 x 128 at launch).
+    if (warp >= 12) {
+        role_registers<false, PT_REGS_REST>();
+        if (warp == 15) {
+            // ---- the products ----
+            const uint32_t id_s = (1u << 4) | (64u >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
+            const uint32_t id_o = (1u << 4) | ((uint32_t)HD >> 3) << 17 | (uint32_t)(PT_M >> 4) << 24;
+            const uint32_t q0 = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t dq = desc_lo(q0), dk = desc_lo(q0 + L::OFF_K), dv = desc_lo(q0 + L::OFF_V);     // (offsets below do not leave 14 bits)
+            const uint32_t lead = elect_one();
+            bool ok = true;
+            for (int j = 0; j <= n && ok; j++) {
+                if (j < n) {                                     // S of page j (its buffer: the O of page j - 2 was issued before)
+                    ok = warp_wait(&sh.kfull, j & 1, abort_flag);
                     if (!ok) break;
                     tc_after();
-                    const uint32_t d = tm + TM_O + y * 128, p = tm + TM_S + (y * 2 + (i & 1)) * 64;
-#pragma unroll
-                    for (int term = 0; term < 3; term++)     // p lo * v hi, p hi * v lo, p hi * v hi
-#pragma unroll
-                        for (int s = 0; s < 4; s++)
-                            umma_ts(d, p + s * 16 + (term == 0 ? 8 : 0), dv + (((term == 1 ? L::V : 0) + s * 32) >> 4), id_o,
-                                    (term | s) != 0, lead);
-                    if (lead) umma_commit(&sh.pvdone[y]);
-                    __syncwarp();
-                }
-            }
-        }
-    } else if (warp >= 8) {
-        // ---- pages into shared memory, then as operand tiles ----
-        const __half2 down = __half2half2(__ushort_as_half(0x2c00));         // 1 / 16
-        // Steps of a staged part: positions that no line sees become 0 (their memory may hold anything), steps that would
-        // overflow and NaN steps of values are noted; all of it rare, and looked for two steps at a time.  Returns what
-        // the part's values have been divided by.  (The barrier in it also says that all have left the page before.)
-        auto look = [&](auto keys_, int w, int j, uint32_t *st) {
-            constexpr bool keys = decltype(keys_)::value;
-            constexpr int ID = keys ? 1 : 2, N = keys ? PT_KT : PT_VT;
-            const int t0 = list[j].y;
-            bool odd = t0 < cr.lo_any || t0 + KV4_PAGE > cr.hi_any;
-            for (int i = w; i < 32 * NG; i += N) odd |= (((st[i] & 0x7fff7fffu) + 0x14001400u) & 0x80008000u) != 0;      // |step| >= 4096, infinity, NaN
-            if (role_and<ID, N>(!odd)) return 1.f;
-            if (w == 0) sh.big[keys] = 0;
-            role_sync<ID, N>();
-            uint16_t *h = reinterpret_cast<uint16_t *>(st);
-            for (int i = w; i < 64 * NG; i += N) {
-                const int t = i / NG, g = i - t * NG;
-                uint16_t v = h[i];
-                if (t0 + t < cr.lo_any || t0 + t >= cr.hi_any) v = 0;
-                if ((v & 0x7fff) >= 0x7c00) {
-                    if (!keys) { atomicOr(&sh.nan[j & 7][g], 1ull << t); sh.anynan[j & 7] = 1; v = 0; }
-                } else if ((v & 0x7fff) >= 0x6c00) sh.big[keys] = 1;
-                h[i] = v;
-            }
-            role_sync<ID, N>();
-            const float f = sh.big[keys] ? 16.f : 1.f;
-            role_sync<ID, N>();
-            return f;
-        };
-        bool ok = true;
-        if (warp < 12) {
-            const int w = tid - 256;
-            for (int j = 0; j < n; j++) {
-                uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW;
-                ok = warp_wait(&sh.rawk[j & 1], j >> 1 & 1, abort_flag);
-                if (!role_and<1, PT_KT>(ok)) break;
-                if (w == 0 && j > 0 && j + 1 < n) load_k(j + 1);
-                const float f = look(std::true_type{}, w, j, reinterpret_cast<uint32_t *>(raw + L::RK));
-                if (w == 0) sh.fk[j & 7] = f;
-                // the keys of page j - 1 are done with (a warp that gives up goes on to the next barrier, where all leave)
-                if (j > 0 && !warp_wait(&sh.sfull[nx - 1][(j - 1) & 1], (j - 1) >> 1 & 1, abort_flag)) continue;
 #pragma unroll 1
-                for (int it = w; it < 256; it += PT_KT) {    // position t, piece jj of a group's four
-                    const int t = (it >> 5) * 8 + (it & 7), jj = it >> 3 & 3;
-                    unsigned kw[NG], st[(NG + 1) / 2];
-                    kv4_ldsw<NG>(kw, raw + t * (HD / 2) + jj * (4 * NG));
-                    kv4_ldsteps<NG>(st, raw + L::RK + t * (2 * NG));
+                    for (int y = 0; y < nx; y++) {
+                        const uint32_t d = tm + TM_S + (y * 2 + (j & 1)) * 64, q = dq + y * (2 * L::Q >> 4);
 #pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        __half2 d = __half2half2(__ushort_as_half((unsigned short)(g & 1 ? st[g >> 1] >> 16 : st[g >> 1])));
-                        if (f != 1.f) d = __hmul2(d, down);
-                        unsigned h[4], l[4];
-                        kv4_values_hl(kw[g], d, h, l);
-                        const int c = 4 * g + jj;
-                        uint8_t *dst = sm + L::OFF_K + (c >> 3) * (64 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4 *>(dst + L::K) = make_uint4(l[0], l[1], l[2], l[3]);
+                        for (int term = 0; term < 3; term++)     // q lo * k hi, q hi * k lo, q hi * k hi
+#pragma unroll
+                            for (int s = 0; s < 2 * NG; s++)
+                                umma_ss(d, q + (((term == 0 ? L::Q : 0) + (s >> 2) * (PT_M * 128) + (s & 3) * 32) >> 4),
+                                        dk + (((term == 1 ? L::K : 0) + (s >> 2) * (64 * 128) + (s & 3) * 32) >> 4), id_s, (term | s) != 0, lead);
+                        if (lead) umma_commit(&sh.sfull[y][j & 1]);
+                        __syncwarp();
                     }
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&sh.kfull);
+                if (j > 0) {                                     // O of page j - 1
+                    const int i = j - 1;
+                    ok = warp_wait(&sh.vfull, i & 1, abort_flag);
+#pragma unroll 1
+                    for (int y = 0; y < nx && ok; y++) {
+                        ok = warp_wait(&sh.pfull[y][i & 1], i >> 1 & 1, abort_flag) && warp_wait(&sh.oempty[y], (i & 1) ^ 1, abort_flag);
+                        if (!ok) break;
+                        tc_after();
+                        const uint32_t d = tm + TM_O + y * 128, p = tm + TM_S + (y * 2 + (i & 1)) * 64;
+#pragma unroll
+                        for (int term = 0; term < 3; term++)     // p lo * v hi, p hi * v lo, p hi * v hi
+#pragma unroll
+                            for (int s = 0; s < 4; s++)
+                                umma_ts(d, p + s * 16 + (term == 0 ? 8 : 0), dv + (((term == 1 ? L::V : 0) + s * 32) >> 4), id_o,
+                                        (term | s) != 0, lead);
+                        if (lead) umma_commit(&sh.pvdone[y]);
+                        __syncwarp();
+                    }
+                }
             }
         } else {
+            // ---- values of a page ----
+            bool ok = true;
             const int w = tid - 384;
             for (int j = 0; j < n; j++) {
                 uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW + L::RK + L::RST;
@@ -431,131 +406,170 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                 mbar_arrive(&sh.vfull);
             }
         }
-    } else if (x < nx) {
-        // ---- softmax: a thread a line ----
-        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        float m = -INFINITY, l = 0.f, o[HD];
-        unsigned nanbits = 0;
-#pragma unroll
-        for (int i = 0; i < HD; i++) o[i] = 0.f;
-        float f = 1.f;                                       // what the O of the page before is still to be multiplied by
+    } else if (warp >= 8) {
+        role_registers<false, PT_REGS_REST>();
+        // ---- keys of a page ----
         bool ok = true;
-        for (int j = 0; j <= n; j++) {
-            const int t0 = j < n ? list[j].y : 0;
-            if (j < n) {
-                ok = warp_wait(&sh.sfull[x][j & 1], j >> 1 & 1, abort_flag);
-                if (!ok) break;
-                tc_after();
-                const float ds = desc * sh.fk[j & 7];
-                const bool inside = t0 >= cr.lo_all && t0 + KV4_PAGE <= cr.hi_all;
-                const uint32_t at = mine + TM_S + (x * 2 + (j & 1)) * 64;
-                float mx = -INFINITY;
-                // (loops kept rolled: unrolled, the roles' code together outgrew the instruction cache)
+        const int w = tid - 256;
+        for (int j = 0; j < n; j++) {
+            uint8_t *raw = sm + L::OFF_RAW + (j & 1) * L::RAW;
+            ok = warp_wait(&sh.rawk[j & 1], j >> 1 & 1, abort_flag);
+            if (!role_and<1, PT_KT>(ok)) break;
+            if (w == 0 && j > 0 && j + 1 < n) load_k(j + 1);
+            const float f = look(std::true_type{}, w, j, reinterpret_cast<uint32_t *>(raw + L::RK));
+            if (w == 0) sh.fk[j & 7] = f;
+            // the keys of page j - 1 are done with (a warp that gives up goes on to the next barrier, where all leave)
+            if (j > 0 && !warp_wait(&sh.sfull[nx - 1][(j - 1) & 1], (j - 1) >> 1 & 1, abort_flag)) continue;
 #pragma unroll 1
-                for (int q = 0; q < 2; q++) {
-                    float v[32];
-                    tm_ld32(v, at + q * 32);
-                    if (!inside) {
+            for (int it = w; it < 256; it += PT_KT) {    // position t, piece jj of a group's four
+                const int t = (it >> 5) * 8 + (it & 7), jj = it >> 3 & 3;
+                unsigned kw[NG], st[(NG + 1) / 2];
+                kv4_ldsw<NG>(kw, raw + t * (HD / 2) + jj * (4 * NG));
+                kv4_ldsteps<NG>(st, raw + L::RK + t * (2 * NG));
 #pragma unroll
-                        for (int i = 0; i < 32; i++) { const int t = t0 + q * 32 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(v[i], v[i + 1]));
-                }
-                mx *= ds;                                    // (the scale is positive)
-                const bool up = mx > m + 8.f;
-                f = 1.f;
-                if (__any_sync(0xffffffffu, up)) {
-                    if (up) { f = kv4_exp2(m - mx); m = mx; }
-                    __syncwarp();
-                    l *= f;
-#pragma unroll
-                    for (int i = 0; i < HD; i++) o[i] *= f;
-                }
-                // weights times 2^6, as hi and lo pairs of consecutive positions, over the scores: 16 columns become 8 of hi
-                // and 8 of lo (a line that has seen nothing yet: all 0)
-                const float mm = m == -INFINITY ? 0.f : m - 6.f;
-                float s0 = 0.f, s1 = 0.f;
-#pragma unroll 1
-                for (int q = 0; q < 4; q++) {
-                    float v[16];
-                    tm_ld16(v, at + q * 16);
-                    if (!inside) {
-#pragma unroll
-                        for (int i = 0; i < 16; i++) { const int t = t0 + q * 16 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
-                    }
-                    unsigned ph[8], pl[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float p0 = kv4_exp2(fmaf(v[2 * i], ds, -mm)), p1 = kv4_exp2(fmaf(v[2 * i + 1], ds, -mm));
-                        s0 += p0; s1 += p1;
-                        kv4_pieces(p0, p1, ph[i], pl[i]);
-                    }
-                    tm_st8(at + q * 16, ph);
-                    tm_st8(at + q * 16 + 8, pl);
-                }
-                l += s0 + s1;
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_before();
-                mbar_arrive(&sh.pfull[x][j & 1]);
-            } else f = 1.f;
-            if (j > 0) {                                     // O of page j - 1 to the registers
-                const int i0 = j - 1;
-                ok = warp_wait(&sh.pvdone[x], i0 & 1, abort_flag);
-                if (!ok) break;
-                tc_after();
-                const float g = f * sh.fv[i0 & 7];
-#pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    float v[32];
-                    tm_ld32(v, mine + TM_O + x * 128 + c);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) o[c + i] = fmaf(v[i], g, o[c + i]);
-                }
-                tc_before();
-                mbar_arrive(&sh.oempty[x]);
-                if (sh.anynan[i0 & 7]) {
-                    const int tn = list[i0].y;
-                    for (int gg = 0; gg < NG; gg++)
-                        for (unsigned long long mk = sh.nan[i0 & 7][gg]; mk; mk &= mk - 1) {
-                            const int t = tn + __ffsll((long long)mk) - 1;
-                            if (t >= clo && t <= chi) nanbits |= 1u << gg;
-                        }
-                    __syncwarp();
+                for (int g = 0; g < NG; g++) {
+                    __half2 d = __half2half2(__ushort_as_half((unsigned short)(g & 1 ? st[g >> 1] >> 16 : st[g >> 1])));
+                    if (f != 1.f) d = __hmul2(d, down);
+                    unsigned h[4], l[4];
+                    kv4_values_hl(kw[g], d, h, l);
+                    const int c = 4 * g + jj;
+                    uint8_t *dst = sm + L::OFF_K + (c >> 3) * (64 * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(dst + L::K) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&sh.kfull);
         }
-        // out through the tile's query rows (their products are done), so that a warp writes whole lines: a thread puts its
-        // line there in pieces of four dims, turned by the line so that eight lanes meet eight bank groups
-        if (__all_sync(0xffffffffu, ok)) {
-            float4 *box = reinterpret_cast<float4 *>(sm + 2 * x * L::Q) + (warp & 3) * (32 * HD / 4);
-            if (tid < ncol && nsplit > 1) *reinterpret_cast<float2 *>(part + (rh * nsplit + split) * (HD + 4)) = make_float2(m, l);
-            const float over = nsplit > 1 ? 1.f : kv4_over(l);
+    } else {
+        role_registers<true, PT_REGS_SOFT>();
+        if (x < nx) {
+            // ---- softmax: a thread a line ----
+            const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            float m = -INFINITY, l = 0.f, o[HD];
+            unsigned nanbits = 0;
 #pragma unroll
-            for (int c = 0; c < HD / 4; c++) {
-                const float no = nanbits >> (c >> 3) & 1 ? __int_as_float(0x7fffffff) : 0.f;
-                box[lane * (HD / 4) + (c ^ (lane & 7))] = make_float4(fmaf(o[4 * c], over, no), fmaf(o[4 * c + 1], over, no), fmaf(o[4 * c + 2], over, no), fmaf(o[4 * c + 3], over, no));
+            for (int i = 0; i < HD; i++) o[i] = 0.f;
+            float f = 1.f;                                       // what the O of the page before is still to be multiplied by
+            bool ok = true;
+            for (int j = 0; j <= n; j++) {
+                const int t0 = j < n ? list[j].y : 0;
+                if (j < n) {
+                    ok = warp_wait(&sh.sfull[x][j & 1], j >> 1 & 1, abort_flag);
+                    if (!ok) break;
+                    tc_after();
+                    const float ds = desc * sh.fk[j & 7];
+                    const bool inside = t0 >= cr.lo_all && t0 + KV4_PAGE <= cr.hi_all;
+                    const uint32_t at = mine + TM_S + (x * 2 + (j & 1)) * 64;
+                    float mx = -INFINITY;
+                    // (loops kept rolled: unrolled, the roles' code together outgrew the instruction cache)
+#pragma unroll 1
+                    for (int q = 0; q < 2; q++) {
+                        float v[32];
+                        tm_ld32(v, at + q * 32);
+                        if (!inside) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) { const int t = t0 + q * 32 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(v[i], v[i + 1]));
+                    }
+                    mx *= ds;                                    // (the scale is positive)
+                    const bool up = mx > m + 8.f;
+                    f = 1.f;
+                    if (__any_sync(0xffffffffu, up)) {
+                        if (up) { f = kv4_exp2(m - mx); m = mx; }
+                        __syncwarp();
+                        l *= f;
+#pragma unroll
+                        for (int i = 0; i < HD; i++) o[i] *= f;
+                    }
+                    // weights times 2^6, as hi and lo pairs of consecutive positions, over the scores: 16 columns become 8 of hi
+                    // and 8 of lo (a line that has seen nothing yet: all 0)
+                    const float mm = m == -INFINITY ? 0.f : m - 6.f;
+                    float s0 = 0.f, s1 = 0.f;
+#pragma unroll 1
+                    for (int q = 0; q < 4; q++) {
+                        float v[16];
+                        tm_ld16(v, at + q * 16);
+                        if (!inside) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) { const int t = t0 + q * 16 + i; if (t < clo || t > chi) v[i] = -INFINITY; }
+                        }
+                        unsigned ph[8], pl[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float p0 = kv4_exp2(fmaf(v[2 * i], ds, -mm)), p1 = kv4_exp2(fmaf(v[2 * i + 1], ds, -mm));
+                            s0 += p0; s1 += p1;
+                            kv4_pieces(p0, p1, ph[i], pl[i]);
+                        }
+                        tm_st8(at + q * 16, ph);
+                        tm_st8(at + q * 16 + 8, pl);
+                    }
+                    l += s0 + s1;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_before();
+                    mbar_arrive(&sh.pfull[x][j & 1]);
+                } else f = 1.f;
+                if (j > 0) {                                     // O of page j - 1 to the registers
+                    const int i0 = j - 1;
+                    ok = warp_wait(&sh.pvdone[x], i0 & 1, abort_flag);
+                    if (!ok) break;
+                    tc_after();
+                    const float g = f * sh.fv[i0 & 7];
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        float v[32];
+                        tm_ld32(v, mine + TM_O + x * 128 + c);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[c + i] = fmaf(v[i], g, o[c + i]);
+                    }
+                    tc_before();
+                    mbar_arrive(&sh.oempty[x]);
+                    if (sh.anynan[i0 & 7]) {
+                        const int tn = list[i0].y;
+                        for (int gg = 0; gg < NG; gg++)
+                            for (unsigned long long mk = sh.nan[i0 & 7][gg]; mk; mk &= mk - 1) {
+                                const int t = tn + __ffsll((long long)mk) - 1;
+                                if (t >= clo && t <= chi) nanbits |= 1u << gg;
+                            }
+                        __syncwarp();
+                    }
+                }
             }
-            __syncwarp();
-            float *const to = nsplit == 1 ? a.ctx + rh * HD : part + (rh * nsplit + split) * (HD + 4) + 4;
+            // out through the tile's query rows (their products are done), so that a warp writes whole lines: a thread puts its
+            // line there in pieces of four dims, turned by the line so that eight lanes meet eight bank groups
+            if (__all_sync(0xffffffffu, ok)) {
+                float4 *box = reinterpret_cast<float4 *>(sm + 2 * x * L::Q) + (warp & 3) * (32 * HD / 4);
+                if (tid < ncol && nsplit > 1) *reinterpret_cast<float2 *>(part + (rh * nsplit + split) * (HD + 4)) = make_float2(m, l);
+                const float over = nsplit > 1 ? 1.f : kv4_over(l);
+#pragma unroll
+                for (int c = 0; c < HD / 4; c++) {
+                    const float no = nanbits >> (c >> 3) & 1 ? __int_as_float(0x7fffffff) : 0.f;
+                    box[lane * (HD / 4) + (c ^ (lane & 7))] = make_float4(fmaf(o[4 * c], over, no), fmaf(o[4 * c + 1], over, no), fmaf(o[4 * c + 2], over, no), fmaf(o[4 * c + 3], over, no));
+                }
+                __syncwarp();
+                float *const to = nsplit == 1 ? a.ctx + rh * HD : part + (rh * nsplit + split) * (HD + 4) + 4;
 #pragma unroll 8
-            for (int i = 0; i < HD / 4; i++) {
-                const int at = i * 32 + lane, line = at / (HD / 4), c = at - line * (HD / 4);
-                float4 *dst = reinterpret_cast<float4 *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), line));
-                if ((warp & 3) * 32 + line + x * PT_M < ncol) dst[c] = box[line * (HD / 4) + (c ^ (line & 7))];
+                for (int i = 0; i < HD / 4; i++) {
+                    const int at = i * 32 + lane, line = at / (HD / 4), c = at - line * (HD / 4);
+                    float4 *dst = reinterpret_cast<float4 *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), line));
+                    if ((warp & 3) * 32 + line + x * PT_M < ncol) dst[c] = box[line * (HD / 4) + (c ^ (line & 7))];
+                }
             }
         }
     }
+    // (behind the roles nothing is kept in registers from before them: what is needed is read anew)
     tc_before();
     __syncthreads();
     tc_after();
     if (sh.abort) {                                          // products still on their way are given time before their memory goes
-        if (tid == 0) atomicExch(err_wait, 1);
+        if (threadIdx.x == 0) atomicExch(err_wait, 1);
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == 15) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (threadIdx.x >> 5 == 15) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "r"(512));
     }
 }
 
