@@ -6,12 +6,13 @@
 //     O = P V     [128 x hd]     three products: p lo * v hi, p hi * v lo, p hi * v hi
 // f32 accuracy from f16 operands: an operand is hi + lo, f16 each.  A value held is code * step, 4 x 11 bits, so k and v are
 // exact as hi + lo (the rest of an f16 product is a multiple of the smallest f16); q (scaled by a power of two a line) and
-// the softmax weights carry 22 bits; the dropped lo * lo term is 2^-22 of a product.  Steps of 4096 and more would overflow
+// the softmax weights (scaled by a power of two a line and page) carry 22 bits down to an end: 2^-38 of the line's largest
+// query value, 2^-39 of its largest weight on the page; the dropped lo * lo term is 2^-22 of a product.  Steps of 4096 and more would overflow
 // f16: a page that has one is brought down by 2^4.  O starts from zero at every page and is added to f32 registers, because
 // the tensor core's own sum drifts over a long prompt.
-//   warps 0-3, 4-7   softmax of a tile, a thread a line: S from TMEM, running maximum (moved when passed by 8 in base-2
-//               units), weights back to TMEM over the scores as the A operand of the second product, then the O of the page
-//               before added to the registers
+//   warps 0-3, 4-7   softmax of a tile, a thread a line: S from TMEM, running maximum (a whole number of base-2 units,
+//               moved when passed by 8), weights back to TMEM over the scores as the A operand of the second product, then
+//               the O of the page before added to the registers
 //   warps 8-11, 12-14   keys and values of a page: bulk copies of codes and steps into shared memory (two pages deep), then k
 //               and v^T operand tiles (K-major, 128-byte swizzle): eight key dims of a position, or eight positions of a
 //               value dim, are one 16-byte piece
@@ -450,10 +451,11 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
             unsigned nanbits = 0;
 #pragma unroll
             for (int i = 0; i < HD; i++) o[i] = 0.f;
-            float f = 1.f;                                       // what the O of the page before is still to be multiplied by
+            float f = 1.f, b = 0.f;                              // what the O of the page before is still to be multiplied by: m's move, its weights' scale
             bool ok = true;
             for (int j = 0; j <= n; j++) {
                 const int t0 = j < n ? list[j].y : 0;
+                const float before = b;
                 if (j < n) {
                     ok = warp_wait(&sh.sfull[x][j & 1], j >> 1 & 1, abort_flag);
                     if (!ok) break;
@@ -475,18 +477,20 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                         for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(v[i], v[i + 1]));
                     }
                     mx *= ds;                                    // (the scale is positive)
-                    const bool up = mx > m + 8.f;
+                    const float mc = ceilf(mx);
+                    const bool up = mc > m + 8.f;
                     f = 1.f;
                     if (__any_sync(0xffffffffu, up)) {
-                        if (up) { f = kv4_exp2(m - mx); m = mx; }
+                        if (up) { f = kv4_two_to(m - mc); m = mc; }
                         __syncwarp();
                         l *= f;
 #pragma unroll
                         for (int i = 0; i < HD; i++) o[i] *= f;
                     }
-                    // weights times 2^6, as hi and lo pairs of consecutive positions, over the scores: 16 columns become 8 of hi
-                    // and 8 of lo (a line that has seen nothing yet: all 0)
-                    const float mm = m == -INFINITY ? 0.f : m - 6.f;
+                    // weights as hi and lo pairs of consecutive positions, over the scores: 16 columns become 8 of hi and 8 of
+                    // lo.  They are brought up to 2^15 by the largest of the line on THIS page (lo ends at 2^-24, which
+                    // then is 2^-39 of it), not by the largest so far, which one position may hold; bn takes it back.
+                    const float mm = mx == -INFINITY ? 0.f : mc - 15.f, bn = mx == -INFINITY ? 0.f : kv4_two_to(mm - m);
                     float s0 = 0.f, s1 = 0.f;
 #pragma unroll 1
                     for (int q = 0; q < 4; q++) {
@@ -506,7 +510,8 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                         tm_st8(at + q * 16, ph);
                         tm_st8(at + q * 16 + 8, pl);
                     }
-                    l += s0 + s1;
+                    l = fmaf(s0 + s1, bn, l);
+                    b = bn;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_before();
                     mbar_arrive(&sh.pfull[x][j & 1]);
@@ -516,7 +521,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                     ok = warp_wait(&sh.pvdone[x], i0 & 1, abort_flag);
                     if (!ok) break;
                     tc_after();
-                    const float g = f * sh.fv[i0 & 7];
+                    const float g = f * before * sh.fv[i0 & 7];
 #pragma unroll
                     for (int c = 0; c < HD; c += 32) {
                         float v[32];

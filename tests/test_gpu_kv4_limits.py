@@ -1,0 +1,82 @@
+"""GPU: the paged 4-bit KV cache where attention's sums are hard -- one position that takes nearly all the weight and holds
+nothing, groups of dims far smaller than the others, long sums of one sign -- and the corners of calls, forks and moves.
+
+Scores here are exact: a query row holds a single 1, a key row a single value of few bits, so that a score is that value.
+What is left, with e = 2^-24 and scores that span `gap` (natural units):
+  * a weight: scale and log2(e) as f32 2 e gap, the exponent's rounding e (gap + 11) (base-2 arguments end 16 below or above
+    their reference), exp2 4 e; numerator and denominator, and joins by two more exp2:  (6 gap + 46) e;
+  * weight, step and value as 16-bit pieces, the quotient: 8 e;
+  * sums of at most 64 products in a matrix unit, which cuts them off, 2 e each: 128 e; then f32 sums of at most T / 16
+    roundings, each at random e of what is there so far (the values' signs are random: three times the root of half of them).
+|error| <= e (6 gap + 182 + 3 sqrt(T / 32)) |result|, in the 2-norm over the 32 dims of a group: of every group by itself.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_kv4 import Pool, attend64, check, quant
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def t():
+    import torch
+    torch.backends.cuda.matmul.allow_tf32 = False
+    return torch
+
+
+# (query heads, rows a sequence, head width): the prompt kernel of tensor memory.  40 sequences of 8 KV heads share one table: a
+# CTA walks many pages.
+KERNELS = [(32, 20, 64), (32, 20, 96), (32, 20, 128)]
+NSEQ, KV = 40, 8
+
+
+def hard(gpu, t, H, rows, hd, T, scores, values, window=0):
+    """Attention of NSEQ sequences over one, and what it should be for some of the rows: (got, want) [n][hd], the scores' span."""
+    p = Pool(gpu, t, KV, hd, [T], seed=H * hd + rows + T)
+    rng = p.rng
+    s = rng.integers(0, 3, T) / 8                            # "even"
+    if scores.startswith("sink"):                            # position 0 stands far above the others, and holds nothing
+        s[0] = float(scores[4:])
+    elif scores == "ragged":                                 # pages of very different weight
+        s = np.round(rng.standard_normal(T) * 48) / 8 + 4 * np.round(rng.standard_normal(T // 64 + 1))[np.arange(T) // 64]
+    p.k[0][:] = 0; p.k[0][:, :, 0] = s[:, None]
+    if scores.startswith("sink"):
+        p.v[0][0] = 0
+    if values == "small":
+        p.v[0] *= np.float32(2**-6)
+    if values == "groups":                                   # the last group's values are 2^14 times smaller
+        p.v[0] *= np.float32(2**-4); p.v[0][:, :, hd - 32:] *= np.float32(2**-14)
+    p.store()
+    q = np.zeros((NSEQ * rows, H, hd), np.float32); q[:, :, 0] = 1
+    got = p.attend(q, H, [rows] * NSEQ, window=window, scale=1.0, lens=[T] * NSEQ, table=np.repeat(p.table, NSEQ, 0)).reshape(NSEQ, rows, H, hd)
+    p.status()
+    k, v = quant(p.k[0])[0], quant(p.v[0])[0]
+    assert np.array_equal(k[:, 0, 0], s) and not k[:, :, 1:].any()
+    a, b = [], []
+    for i, r, h in [(0, 0, 0), (0, rows - 1, H - 1), (NSEQ - 1, rows // 2, H // 2), (NSEQ // 2, rows - 1, 1)]:
+        pos = T - rows + r
+        lo = max(0, pos - window + 1) if window else 0
+        w = np.exp(s[lo:pos + 1] - s[lo:pos + 1].max())
+        a.append(got[i, r, h]); b.append(w @ v[lo:pos + 1, h // (H // KV)] / w.sum())
+    return np.array(a), np.array(b), float(s.max() - s.min())
+
+
+def group_errors(got, want):
+    d = (got - want).reshape(len(want), -1, 32)
+    return np.linalg.norm(d, axis=-1) / np.linalg.norm(want.reshape(d.shape), axis=-1)
+
+
+@pytest.mark.parametrize("T", [2065, 5000])
+@pytest.mark.parametrize("scores,values", [("sink10", "plain"), ("sink14", "plain"), ("sink14", "small"), ("even", "groups"), ("ragged", "small")])
+@pytest.mark.parametrize("H,rows,hd", KERNELS)
+def test_attend_small_weights_and_small_values_keep_their_bits(gpu, t, H, rows, hd, scores, values, T):
+    if values == "groups" and hd == 32:
+        values = "small"                                     # (one group)
+    got, want, gap = hard(gpu, t, H, rows, hd, T, scores, values)
+    assert group_errors(got, want).max() <= E * (6 * gap + 182 + 3 * math.sqrt(T / 32))
