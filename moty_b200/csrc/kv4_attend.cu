@@ -17,8 +17,12 @@ namespace {
 //     output  [32 dims x columns]     += codes [dims x 16 positions] * (weight * value step) pieces
 // PAIR (up to four columns): hi and lo piece of a column are neighbouring columns of one product and land in the same
 // thread, which adds them.  Otherwise eight columns, and hi and lo are two products into the same sums: the same matrix
-// work a column, half the piece arithmetic.  Every warp keeps its own running maximum (moved only when a score passes it by
-// 8 in base-2 units, so weights stay below 256) and exponent of the largest value step.  Warps join in shared memory, spans
+// work a column, half the piece arithmetic.  Every warp keeps its own exponent of the largest value step, and for each column a
+// reference that weights are scaled by, a whole number of base-2 units: where the largest weight of a page leaves 2^6 .. 2^15
+// it is moved to put that one at 2^10, up or down (at 2^15 where others of the page lie 10 below it), for the lower piece
+// ends at 2^-24, and one position that holds nearly all the weight must not take the bits of those beside and after it (that
+// costs 2 %: 64 sequences of up to 8192 103.2 -> 105.5 us; a look at every column's largest on every page, and less
+// room above, 5 %).  Warps join in shared memory, spans
 // through `part` ({m, l, acc[hd]} per (row, head, split)): up to DEC_JOIN of them by the CTA of a tile that ends last
 // (1000 positions, 16 heads on 8: 6.8 us, with a second launch a microsecond more; 2 sequences of 8000 at hd 64, 17 to 32
 // spans: 9.7 us, 13.3 us with a second launch), others by the merge kernels below.  A join is a chain of waits, so it asks
@@ -28,7 +32,9 @@ namespace {
 // 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 103 us, 3.6 TB/s; one sequence of 131072, 32 heads on 4: 34 us;
 // 13 sequences, window 1024, hd 256: 17.7 us.  The steps measured at the first of these: codes straight from memory to
 // fragments 188 us, the ring 107 us, weight * step in f16 pairs and the joins in the launch 103 us.
-constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_WK = 7, DEC_F = 16;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, weights' exponent, pages of a matrix unit's sum
+constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_F = 16;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, pages of a matrix unit's sum
+// exponents of a page's largest weight: the range it may have (DEC_LOW: where each four positions have one as large), where it is put, and how far below the highest reference so far one may be
+constexpr float DEC_HI = 15.f, DEC_LO = 6.f, DEC_LOW = 4.f, DEC_AT = 10.f, DEC_DOWN = 60.f;
 
 // the most pages of a span whose sums stay in the matrix unit (one or two products a page)
 constexpr int kv4_decode_long(bool pair) { return pair ? 32 : 20; }
@@ -163,11 +169,11 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         clo[k] = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
     }
     const int phi = col[2 * NC + (PAIR ? r >> 1 : r)], plo = a.window > 0 ? phi - a.window + 1 : 0;      // limits of operand column r
-    float m[NS], l[NS], acc[NG][2][4];
+    float m[NS], mh[NS], l[NS], acc[NG][2][4];
     float vth = 0.f;                                         // 2^(e + 1) for the exponent e of the largest value step so far
     int dk = 0;                                              // exponent of the steps' factor; see below
 #pragma unroll
-    for (int k = 0; k < NS; k++) { m[k] = -INFINITY; l[k] = 0.f; }   // m: the running maximum less DEC_WK; l: weights times 2^DEC_WK; acc: times 2^(DEC_WK + dk)
+    for (int k = 0; k < NS; k++) { m[k] = mh[k] = -INFINITY; l[k] = 0.f; }   // m: the reference, mh: the highest so far; l: weights over 2^m; acc: times 2^dk too
 #pragma unroll
     for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -243,9 +249,10 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                     if (t < clo[k] || t > chi[k]) { see &= ~(1u << (2 * k + h)); s[k][h] = 0.f; }
                 }
         }
-        // Weights (below 256) are scaled by 2^DEC_WK, to below 2^15.  Where the largest value step so far (NaN left aside), of
-        // exponent e, is 1 or more or below 2^-8, steps are scaled by 2^dk, dk = -1 - e: weight * step stays below 2^15 and its
-        // pieces keep their bits.
+        // Weights stay below 2^15.  Where the largest value step so far (NaN left aside), of exponent e, is 1 or more or below
+        // 2^-4, steps are scaled by 2^dk, dk = -1 - e: weight * step stays below 2^15, and a page's largest weight (2^4 or
+        // more, see below) times that step is 1 or more: pieces end at 2^-25 of it, and at 2^-19 in a group whose steps are 64
+        // times smaller.
         {
             __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
 #pragma unroll
@@ -264,7 +271,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             if (__any_sync(0xffffffffu, big >= vth)) {
                 const unsigned b = __reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23;           // e + 127
                 if (b) {                                     // (f16 subnormals are normal f32; all steps 0: nothing to add, any scale does)
-                    const int e = (int)b - 127, k = e > -1 || e < -8 ? -1 - e : 0;                       // -16 .. 23
+                    const int e = (int)b - 127, k = e > -1 || e < -4 ? -1 - e : 0;                       // -16 .. 23
                     const float f = kv4_pow2(k - dk);
                     vth = kv4_pow2(e + 1); dk = k;
 #pragma unroll
@@ -278,27 +285,49 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             }
         }
         float e[NS][2];                                      // base-2 exponents of the scaled weights
-        bool up = false;
-        constexpr float thr = 8.f + DEC_WK;
+        bool odd = false;                                    // a cheap look first: the largest of each four positions within the range
+        float big[NS];
 #pragma unroll
-        for (int k = 0; k < NS; k++)
+        for (int k = 0; k < NS; k++) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 e[k][h] = fmaf(s[k][h], desc[k], -m[k]);
                 if (!inside && !(see >> (2 * k + h) & 1)) e[k][h] = -INFINITY;
-                up |= e[k][h] > thr;
             }
-        if (__any_sync(0xffffffffu, up)) {
+            big[k] = fmaxf(e[k][0], e[k][1]);
+            big[k] = fmaxf(big[k], __shfl_xor_sync(0xffffffffu, big[k], 16));
+            odd |= !(big[k] > DEC_LOW && big[k] <= DEC_HI);
+        }
+        bool move = __any_sync(0xffffffffu, odd);
+        if (move) {
+            move = false;
+#pragma unroll
+            for (int k = 0; k < NS; k++) {                   // (a column is lane j of every quad; its largest decides)
+                const unsigned large = __ballot_sync(0xffffffffu, big[k] > DEC_LO) & 0x11111111u << j;
+                move |= big[k] > DEC_HI;
+                move |= !large && m[k] > mh[k] - DEC_DOWN;
+            }
+            move = __any_sync(0xffffffffu, move);
+        }
+        if (move) {
 #pragma unroll
             for (int k = 0; k < NS; k++) {
-                float mx = m[k];
+                float mx = -INFINITY, mn = INFINITY;
 #pragma unroll
-                for (int h = 0; h < 2; h++) if (see >> (2 * k + h) & 1) mx = fmaxf(mx, s[k][h] * desc[k] - (float)DEC_WK);
-                for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                float f = mx == -INFINITY ? 1.f : kv4_exp2(m[k] - mx);
-                m[k] = mx; l[k] *= f;
+                for (int h = 0; h < 2; h++) if (see >> (2 * k + h) & 1) { mx = fmaxf(mx, s[k][h] * desc[k]); mn = fminf(mn, s[k][h] * desc[k]); }
+                for (int o = 4; o < 32; o <<= 1) {
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+                }
+                // one far above the others of its own page: no room above it, for their bits; within the range or nothing seen:
+                // the reference is left where it is
+                float to = ceilf(mx) - (mx - mn > DEC_AT ? DEC_HI : DEC_AT);
+                if (mx == -INFINITY || (mx - m[k] > DEC_LO && mx - m[k] <= DEC_HI)) to = m[k];
+                to = fmaxf(to, mh[k] - DEC_DOWN);
+                const float f = to == m[k] ? 1.f : kv4_two_to(m[k] - to);
+                m[k] = to; mh[k] = fmaxf(mh[k], to); l[k] *= f;
 #pragma unroll
-                for (int h = 0; h < 2; h++) e[k][h] = see >> (2 * k + h) & 1 ? fmaf(s[k][h], desc[k], -mx) : -INFINITY;
+                for (int h = 0; h < 2; h++) e[k][h] = see >> (2 * k + h) & 1 ? fmaf(s[k][h], desc[k], -to) : -INFINITY;
 #pragma unroll
                 for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -421,7 +450,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
     // join the warps: a thread holds dims 32 g + 4 r + 0 .. 3 of its score columns
     cp_async_wait<0>();
     __syncthreads();
-    const float vs = kv4_pow2(-DEC_WK - dk), ls = kv4_pow2(-DEC_WK);
+    const float vs = kv4_pow2(-dk);
 #pragma unroll
     for (int k = 0; k < NS; k++) {
         for (int o = 4; o < 32; o <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], o);
@@ -433,7 +462,7 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
             for (int i = 0; i < 4; i++) o[i] = (PAIR ? acc[g][i >> 1][(i & 1) * 2] + acc[g][i >> 1][(i & 1) * 2 + 1] : acc[g][i >> 1][(i & 1) * 2 + k]) * vs;
             *reinterpret_cast<float4 *>(js + ((size_t)warp * NC + c) * HD + g * 32 + 4 * r) = make_float4(o[0], o[1], o[2], o[3]);
         }
-        if (r == 0) { ml[warp * NC + c] = m[k] + (float)DEC_WK; ml[DEC_W * NC + warp * NC + c] = l[k] * ls; }
+        if (r == 0) { ml[warp * NC + c] = m[k]; ml[DEC_W * NC + warp * NC + c] = l[k]; }
     }
     __syncthreads();
     if (warp == 0 && lane < NC) {                            // the factor of each warp's sums; m and l of all

@@ -30,9 +30,9 @@ def t():
     return torch
 
 
-# (query heads, rows a sequence, head width): the prompt kernel of tensor memory.  40 sequences of 8 KV heads share one table: a
-# CTA walks many pages.
-KERNELS = [(32, 20, 64), (32, 20, 96), (32, 20, 128)]
+# (query heads, rows a sequence, head width): decode of four and of eight columns, the prompt kernel of tensor memory.  40
+# sequences of 8 KV heads share one table: a CTA walks many pages.
+KERNELS = [(8, 1, 32), (8, 1, 128), (8, 1, 256), (64, 1, 64), (64, 1, 128), (16, 4, 224), (32, 20, 64), (32, 20, 96), (32, 20, 128)]
 NSEQ, KV = 40, 8
 
 
@@ -72,7 +72,7 @@ def group_errors(got, want):
     return np.linalg.norm(d, axis=-1) / np.linalg.norm(want.reshape(d.shape), axis=-1)
 
 
-@pytest.mark.parametrize("T", [2065, 5000])
+@pytest.mark.parametrize("T", [70, 2065, 5000])
 @pytest.mark.parametrize("scores,values", [("sink10", "plain"), ("sink14", "plain"), ("sink14", "small"), ("even", "groups"), ("ragged", "small")])
 @pytest.mark.parametrize("H,rows,hd", KERNELS)
 def test_attend_small_weights_and_small_values_keep_their_bits(gpu, t, H, rows, hd, scores, values, T):
