@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int PR_W = KV4_LINES / 16;                         // warps a CTA
+constexpr int PR_W = KV4_LINES / 16, PR_F = 16;              // warps a CTA; pages of a lower sum
 
 template <int NG> struct PrL {
     static constexpr int HD = NG * 32, UNIT = 72 * HD, PT = NG <= 4 ? 4 : 2;
@@ -108,10 +108,22 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
     for (int g = 0; g < NG; g++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[g][i >> 2][i & 3] = 0.f;
+    // Sums over a long span are made in two levels: l and acc take PR_F pages and are then added to lt and tot (in local
+    // memory), which keep the maximum and the scale that they were left with.  One level alone: 131072 flat weights 1e-4 off.
+    volatile float lt[2] = {0.f, 0.f}, mt[2] = {-INFINITY, -INFINITY}, vnt = 0.f, tot[NG * 16];
+    int passes = 0;                                          // (tot holds nothing before PR_F pages of them)
     float vth = 0.f, vn = 0.f;                               // 2^(e + 1) and 64 * 2^-e for the exponent e of the largest value step so far
     const int *tab = a.b.table + (size_t)seq * a.b.ld;
     const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
     const size_t page_bytes = kv4_page_bytes(a.geo);
+    // factors that bring lt (of a line) and tot to the present maximum and scale
+    auto total_factors = [&](float (&fl)[2], float (&fa)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            fl[h] = mt[h] == m[h] ? 1.f : kv4_exp2(mt[h] - m[h]);
+            fa[h] = vnt == vn ? fl[h] : vnt == 0.f ? 0.f : fl[h] * (vn / vnt);
+        }
+    };
     auto fetch = [&](int t, int buf) {                       // the unit of position t's page to a stage; false: absent
         bool ok = false;
         if (t < t_hi) {
@@ -202,15 +214,17 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[g][i >> 2][i & 3] *= f[(i & 3) >> 1];
             }
+            float lp[2] = {0.f, 0.f};
 #pragma unroll
             for (int nt = 0; nt < PT; nt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     float p = kv4_exp2(s[nt][i] - m[i >> 1]);
                     if (!inside && !(see >> (4 * nt + i) & 1)) p = 0.f;
-                    l[i >> 1] += p;
+                    lp[i >> 1] += p;
                     s[nt][i] = p;
                 }
+            l[0] += lp[0]; l[1] += lp[1];
             // The pass's own sums start from zero and are added to acc by an ordinary f32 addition: the matrix unit cuts a
             // sum off instead of rounding it, and over a long prompt a sum kept in it drifts (4096 positions: 1.9e-6 off,
             // this way 6e-7, as the f32 torch form is).
@@ -280,9 +294,36 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
 #pragma unroll
                 for (int i = 0; i < 16; i++) acc[g][i >> 2][i & 3] += c[i >> 2][i & 3];
             }
+            if (++passes % (PR_F * KV4_PAGE / (8 * PT)) == 0) {
+                float fl[2], fa[2];
+                total_factors(fl, fa);
+#pragma unroll
+                for (int h = 0; h < 2; h++) { lt[h] = fmaf(lt[h], fl[h], l[h]); l[h] = 0.f; mt[h] = m[h]; }
+                vnt = vn;
+                const bool first = passes == PR_F * KV4_PAGE / (8 * PT);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {               // (a group's loads together: one by one they were a fifth of the kernel's time)
+                    float old[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) old[i] = first ? 0.f : tot[16 * g + i];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        float &x = acc[g][i >> 2][i & 3];
+                        tot[16 * g + i] = fmaf(old[i], fa[(i & 3) >> 1], x);
+                        x = 0.f;
+                    }
+                }
+            }
         }
     }
     // a thread holds, for lines r and r + 8, dims 32 g + 8 j + 0 .. 7: dim i + 4 k of them in acc[g][i][line half * 2 + k]
+    if (passes >= PR_F * KV4_PAGE / (8 * PT)) {
+        float fl[2], fa[2];
+        total_factors(fl, fa);
+        l[0] = fmaf(lt[0], fl[0], l[0]); l[1] = fmaf(lt[1], fl[1], l[1]);
+#pragma unroll
+        for (int i = 0; i < 16 * NG; i++) acc[i >> 4][i >> 2 & 3][i & 3] = fmaf(tot[i], fa[(i & 3) >> 1], acc[i >> 4][i >> 2 & 3][i & 3]);
+    }
     const float vs = vn == 0.f ? 1.f : 1.f / vn;             // (a power of two)
 #pragma unroll
     for (int hlf = 0; hlf < 2; hlf++) {

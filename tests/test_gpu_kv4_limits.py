@@ -80,3 +80,24 @@ def test_attend_small_weights_and_small_values_keep_their_bits(gpu, t, H, rows, 
         values = "small"                                     # (one group)
     got, want, gap = hard(gpu, t, H, rows, hd, T, scores, values)
     assert group_errors(got, want).max() <= E * (6 * gap + 182 + 3 * math.sqrt(T / 32))
+
+
+@pytest.mark.parametrize("H,KV,nseq,rows,hd", [(8, 2, 80, 20, 32), (8, 2, 80, 20, 256)])
+def test_attend_prompts_with_long_sums_of_one_sign(gpu, t, H, KV, nseq, rows, hd):
+    """Weights of three sizes and positive values: every sum grows evenly, and additions to a large sum round the same way
+    again and again.  Sums of at most 64 passes and of 1024 positions each (T / 1024 of them) err by e a step at most, a
+    pass's products by 8 e, numerator and denominator; weights and pieces by (6 gap + 54) e."""
+    T = 66000
+    p = Pool(gpu, t, KV, hd, [T], seed=hd)
+    s = p.rng.integers(0, 3, T) / 8
+    p.k[0][:] = 0; p.k[0][:, :, 0] = s[:, None]
+    p.v[0] = np.abs(p.v[0]) + np.float32(0.5)
+    p.store()
+    q = np.zeros((nseq * rows, H, hd), np.float32); q[:, :, 0] = 1
+    got = p.attend(q, H, [rows] * nseq, scale=1.0, lens=[T] * nseq, table=np.repeat(p.table, nseq, 0)).reshape(nseq, rows, H, hd)
+    p.status()
+    v = quant(p.v[0])[0]
+    for i, r, h in [(0, 0, 0), (nseq - 1, rows - 1, H - 1)]:
+        w = np.exp(s[:T - rows + r + 1] - 0.25)
+        want = w @ v[:T - rows + r + 1, h // (H // KV)] / w.sum()
+        assert np.abs(got[i, r, h] / want - 1).max() <= E * (2 * (8 + 64 + T / 1024) + 6 * 0.25 + 54)
