@@ -18,8 +18,9 @@ namespace {
 // PAIR (up to four columns): hi and lo piece of a column are neighbouring columns of one product and land in the same
 // thread, which adds them.  Otherwise eight columns, and hi and lo are two products into the same sums: the same matrix
 // work a column, half the piece arithmetic.  Every warp keeps its own exponent of the largest value step, and for each column a
-// reference that weights are scaled by, a whole number of base-2 units: where the largest weight of a page leaves 2^6 .. 2^15
-// it is moved to put that one at 2^10, up or down (at 2^15 where others of the page lie 10 below it), for the lower piece
+// reference that weights are scaled by: the first page's largest weight is 2^10 exactly (a row that sees one position is that
+// position's values exactly), and where that of a page leaves 2^6 .. 2^15 the reference is moved by a whole number of base-2
+// units to put that one at 2^10, up or down (at 2^15 where others of the page lie 10 below it), for the lower piece
 // ends at 2^-24, and one position that holds nearly all the weight must not take the bits of those beside and after it (that
 // costs 2 %: 64 sequences of up to 8192 103.2 -> 105.5 us; a look at every column's largest on every page, and less
 // room above, 5 %).  Warps join in shared memory, spans
@@ -321,10 +322,11 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                 }
                 // one far above the others of its own page: no room above it, for their bits; within the range or nothing seen:
                 // the reference is left where it is
-                float to = ceilf(mx) - (mx - mn > DEC_AT ? DEC_HI : DEC_AT);
+                const float at = mx - mn > DEC_AT ? DEC_HI : DEC_AT;
+                float to = m[k] == -INFINITY ? mx - at : m[k] + ceilf(mx - m[k] - at);
                 if (mx == -INFINITY || (mx - m[k] > DEC_LO && mx - m[k] <= DEC_HI)) to = m[k];
                 to = fmaxf(to, mh[k] - DEC_DOWN);
-                const float f = to == m[k] ? 1.f : kv4_two_to(m[k] - to);
+                const float f = to == m[k] ? 1.f : kv4_exp2(m[k] - to);
                 m[k] = to; mh[k] = fmaxf(mh[k], to); l[k] *= f;
 #pragma unroll
                 for (int h = 0; h < 2; h++) e[k][h] = see >> (2 * k + h) & 1 ? fmaf(s[k][h], desc[k], -to) : -INFINITY;

@@ -10,8 +10,8 @@
 // query value, 2^-39 of its largest weight on the page; the dropped lo * lo term is 2^-22 of a product.  Steps of 4096 and more would overflow
 // f16: a page that has one is brought down by 2^4.  O starts from zero at every page and is added to f32 registers, because
 // the tensor core's own sum drifts over a long prompt.
-//   warps 0-3, 4-7   softmax of a tile, a thread a line: S from TMEM, running maximum (a whole number of base-2 units,
-//               moved when passed by 8), weights back to TMEM over the scores as the A operand of the second product, then
+//   warps 0-3, 4-7   softmax of a tile, a thread a line: S from TMEM, running maximum (moved when passed by 8 in base-2
+//               units), weights back to TMEM over the scores as the A operand of the second product, then
 //               the O of the page before added to the registers
 //   warps 8-11, 12-14   keys and values of a page: bulk copies of codes and steps into shared memory (two pages deep), then k
 //               and v^T operand tiles (K-major, 128-byte swizzle): eight key dims of a position, or eight positions of a
@@ -477,11 +477,10 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                         for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(v[i], v[i + 1]));
                     }
                     mx *= ds;                                    // (the scale is positive)
-                    const float mc = ceilf(mx);
-                    const bool up = mc > m + 8.f;
+                    const bool up = mx > m + 8.f;
                     f = 1.f;
                     if (__any_sync(0xffffffffu, up)) {
-                        if (up) { f = kv4_two_to(m - mc); m = mc; }
+                        if (up) { f = kv4_exp2(m - mx); m = mx; }
                         __syncwarp();
                         l *= f;
 #pragma unroll
@@ -489,8 +488,9 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                     }
                     // weights as hi and lo pairs of consecutive positions, over the scores: 16 columns become 8 of hi and 8 of
                     // lo.  They are brought up to 2^15 by the largest of the line on THIS page (lo ends at 2^-24, which
-                    // then is 2^-39 of it), not by the largest so far, which one position may hold; bn takes it back.
-                    const float mm = mx == -INFINITY ? 0.f : mc - 15.f, bn = mx == -INFINITY ? 0.f : kv4_two_to(mm - m);
+                    // then is 2^-39 of it), not by the largest so far, which one position may hold; bn takes it back.  Both are
+                    // a whole number of base-2 units apart: a line that sees one position is that position's values exactly.
+                    const float mm = mx == -INFINITY ? 0.f : m + ceilf(mx - m) - 15.f, bn = mx == -INFINITY ? 0.f : kv4_exp2(mm - m);
                     float s0 = 0.f, s1 = 0.f;
 #pragma unroll 1
                     for (int q = 0; q < 4; q++) {

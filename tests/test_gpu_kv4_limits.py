@@ -101,3 +101,26 @@ def test_attend_prompts_with_long_sums_of_one_sign(gpu, t, H, KV, nseq, rows, hd
         w = np.exp(s[:T - rows + r + 1] - 0.25)
         want = w @ v[:T - rows + r + 1, h // (H // KV)] / w.sum()
         assert np.abs(got[i, r, h] / want - 1).max() <= E * (2 * (8 + 64 + T / 1024) + 6 * 0.25 + 54)
+
+
+@pytest.mark.parametrize("H,rows,hd", [(8, 1, 32), (8, 1, 96), (64, 1, 128), (16, 1, 256), (32, 20, 32), (32, 20, 64), (32, 20, 128), (32, 20, 256)])
+def test_attend_of_one_position_is_its_values(gpu, t, H, rows, hd):
+    """A row that sees a single position is that position's value row, to the bit: the first positions of sequences, and rows
+    with a window of one.  (Activations are quantised after this: values of few bits lie on ties there.)  Scores are exact in
+    the kernels' base-2 units: eighths, scaled by what is 1 after log2(e)."""
+    T, log2e = 150, np.float32(1.44269504)
+    scale = np.float32(1) / log2e
+    assert np.float32(scale * log2e) == 1
+    p = Pool(gpu, t, KV, hd, [T], seed=hd + rows)
+    p.k[0][:] = 0; p.k[0][:, :, 0] = p.rng.integers(-40, 41, (T, 1)) / 8
+    p.store()
+    q = np.zeros((NSEQ * rows, H, hd), np.float32); q[:, :, 0] = 1
+    v = quant(p.v[0])[0].astype(np.float32)
+    G = H // KV
+    got = p.attend(q, H, [rows] * NSEQ, scale=float(scale), window=1, lens=[T] * NSEQ, table=np.repeat(p.table, NSEQ, 0), max_len=T).reshape(NSEQ, rows, H, hd)
+    want = np.repeat(v[T - rows:], G, 1)
+    assert np.array_equal(got, np.broadcast_to(want, got.shape))
+    # the first `rows` positions of a sequence: its row 0 sees position 0 alone
+    got = p.attend(q, H, [rows] * NSEQ, scale=float(scale), lens=[rows] * NSEQ, table=np.repeat(p.table, NSEQ, 0), max_len=p.ld * 64).reshape(NSEQ, rows, H, hd)
+    assert np.array_equal(got[:, 0], np.broadcast_to(np.repeat(v[0], G, 0), got[:, 0].shape))
+    p.status()
