@@ -133,8 +133,6 @@ __device__ __forceinline__ void kv4_scaled_pieces(unsigned yh, unsigned yl, unsi
 // 2^k for -126 <= k <= 127, and x 2^k for any k of the f32 range (two factors, each a normal number)
 __device__ __forceinline__ float kv4_pow2(int k) { return __int_as_float((k + 127) << 23); }
 __device__ __forceinline__ float kv4_scale2(float x, int k) { const int h = k >> 1; return x * kv4_pow2(h) * kv4_pow2(k - h); }
-// 2^d for a whole number d, 0 where that is no normal number (or d is NaN)
-__device__ __forceinline__ float kv4_two_to(float d) { return d >= -126.f ? kv4_pow2((int)fminf(d, 127.f)) : 0.f; }
 // the power of two that brings a query row whose largest magnitude has the bits mb below 2^14 (0 for a row of zeros)
 __device__ __forceinline__ int kv4_q_shift(unsigned mb) { return mb ? 13 + 127 - (int)(mb >> 23 ? mb >> 23 : 1) : 0; }
 __device__ __forceinline__ float kv4_exp2(float x) {

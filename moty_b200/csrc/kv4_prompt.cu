@@ -7,8 +7,9 @@
 //     scores [16 lines x 8 positions] += (q hi + q lo) [16 x 32 dims of a group] * codes, then times the positions' steps
 //     output [16 lines x 8 dims]      += (x hi + x lo) [16 x 16 positions] * codes,   x = weight * step of the dims' group
 // The score fragment of two 8-position tiles is the weight fragment of the second product, so weights never leave the
-// thread.  Query pieces stay in shared memory in fragment order.  Running maximum (moved in steps of at least 8 in base-2
-// units) and the exponent of the largest value step as in the decode kernel.
+// thread.  Query pieces stay in shared memory in fragment order.  The weights' reference is moved up and down as in the decode
+// kernel, so that a line's largest weight of a pass (8 PT positions) lies between 2^-6 and 2^5; x, scaled by the exponent of the
+// largest value step so far and 2^9, then lies below 2^15, and its pieces end at 2^-28 of those two's product at worst.
 // It serves the head widths that the tensor-memory kernel has no operand tiles for, and calls too short for that kernel's
 // set-up.  What bounds it: two pieces make two matrix instructions of half the rate a product, and turning codes into
 // operands is done by every warp for itself; 4096 rows at 4096 positions, 16 heads on 8, hd 128: 573 us (tensor memory:
@@ -19,6 +20,9 @@
 namespace {
 
 constexpr int PR_W = KV4_LINES / 16, PR_F = 16;              // warps a CTA; pages of a lower sum
+// exponents of a line's largest weight of a pass: the range it may have (PR_LOW: where every lane has one as large), where it is
+// put, and how far below the highest reference so far one may be
+constexpr float PR_HI = 5.f, PR_LO = -4.f, PR_LOW = -6.f, PR_AT = 0.f, PR_DOWN = 60.f;
 
 template <int NG> struct PrL {
     static constexpr int HD = NG * 32, UNIT = 72 * HD, PT = NG <= 4 ? 4 : 2;
@@ -26,7 +30,7 @@ template <int NG> struct PrL {
 };
 
 template <int NG>
-__global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
+__global__ void __launch_bounds__(PR_W * 32, NG == 1 ? 4 : 2) kv4_prompt_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
     constexpr int HD = NG * 32, UNIT = PrL<NG>::UNIT, PT = PrL<NG>::PT, NL = 16 * PR_W;
     extern __shared__ __align__(128) uint8_t sm_kv4p[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, j = lane & 3;
@@ -103,7 +107,7 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
         }
     }
     __syncwarp();
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[NG][4][4];
+    float m[2] = {-INFINITY, -INFINITY}, mh[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[NG][4][4];    // m: the reference, mh: the highest so far
 #pragma unroll
     for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -112,7 +116,7 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
     // memory), which keep the maximum and the scale that they were left with.  One level alone: 131072 flat weights 1e-4 off.
     volatile float lt[2] = {0.f, 0.f}, mt[2] = {-INFINITY, -INFINITY}, vnt = 0.f, tot[NG * 16];
     int passes = 0;                                          // (tot holds nothing before PR_F pages of them)
-    float vth = 0.f, vn = 0.f;                               // 2^(e + 1) and 64 * 2^-e for the exponent e of the largest value step so far
+    float vth = 0.f, vn = 0.f;                               // 2^(e + 1) and 2^9 * 2^-e for the exponent e of the largest value step so far
     const int *tab = a.b.table + (size_t)seq * a.b.ld;
     const uint8_t *base = a.mem + (size_t)(a.layer * a.geo.KV + head) * UNIT;
     const size_t page_bytes = kv4_page_bytes(a.geo);
@@ -185,7 +189,6 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
             }
             const bool inside = tb >= wr.lo_all && tb + 8 * PT <= wr.hi_all;
             unsigned see = 0xffffffffu;                      // bit 4 nt + i: that score is seen
-            bool up = false;
 #pragma unroll
             for (int nt = 0; nt < PT; nt++)
 #pragma unroll
@@ -195,19 +198,49 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
                         const int t = tb + nt * 8 + 2 * j + (i & 1);
                         if (t < clo[i >> 1] || t > chi[i >> 1]) { s[nt][i] = -INFINITY; see &= ~(1u << (4 * nt + i)); }
                     }
-                    up |= s[nt][i] > m[i >> 1] + 8.f;
                 }
-            if (__any_sync(0xffffffffu, up)) {
+            bool odd = false;                                // a cheap look first: each lane's largest weight within the range
+            float top[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                top[h] = -INFINITY;
+#pragma unroll
+                for (int nt = 0; nt < PT; nt++) top[h] = fmaxf(top[h], fmaxf(s[nt][2 * h], s[nt][2 * h + 1]));
+                top[h] -= m[h];
+                odd |= !(top[h] > PR_LOW && top[h] <= PR_HI);
+            }
+            bool move = __any_sync(0xffffffffu, odd);
+            if (move) {
+                move = false;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {                // (a line is a quad; its largest decides)
+                    const unsigned large = __ballot_sync(0xffffffffu, top[h] > PR_LO) & 0xfu << 4 * r;
+                    move |= top[h] > PR_HI;
+                    move |= !large && m[h] > mh[h] - PR_DOWN;
+                }
+                move = __any_sync(0xffffffffu, move);
+            }
+            if (move) {
                 float f[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    float mx = m[h];
+                    float mx = -INFINITY, mn = INFINITY;
 #pragma unroll
-                    for (int nt = 0; nt < PT; nt++) mx = fmaxf(mx, fmaxf(s[nt][2 * h], s[nt][2 * h + 1]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    f[h] = mx == -INFINITY ? 1.f : kv4_exp2(m[h] - mx);
-                    m[h] = mx; l[h] *= f[h];
+                    for (int i = 0; i < 2 * PT; i++)
+                        if (see >> (4 * (i >> 1) + 2 * h + (i & 1)) & 1) { mx = fmaxf(mx, s[i >> 1][2 * h + (i & 1)]); mn = fminf(mn, s[i >> 1][2 * h + (i & 1)]); }
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) {
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+                    }
+                    // one far above the others of its own pass: no room above it, for their bits; within the range or nothing
+                    // seen: the reference is left where it is
+                    const float at = mx - mn > 10.f ? PR_HI : PR_AT;
+                    float to = m[h] == -INFINITY ? mx - at : m[h] + ceilf(mx - m[h] - at);
+                    if (mx == -INFINITY || (mx - m[h] > PR_LO && mx - m[h] <= PR_HI)) to = m[h];
+                    to = fmaxf(to, mh[h] - PR_DOWN);
+                    f[h] = to == m[h] ? 1.f : kv4_exp2(m[h] - to);
+                    m[h] = to; mh[h] = fmaxf(mh[h], to); l[h] *= f[h];
                 }
 #pragma unroll
                 for (int g = 0; g < NG; g++)
@@ -252,7 +285,7 @@ __global__ void __launch_bounds__(PR_W * 32) kv4_prompt_kernel(Kv4Attend a, int 
             if (__any_sync(0xffffffffu, big >= vth)) {
                 const unsigned bb = __reduce_max_sync(0xffffffffu, __float_as_uint(big)) & 0x7f800000u;   // 2^e
                 if (bb) {
-                    const float nn = 64.f / __uint_as_float(bb), f = vn == 0.f ? 1.f : nn / vn;
+                    const float nn = 512.f / __uint_as_float(bb), f = vn == 0.f ? 1.f : nn / vn;
                     vth = 2.f * __uint_as_float(bb); vn = nn;
 #pragma unroll
                     for (int g = 0; g < NG; g++)

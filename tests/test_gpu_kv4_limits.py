@@ -30,9 +30,10 @@ def t():
     return torch
 
 
-# (query heads, rows a sequence, head width): decode of four and of eight columns, the prompt kernel of tensor memory.  40
-# sequences of 8 KV heads share one table: a CTA walks many pages.
-KERNELS = [(8, 1, 32), (8, 1, 128), (8, 1, 256), (64, 1, 64), (64, 1, 128), (16, 4, 224), (32, 20, 64), (32, 20, 96), (32, 20, 128)]
+# (query heads, rows a sequence, head width): decode of four and of eight columns, the prompt kernels of matrix instructions
+# (32, 160, 256) and of tensor memory (64 to 128).  40 sequences of 8 KV heads share one table: a CTA walks many pages.
+KERNELS = [(8, 1, 32), (8, 1, 128), (8, 1, 256), (64, 1, 64), (64, 1, 128), (16, 4, 224), (32, 20, 32), (32, 20, 160), (32, 20, 256),
+           (32, 20, 64), (32, 20, 96), (32, 20, 128)]
 NSEQ, KV = 40, 8
 
 
