@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
         if (x < nx) {
             // ---- softmax: a thread a line ----
             const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            float m = -INFINITY, l = 0.f, o[HD];
+            float m = -INFINITY, l = 0.f, lt = 0.f, o[HD];       // lt: the weights' total of whole 16 pages, l: of those after them
             unsigned nanbits = 0;
 #pragma unroll
             for (int i = 0; i < HD; i++) o[i] = 0.f;
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                     if (__any_sync(0xffffffffu, up)) {
                         if (up) { f = kv4_exp2(m - mx); m = mx; }
                         __syncwarp();
-                        l *= f;
+                        l *= f; lt *= f;
 #pragma unroll
                         for (int i = 0; i < HD; i++) o[i] *= f;
                     }
@@ -511,6 +511,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                         tm_st8(at + q * 16 + 8, pl);
                     }
                     l = fmaf(s0 + s1, bn, l);
+                    if ((j & 15) == 15) { lt += l; l = 0.f; }    // (one sum of 512 even pages: 3e-6 off)
                     b = bn;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_before();
@@ -545,6 +546,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
             // out through the tile's query rows (their products are done), so that a warp writes whole lines: a thread puts its
             // line there in pieces of four dims, turned by the line so that eight lanes meet eight bank groups
             if (__all_sync(0xffffffffu, ok)) {
+                l += lt;
                 float4 *box = reinterpret_cast<float4 *>(sm + 2 * x * L::Q) + (warp & 3) * (32 * HD / 4);
                 if (tid < ncol && nsplit > 1) *reinterpret_cast<float2 *>(part + (rh * nsplit + split) * (HD + 4)) = make_float2(m, l);
                 const float over = nsplit > 1 ? 1.f : kv4_over(l);

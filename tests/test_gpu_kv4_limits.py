@@ -125,3 +125,20 @@ def test_attend_of_one_position_is_its_values(gpu, t, H, rows, hd):
     got = p.attend(q, H, [rows] * NSEQ, scale=float(scale), lens=[rows] * NSEQ, table=np.repeat(p.table, NSEQ, 0), max_len=p.ld * 64).reshape(NSEQ, rows, H, hd)
     assert np.array_equal(got[:, 0], np.broadcast_to(np.repeat(v[0], G, 0), got[:, 0].shape))
     p.status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attend_prompts_weights_total_over_a_long_span(gpu, t, hd):
+    """The tensor-memory kernel's span of 512 pages, weights that hardly differ, values that are all the same: the result is the
+    value.  The weights' total is summed over 32 positions, 16 pages and 32 such parts; additions to a sum err by e at most, all
+    the same way where the sum grows evenly, by half of that on the average and of half the final sum:  (32 + 16 + 32) e / 4.
+    The 512 pages' outputs round at random, 0.58 e sqrt(512 / 3), and 12 products' sums are cut off by e / 2 on the average."""
+    T, rows, nseq, H, KV = 32700, 20, 80, 8, 2
+    p = Pool(gpu, t, KV, hd, [T], seed=hd)
+    p.k[0][:] = 0; p.k[0][:, :, 0] = p.rng.integers(0, 3, (T, 1)) / 1024
+    p.v[0][:] = 1.3
+    p.store()
+    q = np.zeros((nseq * rows, H, hd), np.float32); q[:, :, 0] = 1
+    got = p.attend(q, H, [rows] * nseq, scale=1.0, lens=[T] * nseq, table=np.repeat(p.table, nseq, 0)).astype(np.float64)
+    p.status()
+    assert abs(np.mean(got / quant(p.v[0])[0][0, 0, 0]) - 1) <= E * (20 + 0.58 * math.sqrt(512 / 3) + 6)
