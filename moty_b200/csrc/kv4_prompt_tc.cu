@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
     }
     // a softmax thread's line: its query row, limits, scale; the row goes to shared memory in two pieces
     float desc = 0.f;
+    bool fin = true;                                         // a row that is not finite scores 0, and is NaN in the end where it saw anything
     int clo = 0, chi = 0x7fffffff;                           // (lines that are not there see everything, and are not written)
     size_t rh = 0;
     const int x = warp >> 2;                                 // the tile of a softmax warp
@@ -274,9 +275,9 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                 *reinterpret_cast<uint4 *>(dst + L::Q) = make_uint4(l[0], l[1], l[2], l[3]);
             }
         }
-        const bool fin = mb < 0x7f800000u;
+        fin = mb < 0x7f800000u;
         // (not below the smallest normal number: -infinity times it has to stay -infinity)
-        desc = fin ? fmaxf(kv4_scale2(a.scale * 1.44269504f, -kv4_q_shift(mb)), 1.17549435e-38f) : __int_as_float(0x7fffffff);
+        desc = fin ? fmaxf(kv4_scale2(a.scale * 1.44269504f, -kv4_q_shift(mb)), 1.17549435e-38f) : 1.f;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     tc_before();
@@ -547,6 +548,7 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
             // line there in pieces of four dims, turned by the line so that eight lanes meet eight bank groups
             if (__all_sync(0xffffffffu, ok)) {
                 l += lt;
+                if (!fin && l != 0.f) l = __int_as_float(0x7fffffff);
                 float4 *box = reinterpret_cast<float4 *>(sm + 2 * x * L::Q) + (warp & 3) * (32 * HD / 4);
                 if (tid < ncol && nsplit > 1) *reinterpret_cast<float2 *>(part + (rh * nsplit + split) * (HD + 4)) = make_float2(m, l);
                 const float over = nsplit > 1 ? 1.f : kv4_over(l);

@@ -142,3 +142,40 @@ def test_attend_prompts_weights_total_over_a_long_span(gpu, t, hd):
     got = p.attend(q, H, [rows] * nseq, scale=1.0, lens=[T] * nseq, table=np.repeat(p.table, nseq, 0)).astype(np.float64)
     p.status()
     assert abs(np.mean(got / quant(p.v[0])[0][0, 0, 0]) - 1) <= E * (20 + 0.58 * math.sqrt(512 / 3) + 6)
+
+
+# windows that leave rows with one page, with a page's end inside, with all; absent pages in front of, inside and behind them.  Key
+# values of sequences' own tables differ by where pages are missing only.
+@pytest.mark.parametrize("H,hd", [(32, 64), (32, 96), (32, 128), (32, 32), (32, 256)])
+@pytest.mark.parametrize("window", [0, 1, 30, 64, 100, 700])
+def test_attend_prompts_windows_absent_pages_and_rows_that_are_not_finite(gpu, t, H, hd, window):
+    """Prompt kernels (tensor memory at 64 to 128): every mask at once, against the 64-bit form; a query row with an infinity or a
+    NaN is NaN where it sees anything and 0 where it sees nothing, and changes no other row."""
+    T, rows, G = 420, 40, H // KV
+    p = Pool(gpu, t, KV, hd, [T], seed=hd + window, scale=2.0, extra_ld=3)
+    table = np.repeat(p.table, NSEQ, 0)
+    absent = {s: [] for s in range(NSEQ)}
+    absent[1] = [6]; absent[2] = [5, 6]; absent[3] = [0, 3, 4]; absent[4] = list(range(7)); absent[5] = [1, 2, 5]
+    for s, gone in absent.items():
+        table[s, gone] = -1
+    q = p.rng.standard_normal((NSEQ, rows, H, hd)).astype(np.float32)
+    for s in range(6):
+        q[s, 3, 5, 1] = np.nan; q[s, 17, 0, hd - 1] = np.inf; q[s, rows - 1, H - 1, 0] = -np.inf; q[s, 25, 9] = np.nan
+    got = p.attend(q, H, [rows] * NSEQ, window=window, lens=[T] * NSEQ, table=table).reshape(NSEQ, rows, H, hd)
+    p.status()
+    k, v = quant(p.k[0])[0], quant(p.v[0])[0]
+    for s in (0, 1, 2, 3, 4, 5, NSEQ - 1):
+        hidden = np.isin(np.arange(T) // 64, absent[s])
+        for r in (0, 3, 4, 17, 25, 35, 36, rows - 1):
+            pos = T - rows + r
+            for h in {0, 5, 9, H - 1}:
+                g = h // G
+                lo = max(0, pos - window + 1) if window else 0
+                fin = np.isfinite(q[s, r, h]).all()
+                if hidden[lo:pos + 1].all():
+                    assert (got[s, r, h] == 0).all()
+                elif not fin:
+                    assert np.isnan(got[s, r, h]).all()
+                else:
+                    want, tol = attend64(k[:, g:g + 1], v[:, g:g + 1], q[s, r:r + 1, h:h + 1], [pos], 1, window, hidden=hidden)
+                    check(got[s, r:r + 1, h:h + 1], want, tol)
