@@ -551,7 +551,7 @@ __device__ __forceinline__ Kv4Join kv4_join_row(const Kv4Attend &a, int row) {
     int seq, pos;
     const int st = kv4_row<32>(a.b, row, &seq, &pos);
     Kv4Join r{-1, 0, 0};
-    if (st == KV4_ROW_NONE) return r;
+    if (st == KV4_ROW_NONE || st == KV4_ROW_STRAY) return r;
     r.r0 = 0;
     if (st == KV4_ROW_BAD) return r;
     const int r0 = a.b.row0[seq], n = a.b.row0[seq + 1] - r0, len = a.b.len[seq];

@@ -53,7 +53,8 @@ struct Kv4Batch {
     int nseq, rows, ld;
     const int *row0, *len, *table;       // [nseq + 1], [nseq], [nseq][ld]
 };
-enum { KV4_ROW_NONE = 0, KV4_ROW_OK = 1, KV4_ROW_BAD = 2 };
+// KV4_ROW_STRAY: a row that no sequence has, found beside arrays that do not describe one.
+enum { KV4_ROW_NONE = 0, KV4_ROW_OK = 1, KV4_ROW_BAD = 2, KV4_ROW_STRAY = 3 };
 // The row range, first position and length of sequence s.  KV4_ROW_NONE: it has no rows.  KV4_ROW_BAD: the device arrays
 // do not describe one (rows outside the buffers, more rows than positions, positions past the table).
 KV4_HD int kv4_seq(const Kv4Batch &b, int s, int *r0, int *n, int *len) {
@@ -76,12 +77,13 @@ template <int W, class Count> KV4_HD int kv4_find_seq(int nseq, Count count) {
     }
     return lo;
 }
-// The position of row r if it belongs to sequence s.  KV4_ROW_NONE: it does not.
+// The position of row r if it belongs to sequence s.  KV4_ROW_NONE: it does not.  KV4_ROW_BAD: it is a row of a sequence that
+// is refused.  KV4_ROW_STRAY: it lies outside such a one's rows, and is nobody's.
 KV4_HD int kv4_row_in(const Kv4Batch &b, int s, int r, int *pos) {
     int r0, n, len;
     const int st = kv4_seq(b, s, &r0, &n, &len);
     *pos = 0;
-    if (st == KV4_ROW_BAD) return KV4_ROW_BAD;
+    if (st == KV4_ROW_BAD) return b.row0[s] <= r && r < b.row0[s + 1] ? KV4_ROW_BAD : KV4_ROW_STRAY;
     if (st == KV4_ROW_NONE || r < r0 || r >= r0 + n) return KV4_ROW_NONE;
     *pos = len - n + (r - r0);
     return KV4_ROW_OK;

@@ -125,13 +125,13 @@ __device__ __forceinline__ void kv4_rows(Kv4Rows &s, const Kv4Geom &geo, uint8_t
         uint8_t *unit = nullptr;
         if (r >= b.rows) { seq = -1; pos = 0; }
         else {
-            if (st == KV4_ROW_BAD) atomicExch(err, 1);
+            if (st == KV4_ROW_BAD || st == KV4_ROW_STRAY) atomicExch(err, 1);
             if (st == KV4_ROW_OK) {
                 const int page = b.table[(size_t)seq * b.ld + pos / KV4_PAGE];
                 if (kv4_page_ok(geo, page)) unit = mem + kv4_unit_off(geo, page, layer, head);
                 else if (!(absent_ok && page == -1)) atomicExch(err, 1);
             }
-            if (st == KV4_ROW_NONE) seq = -1;
+            else seq = -1;                                     // (nothing is stored or fetched for it)
         }
         s.unit[i] = unit; s.t[i] = pos % KV4_PAGE; s.seq[i] = seq;
     }
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256) kv4_append_rope_kernel(Kv4Geom geo, uint8
     const int hh = isq ? slot : slot - H;
     int seq, pos;
     const int st = kv4_row<32>(b, r, &seq, &pos);
-    if (st != KV4_ROW_OK) { if (st == KV4_ROW_BAD && i == 0) atomicExch(err, 1); return; }       // (the whole CTA)
+    if (st != KV4_ROW_OK) { if (st != KV4_ROW_NONE && i == 0) atomicExch(err, 1); return; }      // (the whole CTA)
     float *row = (isq ? q + (size_t)r * q_ld : k + (size_t)r * ld) + (size_t)hh * hd;
     const float *nw = isq ? a.qn : a.kn;
     float x = row[i];

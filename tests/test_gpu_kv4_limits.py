@@ -179,3 +179,28 @@ def test_attend_prompts_windows_absent_pages_and_rows_that_are_not_finite(gpu, t
                 else:
                     want, tol = attend64(k[:, g:g + 1], v[:, g:g + 1], q[s, r:r + 1, h:h + 1], [pos], 1, window, hidden=hidden)
                     check(got[s, r:r + 1, h:h + 1], want, tol)
+
+
+@pytest.mark.parametrize("rows,lens", [(1, [300, 200]), (40, [300, 200]), (40, [2000, 1900]), (2, [9000, 5000])])
+@pytest.mark.parametrize("what", ["len_past_table", "rows_more_than_len"])
+def test_rows_behind_a_refused_sequence_stay(gpu, t, rows, lens, what):
+    """The last sequence is refused: its rows become 0 (attend) or stay (fetch), the rows behind it stay, the first sequence's
+    come out as always -- in one launch and with spans joined in a second."""
+    H, hd, pad = 4, 64, 5
+    p = Pool(gpu, t, 2, hd, lens, seed=rows)
+    q = p.rng.standard_normal((2 * rows + pad, H, hd)).astype(np.float32)
+    good = p.attend(q[:2 * rows], H, [rows, rows])
+    bad = [lens[0], 64 * p.ld + 1 if what == "len_past_table" else rows - 1]
+    got = p.attend(q, H, [rows, rows], pad=pad, lens=bad, max_len=max(lens))
+    with pytest.raises(gpu.MotyCudaError, match="4-bit KV"):
+        p.status()
+    assert got[:rows].tobytes() == good[:rows].tobytes() and (got[rows:2 * rows] == 0).all() and (got[2 * rows:] == 7).all()
+    b = p.batch([rows, rows], lens=bad, pad=pad, max_len=max(lens))
+    k = t.full((2 * rows + pad, 2 * hd), 5.0, device="cuda"); v = k.clone()
+    p.kv.fetch_dev(0, k.data_ptr(), v.data_ptr(), b, stream=p.sh())
+    t.cuda.synchronize()
+    with pytest.raises(gpu.MotyCudaError, match="4-bit KV"):
+        p.status()
+    for x, held in ((k, p.k[0]), (v, p.v[0])):
+        assert (x[rows:] == 5).all()
+        assert np.array_equal(x[:rows].cpu().numpy().reshape(rows, 2, hd), quant(held[lens[0] - rows:])[0].astype(np.float32))

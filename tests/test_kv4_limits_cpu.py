@@ -1,6 +1,8 @@
 """CPU: what the paged 4-bit KV cache's kernels rely on that no result shows, and its decoder's books when a step fails."""
+import ctypes as C
 import os
 import re
+import subprocess
 
 import pytest
 
@@ -22,3 +24,22 @@ def test_roles_take_their_registers_in_their_own_branch():
         assert low % 4 == 0 and (more == "true") == (value(regs) > value("PT_REGS"))
         total += (edge - low) * 32 * value(regs); edge = low
     assert edge == 0 and total <= value("PT_T") * value("PT_REGS") <= 65536
+
+
+def test_rows_behind_a_refused_sequence_are_nobodys(tmp_path):
+    """Rows behind the last sequence belong to none, also where that sequence is refused (a length past its table): only its own
+    rows count as refused."""
+    src, so = str(tmp_path / "r.cpp"), str(tmp_path / "r.so")
+    with open(src, "w") as f:
+        f.write('#include "kv4_index.h"\nextern "C" int row(int nseq, int rows, int ld, const int *row0, const int *len, int r) {\n'
+                "    Kv4Batch b{nseq, rows, ld, row0, len, nullptr}; int s, p; return kv4_row(b, r, &s, &p); }\n")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", CSRC, src, "-o", so], check=True)
+    lib = C.CDLL(so)
+    arr = lambda a: (C.c_int * len(a))(*a)
+    none, ok, bad, stray = 0, 1, 2, 3
+    look = lambda row0, lens, rows, ld=2: [lib.row(len(lens), rows, ld, arr(row0), arr(lens), r) for r in range(rows)]
+    assert look([0, 2, 5], [9, 9], 8) == [ok] * 5 + [none] * 3
+    assert look([0, 2, 5], [9, 129], 8) == [ok] * 2 + [bad] * 3 + [stray] * 3
+    assert look([0, 2, 5], [129, 9], 8) == [bad] * 2 + [ok] * 3 + [none] * 3
+    assert look([1, 3, 2], [9, 9], 5) == [none, ok, ok, stray, stray]              # the second ends before it begins
+    assert look([0, 9], [20], 5) == [bad] * 5                                      # ends behind the buffers
