@@ -516,7 +516,7 @@ int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_dev, const f
  * fork's source or target, a fresh page given twice, or an index out of range is skipped and reported by kernel_status.
  * compact: pages src[i] -> dst[i] for all layers, and out[j] = the new id of table[j] for count entries (ids not in src and
  * -1 stay; out may be table).  src and dst strictly ascending and without a common id, as compact_plan gives them; moves
- * that break this are skipped and reported. */
+ * that break this are skipped and reported, and entries that name their pages keep the ids. */
 int moty_cuda_kv4_fork_dev(MotyCudaKv4 *kv, int n, const int *src_dev, const int *dst_dev, const int *fresh_dev, int nseq, int *len_dev,
                            int *table_dev, int table_ld, void *stream);
 int moty_cuda_kv4_compact_dev(MotyCudaKv4 *kv, int n, const int *src_dev, const int *dst_dev, int64_t count, const int *table_dev, int *out_dev,

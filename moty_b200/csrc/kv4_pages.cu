@@ -60,9 +60,16 @@ __device__ __forceinline__ int kv4_find_id(const int *list, int n, int id) {
     return -1;
 }
 
+// Whether move i may be made: ids in the pool, its place in both lists, and a target that is no source.
+__device__ __forceinline__ bool kv4_move_ok(const Kv4Geom &geo, const int *src, const int *dst, int n, int i) {
+    const int s = src[i], d = dst[i];
+    return kv4_page_ok(geo, s) && kv4_page_ok(geo, d) && (i == 0 || (src[i - 1] < s && dst[i - 1] < d)) && kv4_find_id(src, n, d) < 0;
+}
+
 // CTAs 0 .. n * nchunk - 1 copy pages src[i] -> dst[i]; the others rename the table's entries.  Both lists must be
 // strictly ascending and share no id, which makes every copy's target distinct from every page that is read; each CTA
-// checks what it relies on (its neighbours in the lists, its target against the sources).
+// checks what it relies on (its neighbours in the lists, its target against the sources).  An entry keeps its id where the
+// move is refused.
 __global__ void __launch_bounds__(PG_THREADS) kv4_compact_kernel(Kv4Geom geo, uint8_t *mem, int n, const int *src, const int *dst, int nchunk,
                                                                  long long count, const int *table, int *out, int *err) {
     const int tid = threadIdx.x;
@@ -70,17 +77,17 @@ __global__ void __launch_bounds__(PG_THREADS) kv4_compact_kernel(Kv4Geom geo, ui
     pdl_wait();
     const long long ncopy = (long long)n * nchunk;
     if (blockIdx.x < ncopy) {
-        const int i = blockIdx.x / nchunk, chunk = blockIdx.x - i * nchunk, s = src[i], d = dst[i];
-        if (!kv4_page_ok(geo, s) || !kv4_page_ok(geo, d) || (i > 0 && (src[i - 1] >= s || dst[i - 1] >= d)) || kv4_find_id(src, n, d) >= 0) {
+        const int i = blockIdx.x / nchunk, chunk = blockIdx.x - i * nchunk;
+        if (!kv4_move_ok(geo, src, dst, n, i)) {
             if (tid == 0) atomicExch(err, 1);
             return;
         }
-        kv4_copy_chunk(mem, kv4_page_bytes(geo), s, d, chunk, nchunk);
+        kv4_copy_chunk(mem, kv4_page_bytes(geo), src[i], dst[i], chunk, nchunk);
         return;
     }
     for (long long i = (blockIdx.x - ncopy) * PG_THREADS + tid; i < count; i += (gridDim.x - ncopy) * PG_THREADS) {
         const int id = table[i], at = id < 0 ? -1 : kv4_find_id(src, n, id);
-        out[i] = at < 0 ? id : dst[at];
+        out[i] = at >= 0 && kv4_move_ok(geo, src, dst, n, at) ? dst[at] : id;
     }
 }
 

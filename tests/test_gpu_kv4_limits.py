@@ -204,3 +204,27 @@ def test_rows_behind_a_refused_sequence_stay(gpu, t, rows, lens, what):
     for x, held in ((k, p.k[0]), (v, p.v[0])):
         assert (x[rows:] == 5).all()
         assert np.array_equal(x[:rows].cpu().numpy().reshape(rows, 2, hd), quant(held[lens[0] - rows:])[0].astype(np.float32))
+
+
+@pytest.mark.parametrize("src,dst,made", [([5, 4], [0, 1], {5: 0}), ([4, 5], [1, 0], {4: 1}), ([4, 5], [1, 1], {4: 1}), ([3, 5], [0, 3], {3: 0}), ([-1, 5], [0, 1], {5: 1}),
+                                          ([4, 5], [-2, 1], {5: 1}), ([4, 5], [8, 9], {}), ([4, 5], [0, 1], {4: 0, 5: 1})])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_move_that_is_refused_renames_nothing(gpu, t, src, dst, made, in_place):
+    """Entries follow the pages that were copied, and no others: lists out of order, that meet, or that leave the pool."""
+    layers, heads, hd, pages = 2, 1, 64, 8
+    g = t.Generator(device="cuda").manual_seed(5)
+    mem = t.randint(0, 256, (pages, gpu.Kv4.page_bytes(layers, heads, hd)), generator=g, device="cuda", dtype=t.uint8)
+    before = mem.cpu().numpy()
+    kv = gpu.Kv4(layers, heads, hd, pages, mem_ptr=mem.data_ptr())
+    d = lambda a: t.tensor(a, device="cuda", dtype=t.int32)
+    S, D, T = d(src), d(dst), d([-1, 4, 5, 3, 0, 7, 5, 4, -1])
+    want = [made.get(int(x), int(x)) for x in T.cpu()]
+    out = T if in_place else t.full_like(T, 99)
+    sh = gpu.stream_handle(t.cuda.current_stream())
+    kv.compact_dev(2, S.data_ptr(), D.data_ptr(), T.numel(), T.data_ptr(), out.data_ptr(), stream=sh)
+    t.cuda.synchronize()
+    assert gpu.lib().moty_cuda_kernel_status(0, sh) == (0 if len(made) == 2 else -6)
+    assert out.cpu().tolist() == want
+    after = mem.cpu().numpy()
+    for a, b in made.items():
+        assert np.array_equal(after[b], before[a])
