@@ -513,7 +513,8 @@ int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_dev, const f
 /* fork: sequence dst[f] of the table [nseq][table_ld] and len [nseq] becomes a copy of sequence src[f], f = 0 .. n - 1: ids of full
  * pages are shared (the caller retains them), a partial last page is copied, all layers, to page fresh[f] (from alloc; -1
  * where len[src] is a multiple of 64); the rest of the row becomes -1.  A source may repeat; a target that is another
- * fork's source or target, a fresh page given twice, or an index out of range is skipped and reported by kernel_status.
+ * fork's source or target, a fresh page given twice or that is the partial last page of a source of the call, or an index out of
+ * range is skipped and reported by kernel_status.
  * compact: pages src[i] -> dst[i] for all layers, and out[j] = the new id of table[j] for count entries (ids not in src and
  * -1 stay; out may be table).  src and dst strictly ascending and without a common id, as compact_plan gives them; moves
  * that break this are skipped and reported, and entries that name their pages keep the ids. */

@@ -28,16 +28,21 @@ __global__ void __launch_bounds__(PG_THREADS) kv4_fork_kernel(Kv4Geom geo, uint8
     pdl_trigger();
     pdl_wait();
     __syncthreads();
-    const int s = src[f], d = dst[f];
-    // a target (row or page) that another fork reads or writes too: refused, and reported
+    const int s = src[f], d = dst[f], to = fresh[f];
+    // the partial last page of a source, -1: none (no fork writes a source's row or length: a target that is one is refused)
+    auto last_page = [&](int r) {
+        const int L = r >= 0 && r < nseq ? len[r] : 0;
+        return L > 0 && L % KV4_PAGE && L / KV4_PAGE < ld ? table[(size_t)r * ld + L / KV4_PAGE] : -1;
+    };
+    const int from = last_page(s);
+    // a target (row or page) that some fork reads, or another one writes too: refused, and reported
     if (s < 0 || s >= nseq || d < 0 || d >= nseq) bad = 1;
     else
         for (int i = tid; i < n; i += PG_THREADS)
-            if (src[i] == d || (i != f && (dst[i] == d || (fresh[i] == fresh[f] && fresh[f] >= 0)))) bad = 1;
+            if (src[i] == d || (i != f && (dst[i] == d || (fresh[i] == to && to >= 0))) || (from >= 0 && to >= 0 && last_page(src[i]) == to)) bad = 1;
     __syncthreads();
     if (bad) { if (tid == 0) atomicExch(err, 1); return; }
     const int L = len[s], full = L / KV4_PAGE, tail = L % KV4_PAGE;
-    const int from = L >= 0 && tail && full < ld ? table[(size_t)s * ld + full] : -1, to = fresh[f];
     if (L < 0 || (long long)L > (long long)ld * KV4_PAGE || (tail && (!kv4_page_ok(geo, from) || !kv4_page_ok(geo, to)))) {
         if (tid == 0) atomicExch(err, 1);
         return;
@@ -46,7 +51,7 @@ __global__ void __launch_bounds__(PG_THREADS) kv4_fork_kernel(Kv4Geom geo, uint8
         for (int i = tid; i < ld; i += PG_THREADS) table[(size_t)d * ld + i] = i < full ? table[(size_t)s * ld + i] : i == full && tail ? to : -1;
         if (tid == 0) len[d] = L;
     }
-    if (tail && from != to) kv4_copy_chunk(mem, kv4_page_bytes(geo), from, to, blockIdx.y, gridDim.y);
+    if (tail) kv4_copy_chunk(mem, kv4_page_bytes(geo), from, to, blockIdx.y, gridDim.y);
 }
 
 // the index of `id` in the ascending list, or -1

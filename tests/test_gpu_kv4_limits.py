@@ -228,3 +228,34 @@ def test_a_move_that_is_refused_renames_nothing(gpu, t, src, dst, made, in_place
     after = mem.cpu().numpy()
     for a, b in made.items():
         assert np.array_equal(after[b], before[a])
+
+
+@pytest.mark.parametrize("lens,new,sound", [
+    ([70, 100], [5, 1], [0]),                    # into the page that the first fork copies from
+    ([70, 100], [3, 6], [1]),                    # into the page that the second copies from
+    ([70, 100], [1, 6], [1]), ([70, 100], [5, 3], [0]),      # into its own source's last page
+    ([70, 100], [3, 1], []),                     # each into the other's
+    ([70, 128], [5, 1], [0, 1]),                 # a source that ends with its page takes no fresh one: whatever is given is not used
+    ([70, 100], [0, 2], [0, 1]),                 # (pages in front of the last ones are not read: which pages are free is the caller's to know)
+])
+def test_forks_into_a_page_that_is_copied_are_refused(gpu, t, lens, new, sound):
+    layers, heads, hd, pages, ld = 2, 1, 64, 8, 3
+    g = t.Generator(device="cuda").manual_seed(2)
+    mem = t.randint(0, 256, (pages, gpu.Kv4.page_bytes(layers, heads, hd)), generator=g, device="cuda", dtype=t.uint8)
+    before = mem.cpu().numpy()
+    kv = gpu.Kv4(layers, heads, hd, pages, mem_ptr=mem.data_ptr())
+    table = np.full((4, ld), -1, np.int32); table[0, :2] = [0, 1]; table[1, :2] = [2, 3]
+    ln = np.array(lens + [0, 0], np.int32)
+    d = lambda a: t.tensor(a, device="cuda", dtype=t.int32)
+    S, D, N, T, L = d([0, 1]), d([2, 3]), d(new), d(table), d(ln)
+    sh = gpu.stream_handle(t.cuda.current_stream())
+    kv.fork_dev(2, S.data_ptr(), D.data_ptr(), N.data_ptr(), 4, L.data_ptr(), T.data_ptr(), ld, stream=sh)
+    t.cuda.synchronize()
+    assert gpu.lib().moty_cuda_kernel_status(0, sh) == (0 if len(sound) == 2 else -6)
+    want, wl = before.copy(), ln.copy()
+    for f in sound:
+        tail = lens[f] % 64 > 0
+        table[2 + f] = table[f]; wl[2 + f] = lens[f]
+        if tail:
+            want[new[f]] = before[table[f, lens[f] // 64]]; table[2 + f, lens[f] // 64] = new[f]
+    assert np.array_equal(mem.cpu().numpy(), want) and np.array_equal(T.cpu().numpy(), table) and np.array_equal(L.cpu().numpy(), wl)
