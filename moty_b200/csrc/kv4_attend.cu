@@ -687,7 +687,7 @@ Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     p.decode = cols <= (NG == 3 || NG == 4 ? 48 : 64);
     const long long seen = a.window > 0 && a.window + 2LL * KV4_PAGE < a.max_len ? a.window + 2LL * KV4_PAGE : a.max_len;
     const long long pages64 = (long long)a.b.nseq * a.geo.KV * ((cols + 63) / 64) * ((seen + KV4_PAGE - 1) / KV4_PAGE);
-    p.tc = cols > KV4_LINES && NG >= 2 && NG <= 4 && pages64 > 6LL * sms;
+    p.tc = a.tc && cols > KV4_LINES && NG >= 2 && NG <= 4 && pages64 > 6LL * sms;
     p.cols = p.tc ? KV4_TC_LINES : !p.decode ? KV4_LINES : cols > 4 ? 8 : 4;
     p.ntile = (int)((cols + p.cols - 1) / p.cols);
     if (p.ntile < 1) p.ntile = 1;

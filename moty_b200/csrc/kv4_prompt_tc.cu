@@ -582,20 +582,24 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
     }
 }
 
+// The roles' register shares (setmaxnreg) must add up to what the threads are launched with, which the compiler decides: where
+// it gave another number the other prompt kernel serves the call.  Looked at once a device.
+template <int NG> bool ready() {
+    static signed char state[MOTY_MAX_DEV];                  // 0: not looked at yet, 1: yes, -1: no
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MOTY_MAX_DEV) { cudaGetLastError(); return false; }
+    if (!state[dev]) {
+        cudaFuncAttributes fa;
+        const bool ok = cudaFuncGetAttributes(&fa, kv4_prompt_tc_kernel<NG>) == cudaSuccess && fa.numRegs == PT_REGS &&
+                        cudaFuncSetAttribute(kv4_prompt_tc_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PtL<NG>::SMEM) == cudaSuccess;
+        if (!ok) cudaGetLastError();
+        state[dev] = ok ? 1 : -1;
+    }
+    return state[dev] > 0;
+}
+
 template <int NG>
 int go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *err_wait, cudaStream_t st) {
-    static bool attr[MOTY_MAX_DEV];
-    int dev = 0;
-    CK(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= MOTY_MAX_DEV) return moty_set_error(MOTY_CUDA_EARG, "kv4_attend: device %d", dev);
-    if (!attr[dev]) {
-        CK(cudaFuncSetAttribute(kv4_prompt_tc_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PtL<NG>::SMEM));
-        // the register shares of the roles (setmaxnreg) add up to what the threads are launched with
-        cudaFuncAttributes fa;
-        CK(cudaFuncGetAttributes(&fa, kv4_prompt_tc_kernel<NG>));
-        if (fa.numRegs != PT_REGS) return moty_set_error(MOTY_CUDA_ECUDA, "kv4_attend: prompt kernel built with %d registers, not %d", fa.numRegs, PT_REGS);
-        attr[dev] = true;
-    }
     const long long grid = (long long)a.b.nseq * a.geo.KV * p.ntile * p.nsplit;
     if (grid > 0x7fffffffLL) return moty_set_error(MOTY_CUDA_ELIMIT, "kv4_attend: %lld CTAs", grid);
     CK(moty_launch_pdl(kv4_prompt_tc_kernel<NG>, dim3((unsigned)grid), dim3(PT_T), (size_t)PtL<NG>::SMEM, st, a, p.ntile, p.nsplit, p.span, part, err_wait));
@@ -603,6 +607,8 @@ int go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *err_wait, cudaStr
 }
 
 }  // namespace
+
+bool kv4_prompt_tc_ready(int hd) { return hd == 64 ? ready<2>() : hd == 96 ? ready<3>() : hd == 128 ? ready<4>() : false; }
 
 int launch_kv4_prompt_tc(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st) {
     int *err_wait = a.err - 4;                               // the library's error words: [0] tensor-core pipeline waits, [4] this cache's batches

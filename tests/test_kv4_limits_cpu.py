@@ -43,3 +43,38 @@ def test_rows_behind_a_refused_sequence_are_nobodys(tmp_path):
     assert look([0, 2, 5], [129, 9], 8) == [bad] * 2 + [ok] * 3 + [none] * 3
     assert look([1, 3, 2], [9, 9], 5) == [none, ok, ok, stray, stray]              # the second ends before it begins
     assert look([0, 9], [20], 5) == [bad] * 5                                      # ends behind the buffers
+
+
+def test_prompts_fall_back_where_the_tensor_memory_kernel_cannot_run(tmp_path):
+    """How a call is cut when that kernel was built with other registers than its roles share out: the other prompt kernel's
+    tiles, for every call that would have gone to it."""
+    import moty_b200 as mb
+    src, exe = str(tmp_path / "p.cpp"), str(tmp_path / "p")
+    with open(src, "w") as f:
+        f.write(r'''
+#include "kv4_attend.cuh"
+#include <cstdio>
+int main() {
+    int seen = 0;
+    for (int hd : {32, 64, 96, 128, 160, 256})
+        for (int rows : {1, 20, 400, 4096})
+            for (int len : {4096, 40000}) {
+                Kv4Attend a{};
+                a.geo = Kv4Geom{1, 8, hd, 100}; a.b.nseq = 2; a.b.rows = 2 * rows; a.b.ld = 1000;
+                a.H = 32; a.G = 4; a.max_rows = rows; a.max_len = len;
+                a.tc = true;
+                const Kv4Plan p = kv4_plan(a, 148);
+                a.tc = false;
+                const Kv4Plan q = kv4_plan(a, 148);
+                seen += p.tc;
+                if (q.tc || q.decode != p.decode || q.span % KV4_PAGE || (long long)q.span * q.nsplit < len) return 1;
+                if (p.tc ? q.cols != KV4_LINES || (long long)q.ntile * KV4_LINES < 4LL * rows
+                         : q.cols != p.cols || q.ntile != p.ntile || q.span != p.span || q.nsplit != p.nsplit) return 2;
+            }
+    printf("%d\n", seen);
+    return 0;
+}
+''')
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", CSRC, "-I", os.path.join(ROOT, "include"), "-I", "/usr/local/cuda/include", src, mb.LIB_PATH,
+                    "-L/usr/local/cuda/lib64", "-lcudart", "-Wl,-rpath," + os.path.dirname(mb.LIB_PATH), "-o", exe], check=True)
+    assert int(subprocess.run([exe], check=True, capture_output=True, text=True).stdout) >= 6
