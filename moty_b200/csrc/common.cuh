@@ -81,20 +81,19 @@ struct DevCtx {
     unsigned long long gen = 0;
 };
 
-// Every entry point that makes a GPU current puts the caller's device back before it returns.
+// Every entry point that makes a GPU current puts the caller's device back before it returns.  cudaSetDevice is called where the
+// device is current already, too: the thread's context may be one that the driver API made, and the library's streams and
+// memory live in the primary one.
 struct MotyDevGuard {
     int prev = -1;
-    bool moved = false;
     cudaError_t set(int device) {
         if (prev < 0) {
             cudaError_t e = cudaGetDevice(&prev);
             if (e != cudaSuccess) { prev = -1; return e; }
         }
-        if (device == prev && !moved) return cudaSuccess;
-        moved = true;
         return cudaSetDevice(device);
     }
-    ~MotyDevGuard() { if (moved) cudaSetDevice(prev); }
+    ~MotyDevGuard() { if (prev >= 0) cudaSetDevice(prev); }
 };
 #define MOTY_CAT2(a, b) a##b
 #define MOTY_CAT(a, b) MOTY_CAT2(a, b)

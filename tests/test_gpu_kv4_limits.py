@@ -259,3 +259,37 @@ def test_forks_into_a_page_that_is_copied_are_refused(gpu, t, lens, new, sound):
         if tail:
             want[new[f]] = before[table[f, lens[f] // 64]]; table[2 + f, lens[f] // 64] = new[f]
     assert np.array_equal(mem.cpu().numpy(), want) and np.array_equal(T.cpu().numpy(), table) and np.array_equal(L.cpu().numpy(), wl)
+
+
+def test_calls_from_a_thread_with_a_context_of_the_driver_api(gpu, t):
+    """A thread whose current context on the device is not the primary one: the library's calls run in theirs all the same."""
+    import threading
+
+    p = Pool(gpu, t, 2, 64, [100], seed=3)
+    q = p.rng.standard_normal((1, 4, 64)).astype(np.float32)
+    want = p.attend(q, 4, [1])
+    b, qd, ctx = p.batch([1]), p.dev(q, np.float32), t.zeros((1, 256), device="cuda")
+    t.cuda.synchronize()
+    cu = C.CDLL("libcuda.so.1")
+    failed = []
+
+    def work():
+        try:
+            dev, own = C.c_int(), C.c_void_p()
+            assert cu.cuDeviceGet(C.byref(dev), 0) == 0 and cu.cuCtxCreate_v2(C.byref(own), 0, dev) == 0
+            try:
+                p.kv.attend_dev(0, ctx.data_ptr(), qd.data_ptr(), 4, b)            # (the library's own stream)
+                gpu.sync(0)
+                more = gpu.Kv4(1, 1, 32, 2)
+                more.close()
+            finally:
+                assert cu.cuCtxDestroy_v2(own) == 0
+        except BaseException as e:
+            failed.append(e)
+
+    th = threading.Thread(target=work)
+    th.start(); th.join()
+    assert not failed, failed
+    assert ctx.cpu().numpy().tobytes() == want.tobytes()
+    assert np.array_equal(p.attend(q, 4, [1]), want)
+    p.status()
