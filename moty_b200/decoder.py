@@ -10,6 +10,7 @@ entries it calls (``moty_cuda_mat_apply_dev``, ``moty_cuda_attn_core_dev``, ``mo
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -393,7 +394,8 @@ class PagedDecoder(DenseDecoder):
     only the attention core differs (append_rope + attend on the pages instead of ``Attn``).
 
     ``pages``: pages of 64 positions in the pool (all layers of a position lie in one page).  ``max_pages``: the most a
-    sequence may hold.  ``run`` raises when the pool is out of pages, and changes nothing then."""
+    sequence may hold.  A call that raises (the pool is out of pages, an allocation or a launch fails, a kernel reports an
+    error) leaves lengths, pages and books as they were."""
 
     def __init__(self, layers, head: Mat, final_norm, n_heads, n_kv_heads, head_dim, pages, max_seqs=64, max_pages=64, theta=1e6, eps=1e-6,
                  rot=None, device=0, max_S=64):
@@ -493,8 +495,9 @@ class PagedDecoder(DenseDecoder):
             if i.min() < 0 or i.max() >= self.head.O:
                 raise MotyCudaError(f"a token id outside the vocabulary of {self.head.O}")
 
-    def _reserve(self, sids, more):
-        """Pages for `more[i]` further positions of each sequence: all of them or none."""
+    @contextlib.contextmanager
+    def _taken(self, sids, more):
+        """Pages for `more[i]` further positions of each sequence: all of them or none, and none again where the block fails."""
         grow = []
         for s, n in zip(sids, more):
             have, want = -(-int(self.lens[s]) // Kv4.PAGE), -(-(int(self.lens[s]) + int(n)) // Kv4.PAGE)
@@ -505,6 +508,21 @@ class PagedDecoder(DenseDecoder):
         at = 0
         for s, g in zip(sids, grow):
             self.table[s, g] = ids[at:at + len(g)]; at += len(g)
+        try:
+            yield
+        except BaseException:
+            self._settle()
+            for s, g in zip(sids, grow):
+                self.table[s, g] = -1
+            self.kv.release(ids)
+            raise
+
+    def _settle(self):
+        """After a failure: what is still on its way is done with the pages before others get them."""
+        try:
+            self.stream.synchronize()
+        except Exception:
+            pass
 
     # -- steps ----------------------------------------------------------------------------------------------------------
     def run(self, batch, want_logits=False):
@@ -520,26 +538,29 @@ class PagedDecoder(DenseDecoder):
         self._check_tokens(toks)
         counts = [i.size for i in toks]
         S, n = sum(counts), len(sids)
-        self._reserve(sids, counts)
-        self._drop_graph()                       # a batch of another shape may grow the library's scratch
-        if S > self.cap:
-            self._alloc(S)
-        self.lens[sids] += np.array(counts, np.int32)
-        row0 = np.concatenate([[0], np.cumsum(counts)])
-        with t.cuda.stream(self.stream):
-            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
-            d_row0, d_len, d_tab = up(row0), up(self.lens[sids]), up(self.table[sids])
-            b = Kv4Batch(n, S, d_row0.data_ptr(), d_len.data_ptr(), d_tab.data_ptr(), self.max_pages, max_rows=max(counts),
-                         max_len=int(self.lens[sids].max()))
-            self.ids[:S].copy_(t.from_numpy(np.concatenate(toks)))
-            self._embed_rows(S)
-            self._layers_paged(S, b)
-            last = self.x[:S].index_select(0, (d_row0[1:] - 1).long())
-            logits = t.empty((n, self.head.O), device=self.dev, dtype=t.float32)
-            self._head(last, n, logits)
-            out = self.out_id[:n].cpu().numpy().copy()
-            self._check_kernels()
-            return (out, logits.cpu().numpy()) if want_logits else out
+        with self._taken(sids, counts):
+            self._drop_graph()                   # a batch of another shape may grow the library's scratch
+            if S > self.cap:
+                self._alloc(S)
+            lens = self.lens[sids] + np.array(counts, np.int32)
+            row0 = np.concatenate([[0], np.cumsum(counts)])
+            with t.cuda.stream(self.stream):
+                up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
+                d_row0, d_len, d_tab = up(row0), up(lens), up(self.table[sids])
+                b = Kv4Batch(n, S, d_row0.data_ptr(), d_len.data_ptr(), d_tab.data_ptr(), self.max_pages, max_rows=max(counts),
+                             max_len=int(lens.max()))
+                self.ids[:S].copy_(t.from_numpy(np.concatenate(toks)))
+                self._embed_rows(S)
+                self._layers_paged(S, b)
+                last = self.x[:S].index_select(0, (d_row0[1:] - 1).long())
+                logits = t.empty((n, self.head.O), device=self.dev, dtype=t.float32)
+                self._head(last, n, logits)
+                out = self.out_id[:n].cpu().numpy().copy()
+                self._check_kernels()
+                if want_logits:
+                    logits = logits.cpu().numpy()
+            self.lens[sids] = lens               # nothing can fail from here on
+        return (out, logits) if want_logits else out
 
     def greedy(self, sids, tokens, n):
         """n greedy tokens for each of the sequences after ``tokens``, the step captured ONCE into a CUDA graph and replayed
@@ -555,50 +576,51 @@ class PagedDecoder(DenseDecoder):
         if tokens.size != k:
             raise MotyCudaError(f"{tokens.size} tokens for {k} sequences")
         self._check_tokens([tokens])
-        self._reserve(sids, [n] * k)
-        if k > self.cap:
-            self._alloc(k)
-        self._drop_graph()
-        start = self.lens[sids].copy()
-        with t.cuda.stream(self.stream):
-            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
-            row0, tab, lens = up(np.arange(k + 1)), up(self.table[sids]), up(start)
-            first = up(tokens)
-            hist, cnt = t.zeros((n + 1, k), device=self.dev, dtype=t.int32), t.zeros((1,), device=self.dev, dtype=t.int64)
-            logits = t.empty((k, self.head.O), device=self.dev, dtype=t.float32)
-            b = Kv4Batch(k, k, row0.data_ptr(), lens.data_ptr(), tab.data_ptr(), self.max_pages, max_rows=1, max_len=int(start.max()) + n)
-
-            def body():
-                lens.add_(1)
-                self._embed_rows(k)
-                self._layers_paged(k, b)
-                self._head(self.x[:k], k, logits)
-                self.ids[:k].copy_(self.out_id[:k])
-                hist.index_copy_(0, cnt, self.out_id[:k].view(1, k))
-                cnt.add_(1)
-
-            def reset():
-                self.ids[:k].copy_(first); lens.copy_(up(start)); cnt.zero_()
-
-            reset()
-            body()                               # one plain run: scratch, kernel attributes (its rows are written again below)
-        self.stream.synchronize()
-        _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 1))
-        try:
-            g = t.cuda.CUDAGraph()
-            with t.cuda.graph(g, stream=self.stream):
-                body()
+        with self._taken(sids, [n] * k):
+            if k > self.cap:
+                self._alloc(k)
+            self._drop_graph()
+            start = self.lens[sids].copy()
             with t.cuda.stream(self.stream):
+                up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
+                row0, tab, lens = up(np.arange(k + 1)), up(self.table[sids]), up(start)
+                first = up(tokens)
+                hist, cnt = t.zeros((n + 1, k), device=self.dev, dtype=t.int32), t.zeros((1,), device=self.dev, dtype=t.int64)
+                logits = t.empty((k, self.head.O), device=self.dev, dtype=t.float32)
+                b = Kv4Batch(k, k, row0.data_ptr(), lens.data_ptr(), tab.data_ptr(), self.max_pages, max_rows=1, max_len=int(start.max()) + n)
+
+                def body():
+                    lens.add_(1)
+                    self._embed_rows(k)
+                    self._layers_paged(k, b)
+                    self._head(self.x[:k], k, logits)
+                    self.ids[:k].copy_(self.out_id[:k])
+                    hist.index_copy_(0, cnt, self.out_id[:k].view(1, k))
+                    cnt.add_(1)
+
+                def reset():
+                    self.ids[:k].copy_(first); lens.copy_(up(start)); cnt.zero_()
+
                 reset()
-                for _ in range(n):
-                    g.replay()
+                body()                               # one plain run: scratch, kernel attributes (its rows are written again below)
             self.stream.synchronize()
-            self._check_kernels()
-            del g
-        finally:
-            _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 0))
-        self.lens[sids] += n
-        return hist[:n].cpu().numpy().T.copy()
+            _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 1))
+            try:
+                g = t.cuda.CUDAGraph()
+                with t.cuda.graph(g, stream=self.stream):
+                    body()
+                with t.cuda.stream(self.stream):
+                    reset()
+                    for _ in range(n):
+                        g.replay()
+                self.stream.synchronize()
+                self._check_kernels()
+                del g
+            finally:
+                _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 0))
+            out = hist[:n].cpu().numpy().T.copy()
+            self.lens[sids] += n                     # nothing can fail from here on
+        return out
 
     def _embed_rows(self, S):
         p = lambda ten: C.c_void_p(ten.data_ptr())

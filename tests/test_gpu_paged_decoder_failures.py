@@ -1,0 +1,67 @@
+"""GPU: PagedDecoder when a call fails on the host -- an allocation, a launch, the kernels' status -- and what forks share.  The
+failures are raised by the test in place of the real call; nothing faults on the GPU."""
+import numpy as np
+import pytest
+
+from test_gpu_paged_decoder import _model
+
+pytestmark = pytest.mark.gpu
+
+H, KV, HD, V = 4, 2, 32, 300
+
+
+def make(gpu, **kw):
+    from moty_b200.decoder import PagedDecoder
+    W, layers, head = _model(gpu, np.random.default_rng(4), H, KV, HD, 128, 256, V, 2, True)
+    return PagedDecoder(layers, head, W["final_norm"], H, KV, HD, **{**dict(pages=10, max_seqs=5, max_pages=4), **kw})
+
+
+def state(dec):
+    return dec.table.tolist(), dec.lens.tolist(), dec.used.tolist(), dec.kv.free_pages()
+
+
+class Failure(Exception):
+    pass
+
+
+def fail(*a, **k):
+    raise Failure
+
+
+def failing(monkeypatch, dec, what):
+    """`what` of the decoder raises: as a method, or (after:) once the real one has been called."""
+    if what.startswith("after:"):
+        name = what[6:]
+        real = getattr(dec, name)
+
+        def call(*a, **k):
+            real(*a, **k)
+            raise Failure
+        monkeypatch.setattr(dec, name, call)
+    else:
+        monkeypatch.setattr(dec, what, fail)
+
+
+@pytest.mark.parametrize("what", ["_embed_rows", "_layers_paged", "after:_layers_paged", "_head", "after:_head", "_check_kernels"])
+@pytest.mark.parametrize("call", ["run", "greedy"])
+def test_a_step_that_fails_changes_nothing(gpu, monkeypatch, call, what):
+    rng = np.random.default_rng(1)
+    prompt, more = rng.integers(0, V, 60), rng.integers(0, V, 80)
+    good = make(gpu)
+    a = good.new()
+    good.run([(a, prompt)])
+    want, want_lg = good.run([(a, more)], want_logits=True)
+    dec = make(gpu)
+    s, other = dec.new(), dec.new()
+    tok = dec.run([(s, prompt)])
+    dec.run([(other, prompt[:5])])
+    before = state(dec)
+    for _ in range(2):
+        with monkeypatch.context() as m:
+            failing(m, dec, what)
+            with pytest.raises(Failure):
+                dec.run([(s, more), (other, [1])]) if call == "run" else dec.greedy([s, other], [int(tok[0]), 1], 70)
+        assert state(dec) == before
+    out, lg = dec.run([(s, more)], want_logits=True)
+    assert out[0] == want[0] and np.array_equal(lg, want_lg)
+    good.close(); dec.close()
