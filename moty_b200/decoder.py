@@ -457,17 +457,22 @@ class PagedDecoder(DenseDecoder):
         if free.size < n:
             raise MotyCudaError(f"{n} forks, {free.size} sequences free")
         fresh = self.kv.alloc(n) if L % Kv4.PAGE else np.full(n, -1, np.int32)
-        for _ in range(n):
-            self.kv.retain(self.table[sid, :full])
         t = self.torch
-        with t.cuda.stream(self.stream):
-            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
-            table, lens = up(self.table), up(self.lens)
-            src, dst, new = up(np.full(n, sid)), up(free), up(fresh)
-            self.kv.fork_dev(n, src.data_ptr(), dst.data_ptr(), new.data_ptr(), self.max_seqs, lens.data_ptr(), table.data_ptr(),
-                             self.max_pages, stream=stream_handle(self.stream))
-            self.table, self.lens = table.cpu().numpy(), lens.cpu().numpy()
-            self._check_kernels()
+        try:
+            with t.cuda.stream(self.stream):
+                up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
+                table, lens = up(self.table), up(self.lens)
+                src, dst, new = up(np.full(n, sid)), up(free), up(fresh)
+                self.kv.fork_dev(n, src.data_ptr(), dst.data_ptr(), new.data_ptr(), self.max_seqs, lens.data_ptr(), table.data_ptr(),
+                                 self.max_pages, stream=stream_handle(self.stream))
+                table, lens = table.cpu().numpy(), lens.cpu().numpy()
+                self._check_kernels()
+            self.kv.retain(np.tile(self.table[sid, :full], n))       # all or none
+        except BaseException:
+            self._settle()
+            self.kv.release(fresh)
+            raise
+        self.table, self.lens = table, lens
         self.used[free] = True
         return [int(s) for s in free]
 

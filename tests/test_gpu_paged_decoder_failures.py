@@ -65,3 +65,27 @@ def test_a_step_that_fails_changes_nothing(gpu, monkeypatch, call, what):
     out, lg = dec.run([(s, more)], want_logits=True)
     assert out[0] == want[0] and np.array_equal(lg, want_lg)
     good.close(); dec.close()
+
+
+@pytest.mark.parametrize("tokens", [70, 64])                 # with a partial last page and without
+@pytest.mark.parametrize("what", ["fork_dev", "retain", "_check_kernels"])
+def test_a_fork_that_fails_changes_nothing(gpu, monkeypatch, what, tokens):
+    dec = make(gpu)
+    s = dec.new()
+    dec.run([(s, np.arange(tokens))])
+    before = state(dec)
+    for _ in range(2):
+        with monkeypatch.context() as m:
+            m.setattr(dec if what == "_check_kernels" else dec.kv, what, fail)
+            with pytest.raises(Failure):
+                dec.fork(s, 2)
+        assert state(dec) == before
+    assert dec.new() == 1                                    # a sequence of nothing, as before
+    dec.end(1)
+    f = dec.fork(s, 2)
+    out, lg = dec.run([(x, [7]) for x in [s] + f], want_logits=True)
+    assert np.array_equal(lg[0], lg[1]) and np.array_equal(lg[0], lg[2])
+    for x in [s] + f:
+        dec.end(x)
+    assert dec.kv.free_pages() == 10
+    dec.close()
