@@ -395,7 +395,7 @@ class PagedDecoder(DenseDecoder):
 
     ``pages``: pages of 64 positions in the pool (all layers of a position lie in one page).  ``max_pages``: the most a
     sequence may hold.  A call that raises (the pool is out of pages, an allocation or a launch fails, a kernel reports an
-    error) leaves lengths, pages and books as they were."""
+    error) leaves lengths, pages and books as they were (``compact`` says what happens there)."""
 
     def __init__(self, layers, head: Mat, final_norm, n_heads, n_kv_heads, head_dim, pages, max_seqs=64, max_pages=64, theta=1e6, eps=1e-6,
                  rot=None, device=0, max_S=64):
@@ -415,6 +415,7 @@ class PagedDecoder(DenseDecoder):
         self.table = np.full((max_seqs, max_pages), -1, np.int32)        # row = sequence id
         self.lens = np.zeros(max_seqs, np.int32)
         self.used = np.zeros(max_seqs, bool)
+        self._broken = False
         self.stream = torch.cuda.Stream(device=self.dev)
         self._alloc(max_S)
 
@@ -433,6 +434,7 @@ class PagedDecoder(DenseDecoder):
     # -- sequences ------------------------------------------------------------------------------------------------------
     def new(self) -> int:
         """An empty sequence; returns its id."""
+        self._usable()
         free = np.flatnonzero(~self.used)
         if not free.size:
             raise MotyCudaError(f"all {self.max_seqs} sequences are in use")
@@ -477,21 +479,36 @@ class PagedDecoder(DenseDecoder):
         return [int(s) for s in free]
 
     def compact(self) -> int:
-        """Move the pages in use to the lowest ids; returns how many moved."""
+        """Move the pages in use to the lowest ids; returns how many moved.  Should the moves themselves fail, the books already
+        name the new places: the decoder refuses every further call then."""
+        self._usable()
         self._drop_graph()
-        src, dst = self.kv.compact_plan()
-        if not src.size:
-            return 0
         t = self.torch
-        with t.cuda.stream(self.stream):
-            up = lambda a: t.from_numpy(np.ascontiguousarray(a, np.int32)).to(self.dev)
-            table, s, d = up(self.table), up(src), up(dst)
-            self.kv.compact_dev(src.size, s.data_ptr(), d.data_ptr(), table.numel(), table.data_ptr(), table.data_ptr(), stream=stream_handle(self.stream))
-            self.table = table.cpu().numpy()
-            self._check_kernels()
-        return int(src.size)
+        with t.cuda.stream(self.stream):         # what can fail for want of memory comes before the books change
+            table = t.from_numpy(self.table).to(self.dev)
+            moves = t.empty((2, self.kv.pages), device=self.dev, dtype=t.int32)
+            src, dst = self.kv.compact_plan()
+            n = int(src.size)
+            if not n:
+                return 0
+            try:
+                moves[0, :n].copy_(t.from_numpy(src)); moves[1, :n].copy_(t.from_numpy(dst))
+                self.kv.compact_dev(n, moves[0].data_ptr(), moves[1].data_ptr(), table.numel(), table.data_ptr(), table.data_ptr(),
+                                    stream=stream_handle(self.stream))
+                table = table.cpu().numpy()
+                self._check_kernels()
+            except BaseException:
+                self._broken = True
+                raise
+        self.table = table
+        return n
+
+    def _usable(self):
+        if self._broken:
+            raise MotyCudaError("a compaction failed: the pages no longer fit the sequences")
 
     def _check(self, sid):
+        self._usable()
         if not (0 <= sid < self.max_seqs and self.used[sid]):
             raise MotyCudaError(f"sequence {sid} is not in use")
 

@@ -89,3 +89,35 @@ def test_a_fork_that_fails_changes_nothing(gpu, monkeypatch, what, tokens):
         dec.end(x)
     assert dec.kv.free_pages() == 10
     dec.close()
+
+
+@pytest.mark.parametrize("what", ["to", "plan", "move", "_check_kernels"])
+def test_a_compaction_that_fails(gpu, monkeypatch, what):
+    """For want of memory, or of a plan: nothing has changed, and it can be asked again.  In the moves: every call is refused."""
+    dec = make(gpu)
+    a, b = dec.new(), dec.new()
+    dec.run([(a, np.arange(70)), (b, np.arange(100))])
+    dec.end(a)
+    before = state(dec)
+    with monkeypatch.context() as m:
+        if what == "to":
+            m.setattr(dec, "dev", "nowhere")                 # (no tensor can be made there)
+        elif what == "_check_kernels":
+            m.setattr(dec, what, fail)
+        else:
+            m.setattr(dec.kv, {"plan": "compact_plan", "move": "compact_dev"}[what], fail)
+        with pytest.raises((Failure, RuntimeError)):
+            dec.compact()
+    assert state(dec)[1:] == before[1:]
+    if what in ("to", "plan"):
+        assert dec.table.tolist() == before[0]
+        want = make(gpu)
+        x = want.new(); want.run([(x, np.arange(100))])
+        assert dec.compact() > 0 and sorted(dec.table[dec.table >= 0].tolist()) == [0, 1]
+        assert np.array_equal(dec.run([(b, [3])], want_logits=True)[1], want.run([(x, [3])], want_logits=True)[1])
+        want.close()
+    else:
+        for call in (lambda: dec.run([(b, [3])]), lambda: dec.fork(b), lambda: dec.greedy([b], [3], 2), lambda: dec.end(b), dec.new, dec.compact):
+            with pytest.raises(gpu.MotyCudaError, match="compaction"):
+                call()
+    dec.close()
