@@ -68,7 +68,7 @@ class DenseDecoder:
         qw, kw = self.H * self.hd, self.KV * self.hd
         e = lambda *shape: t.empty(shape, device=dev, dtype=t.float32)
         self._drop_graph()                       # a captured step holds the addresses of the buffers replaced below
-        self.cap = S
+        self.cap = 0                             # until all of them are there: a failed allocation must not leave small ones for S rows
         self.x, self.nrm, self.tmp = e(S, self.D), e(S, self.D), e(S, self.D)
         self.x_alt = e(1, self.D)
         self.qb, self.kb, self.vb, self.ctx = e(S, qw), e(S, kw), e(S, kw), e(S, qw)
@@ -76,6 +76,7 @@ class DenseDecoder:
         self.ids = t.empty((S,), device=dev, dtype=t.int32)
         self.out_id = t.empty((1,), device=dev, dtype=t.int32)
         self.logits = e(1, self.head.O)
+        self.cap = S
 
     def _drop_graph(self):
         """Forget the captured decode step and let the library's scratch grow again."""
@@ -281,7 +282,7 @@ class GemmaDecoder(DenseDecoder):
         t, dev = self.torch, self.dev
         e = lambda *shape: t.empty(shape, device=dev, dtype=t.float32)
         self._drop_graph()
-        self.cap = S
+        self.cap = 0                             # until all of them are there: a failed allocation must not leave small ones for S rows
         self.x, self.nrm, self.tmp = e(S, self.D), e(S, self.D), e(S, self.D)
         self.x_alt = e(1, self.D)
         self.qb, self.kb, self.vb, self.ctx = e(S, self._qw), e(S, self._kw), e(S, self._kw), e(S, self._qw)
@@ -289,6 +290,7 @@ class GemmaDecoder(DenseDecoder):
         self.ids = t.empty((S,), device=dev, dtype=t.int32)
         self.out_id = t.empty((1,), device=dev, dtype=t.int32)
         self.logits = e(1, self.head.O)
+        self.cap = S
 
     def _embed(self, S, sh):
         p = lambda ten: C.c_void_p(ten.data_ptr())
@@ -424,12 +426,13 @@ class PagedDecoder(DenseDecoder):
         qw, kw = self.H * self.hd, self.KV * self.hd
         e = lambda *shape: t.empty(shape, device=dev, dtype=t.float32)
         self._drop_graph()
-        self.cap = S
+        self.cap = 0                             # until all of them are there: a failed allocation must not leave small ones for S rows
         self.x, self.nrm, self.tmp, self.ctx = e(S, self.D), e(S, self.D), e(S, self.D), e(S, qw)
         self.qkvb = e(S, qw + 2 * kw)
         self.ids = t.empty((S,), device=dev, dtype=t.int32)
         self.out_id = t.empty((S,), device=dev, dtype=t.int32)
         self.logits = None
+        self.cap = S
 
     # -- sequences ------------------------------------------------------------------------------------------------------
     def new(self) -> int:

@@ -78,3 +78,35 @@ int main() {
     subprocess.run(["g++", "-O1", "-std=c++17", "-I", CSRC, "-I", os.path.join(ROOT, "include"), "-I", "/usr/local/cuda/include", src, mb.LIB_PATH,
                     "-L/usr/local/cuda/lib64", "-lcudart", "-Wl,-rpath," + os.path.dirname(mb.LIB_PATH), "-o", exe], check=True)
     assert int(subprocess.run([exe], check=True, capture_output=True, text=True).stdout) >= 6
+
+
+@pytest.mark.parametrize("name", ["DenseDecoder", "GemmaDecoder", "PagedDecoder"])
+def test_an_allocation_that_fails_leaves_no_room_behind(name):
+    """Buffers for more rows that could not all be made: the decoder must not take the smaller ones that are left for them."""
+    import types
+
+    import torch
+    from moty_b200 import decoder
+    d = object.__new__(getattr(decoder, name))
+    d.H, d.KV, d.hd, d.D, d._qw, d._kw = 4, 2, 32, 128, 128, 64
+    d.head = types.SimpleNamespace(O=300)
+    d.dev, left = "cpu", [99]
+
+    def empty(*a, **k):
+        left[0] -= 1
+        if left[0] < 0:
+            raise MemoryError
+        return torch.empty(*a, **k)
+
+    d.torch = types.SimpleNamespace(empty=empty, float32=torch.float32, int32=torch.int32)
+    d._alloc(4)
+    made = 99 - left[0]
+    assert d.cap == 4
+    for n in range(made):
+        left[0] = n
+        with pytest.raises(MemoryError):
+            d._alloc(50)
+        assert d.cap <= min(len(d.x), len(d.ctx), len(d.ids), len(d.nrm), len(d.tmp))
+        left[0] = 99
+        d._alloc(4)
+        assert d.cap == 4
