@@ -121,3 +121,41 @@ def test_a_compaction_that_fails(gpu, monkeypatch, what):
             with pytest.raises(gpu.MotyCudaError, match="compaction"):
                 call()
     dec.close()
+
+
+def held(gpu, dec, sid):
+    """The key and value rows that a sequence holds, every layer."""
+    import torch
+    n = int(dec.lens[sid])
+    d = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")
+    row0, ln, tab = d([0, n]), d([n]), d(dec.table[sid])
+    b = gpu.Kv4Batch(1, n, row0.data_ptr(), ln.data_ptr(), tab.data_ptr(), dec.max_pages)
+    out = []
+    for layer in range(len(dec.layers)):
+        k, v = (torch.full((n, KV * HD), 9.0, device="cuda") for _ in range(2))
+        dec.kv.fetch_dev(layer, k.data_ptr(), v.data_ptr(), b, stream=gpu.stream_handle(torch.cuda.current_stream()))
+        out.append(np.stack([k.cpu().numpy(), v.cpu().numpy()]))
+    return np.stack(out)
+
+
+@pytest.mark.parametrize("tokens", [70, 64])
+def test_what_forks_append_is_their_own(gpu, tokens):
+    """Forks that go on differently: full pages shared, last pages each one's own, and every sequence's earlier rows byte for byte
+    what they were."""
+    dec = make(gpu)
+    s = dec.new()
+    dec.run([(s, np.arange(tokens) * 3 % V)])
+    before = held(gpu, dec, s)
+    forks = dec.fork(s, 2)
+    for step in range(3):
+        dec.run([(x, [(50 * i + step) % V]) for i, x in enumerate([s] + forks)])
+    full = tokens // 64
+    last = [int(dec.table[x, full]) for x in [s] + forks]
+    assert len(set(last)) == 3 and min(last) >= 0
+    for x in forks:
+        assert dec.table[x, :full].tolist() == dec.table[s, :full].tolist()
+    rows = [held(gpu, dec, x) for x in [s] + forks]
+    for r in rows:
+        assert r[:, :, :tokens].tobytes() == before.tobytes()
+    assert not np.array_equal(rows[0][:, :, tokens:], rows[1][:, :, tokens:]) and not np.array_equal(rows[1][:, :, tokens:], rows[2][:, :, tokens:])
+    dec.close()
