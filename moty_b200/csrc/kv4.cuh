@@ -32,8 +32,8 @@ int launch_kv4_fetch(const Kv4Geom &geo, const uint8_t *mem, int layer, float *k
 // `span` positions
 struct Kv4Plan { bool decode, tc; int cols, ntile, nsplit, span; };
 Kv4Plan kv4_plan(const Kv4Attend &a, int sms);
-// kv4_prompt_tc.cu: whether that kernel was built with the registers that its roles share out (head width hd, current device)
-bool kv4_prompt_tc_ready(int hd);
+// kv4_prompt_tc.cu: whether that kernel was built with the registers that its roles share out (head width hd, the current device)
+bool kv4_prompt_tc_ready(int hd, int device);
 size_t kv4_attend_scratch_bytes(const Kv4Attend &a, const Kv4Plan &p);
 size_t kv4_attend_counters(const Kv4Attend &a, const Kv4Plan &p);
 int launch_kv4_attend(const Kv4Attend &a, const Kv4Plan &p, float *part, int *count, cudaStream_t st);

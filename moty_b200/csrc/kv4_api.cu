@@ -205,7 +205,7 @@ extern "C" int moty_cuda_kv4_attend_dev(MotyCudaKv4 *kv, int layer, float *ctx_d
     MOTY_USE_DEVICE(kv->device);
     a.H = n_heads; a.G = n_heads / kv->geo.KV; a.q = q_dev; a.ctx = ctx_dev; a.max_rows = batch->max_rows; a.max_len = batch->max_len;
     a.window = window; a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)kv->geo.hd); a.err = c->err_dev + 4;
-    a.tc = kv4_prompt_tc_ready(kv->geo.hd);
+    a.tc = kv4_prompt_tc_ready(kv->geo.hd, kv->device);
     const Kv4Plan p = kv4_plan(a, c->sms);
     const size_t sb = kv4_attend_scratch_bytes(a, p), nc = kv4_attend_counters(a, p) * 4;
     if (sb) CKR(moty_grow(c, &c->attn, sb));

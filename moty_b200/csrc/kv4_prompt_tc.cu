@@ -584,10 +584,9 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
 
 // The roles' register shares (setmaxnreg) must add up to what the threads are launched with, which the compiler decides: where
 // it gave another number the other prompt kernel serves the call.  Looked at once a device.
-template <int NG> bool ready() {
+template <int NG> bool ready(int dev) {
     static signed char state[MOTY_MAX_DEV];                  // 0: not looked at yet, 1: yes, -1: no
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MOTY_MAX_DEV) { cudaGetLastError(); return false; }
+    if (dev < 0 || dev >= MOTY_MAX_DEV) return false;
     if (!state[dev]) {
         cudaFuncAttributes fa;
         const bool ok = cudaFuncGetAttributes(&fa, kv4_prompt_tc_kernel<NG>) == cudaSuccess && fa.numRegs == PT_REGS &&
@@ -608,7 +607,7 @@ int go(const Kv4Attend &a, const Kv4Plan &p, float *part, int *err_wait, cudaStr
 
 }  // namespace
 
-bool kv4_prompt_tc_ready(int hd) { return hd == 64 ? ready<2>() : hd == 96 ? ready<3>() : hd == 128 ? ready<4>() : false; }
+bool kv4_prompt_tc_ready(int hd, int device) { return hd == 64 ? ready<2>(device) : hd == 96 ? ready<3>(device) : hd == 128 ? ready<4>(device) : false; }
 
 int launch_kv4_prompt_tc(const Kv4Attend &a, const Kv4Plan &p, float *part, cudaStream_t st) {
     int *err_wait = a.err - 4;                               // the library's error words: [0] tensor-core pipeline waits, [4] this cache's batches
