@@ -181,9 +181,15 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] = 0.f;
     // The matrix unit cuts its sums off, it does not round them, 1.6e-8 of a result a product: with 99 pages to a span and two
     // products a page results were 3.2e-6 off, with kv4_decode_long pages 0.6e-6 at most.  Of longer spans what acc holds is
-    // added to rounded sums every DEC_F pages.  These lie in local memory, and the code beside the loop costs 10 % (64
-    // sequences of up to 8192: 114 us), so shorter spans have a kernel without.
-    volatile float tot[LONG ? NG * 8 : 1];
+    // added to rounded sums every DEC_F pages.  These lie in local memory, with the reference and the steps' factor that they
+    // were left with, and the code beside the loop costs 10 % (64 sequences of up to 8192: 114 us), so shorter spans have a
+    // kernel without.
+    volatile float tot[LONG ? NG * 8 : 1], mt[NS];
+    volatile int dkt;
+    auto tot_factors = [&](float (&f)[NS]) {                 // what brings tot to the present ones
+#pragma unroll
+        for (int k = 0; k < NS; k++) f[k] = (mt[k] == m[k] ? 1.f : kv4_exp2(mt[k] - m[k])) * kv4_pow2(dk - dkt);
+    };
     int pages = 0;                                           // (tot holds nothing before DEC_F of them)
     for (int it = 0, slot = 0; it < np; it++) {
         cp_async_wait<DEC_ST - 2>();
@@ -279,9 +285,6 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                     for (int g = 0; g < NG; g++)
 #pragma unroll
                         for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] *= f;
-                    if (LONG && pages >= DEC_F)
-#pragma unroll
-                        for (int i = 0; i < NG * 8; i++) tot[LONG ? i : 0] *= f;
                 }
             }
         }
@@ -338,10 +341,6 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
                         acc[g][i >> 1][at] *= f;
                         if (PAIR) acc[g][i >> 1][at + 1] *= f;
                     }
-                if (LONG && pages >= DEC_F)
-#pragma unroll
-                    for (int i = 0; i < NG * 8; i++) if (PAIR || (i & 1) == k) tot[LONG ? i : 0] *= f;
-
             }
         }
         // scaled weights of positions 2 j, 2 j + 1, 2 j + 8, 2 j + 9 for column r
@@ -434,21 +433,34 @@ __global__ void __launch_bounds__(DEC_W * 32, DecL<NG, PAIR>::CTAS) kv4_decode_k
         else body(std::false_type{});
         if (LONG && ++pages % DEC_F == 0) {
             const bool first = pages == DEC_F;
+            float f[NS];
 #pragma unroll
-            for (int g = 0; g < NG; g++)
+            for (int k = 0; k < NS; k++) f[k] = 1.f;
+            if (!first) tot_factors(f);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {                   // (a group's loads together)
+                float old[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) old[i] = first ? 0.f : tot[LONG ? 8 * g + i : 0];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    volatile float &s = tot[LONG ? 8 * g + i : 0];
-                    s = first ? acc[g][i >> 2][i & 3] : s + acc[g][i >> 2][i & 3];
+                    tot[LONG ? 8 * g + i : 0] = fmaf(old[i], f[PAIR ? 0 : i & (NS - 1)], acc[g][i >> 2][i & 3]);
                     acc[g][i >> 2][i & 3] = 0.f;
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < NS; k++) mt[k] = m[k];
+            dkt = dk;
         }
     }
-    if (LONG && pages >= DEC_F)
+    if (LONG && pages >= DEC_F) {
+        float f[NS];
+        tot_factors(f);
 #pragma unroll
         for (int g = 0; g < NG; g++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] += tot[LONG ? 8 * g + i : 0];
+            for (int i = 0; i < 8; i++) acc[g][i >> 2][i & 3] = fmaf(tot[LONG ? 8 * g + i : 0], f[PAIR ? 0 : i & (NS - 1)], acc[g][i >> 2][i & 3]);
+    }
     // join the warps: a thread holds dims 32 g + 4 r + 0 .. 3 of its score columns
     cp_async_wait<0>();
     __syncthreads();
