@@ -679,13 +679,14 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
 
 // How a call is cut.  Host numbers only (the limits the caller gave), so a captured call stays valid for any batch within
 // them.  Which kernel, by (row, query head) pairs of a KV head ("columns"):
-//   decode, which re-reads the pages for every 8 columns, up to 64 of them, up to 48 where the tensor-memory kernel has the
-//     heads' width and their dims are many (8 sequences of 4096, 8 KV heads, hd 128: 72 us against 89 / 85 us of the prompt
-//     kernels at 48 columns, 107 against 92 / 87 us at 64; hd 64, 64 columns: 59 against 74 / 65 us; hd 256: 185 against
-//     179 us, and one sequence of 1024 16 against 31 us);
-//   tensor memory above 64 columns at hd 64, 96, 128 when there are more than six pages of 64 columns an SM: below that its
-//     set-up (13 us) is more than the matrix work it saves (one sequence of 1024, 8 KV heads, hd 128, 256 columns: 25 us
-//     against 20 us of the other; of 4096: 33 us against 51 us; 8 of 4096: 119 us against 327 us).
+//   decode, which re-reads the pages for every 8 columns, up to 48 of them (8 sequences of 4096, 4 KV heads, 48 columns: hd 128
+//     48 us against 51 us of the matrix-instruction prompt kernel, hd 64 30 against 33, hd 256 86 against 103); up to 64 at
+//     the narrowest and widest heads (56 columns: hd 32 31 against 38 us, hd 256 98 against 107; but
+//     hd 64 41 against 34, hd 128 60 against 52, hd 160 74 against 67), and where there are six pages of 64 columns an SM or
+//     fewer (one sequence of 1024, 56 columns: hd 64 9.3 against 10.8 us, hd 128 10.7 against 13.8, hd 160 11.9 against 17.1);
+//   tensor memory above 64 columns at hd 64, 96, 128 when there are more than those six pages: below that its set-up (13 us) is
+//     more than the matrix work it saves (one sequence of 1024, 8 KV heads, hd 128, 256 columns: 25 us against 21 us of
+//     the other; of 4096: 33 us against 52 us; 8 of 4096: 119 us against 336 us).
 // Spans of decode: with `units` (sequence, KV head, tile) triples of P pages on `slots` resident CTAs, a CTA costs its pages
 // plus about FIX pages' time of set-up and join.  When all CTAs are resident at once the longest one counts; otherwise the
 // total work over the slots plus a last CTA (lengths of a ragged batch are taken as 0.6 of the limit).  The cut with the
@@ -696,10 +697,11 @@ Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     Kv4Plan p{};
     const long long cols = (long long)a.max_rows * a.G;
     const int NG = a.geo.hd / 32;
-    p.decode = cols <= (NG == 3 || NG == 4 ? 48 : 64);
     const long long seen = a.window > 0 && a.window + 2LL * KV4_PAGE < a.max_len ? a.window + 2LL * KV4_PAGE : a.max_len;
     const long long pages64 = (long long)a.b.nseq * a.geo.KV * ((cols + 63) / 64) * ((seen + KV4_PAGE - 1) / KV4_PAGE);
-    p.tc = a.tc && cols > KV4_LINES && NG >= 2 && NG <= 4 && pages64 > 6LL * sms;
+    const bool many = pages64 > 6LL * sms;
+    p.decode = cols <= 48 || (cols <= 64 && (NG == 1 || NG >= 6 || !many));
+    p.tc = a.tc && cols > KV4_LINES && NG >= 2 && NG <= 4 && many;
     p.cols = p.tc ? KV4_TC_LINES : !p.decode ? KV4_LINES : cols > 4 ? 8 : 4;
     p.ntile = (int)((cols + p.cols - 1) / p.cols);
     if (p.ntile < 1) p.ntile = 1;
