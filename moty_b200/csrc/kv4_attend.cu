@@ -19,19 +19,21 @@ namespace {
 // thread, which adds them.  Otherwise eight columns, and hi and lo are two products into the same sums: the same matrix
 // work a column, half the piece arithmetic.  Every warp keeps its own exponent of the largest value step, and for each column a
 // reference that weights are scaled by: the first page's largest weight is 2^10 exactly (a row that sees one position is that
-// position's values exactly), and where that of a page leaves 2^6 .. 2^15 the reference is moved by a whole number of base-2
+// position's values, unless its score's own rounding shows), and where that of a page leaves 2^6 .. 2^15 the reference is moved by a whole number of base-2
 // units to put that one at 2^10, up or down (at 2^15 where others of the page lie 10 below it), for the lower piece
 // ends at 2^-24, and one position that holds nearly all the weight must not take the bits of those beside and after it (that
 // costs 2 %: 64 sequences of up to 8192 103.2 -> 105.5 us; a look at every column's largest on every page, and less
 // room above, 5 %).  Warps join in shared memory, spans
 // through `part` ({m, l, acc[hd]} per (row, head, split)): up to DEC_JOIN of them by the CTA of a tile that ends last
-// (1000 positions, 16 heads on 8: 6.8 us, with a second launch a microsecond more; 2 sequences of 8000 at hd 64, 17 to 32
+// (1000 positions, 16 heads on 8: 7 us, with a second launch a microsecond more; 2 sequences of 8000 at hd 64, 17 to 32
 // spans: 9.7 us, 13.3 us with a second launch), others by the merge kernels below.  A join is a chain of waits, so it asks
 // for the sums of its spans before it knows their weights (7.8 -> 6.8 us; one sequence of 131072 39.8 -> 33.7 us).
-// What bounds it: instructions.  A warp's 16 positions of 128 dims against 4 columns take about 400 (32 matrix products,
-// the rest unpacking codes, the two pieces of weight * step, softmax), issued in 68 of 100 cycles; memory is not the limit:
-// 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 103 us, 3.6 TB/s; one sequence of 131072, 32 heads on 4: 34 us;
-// 13 sequences, window 1024, hd 256: 17.7 us.  The steps measured at the first of these: codes straight from memory to
+// What bounds it: instructions and the waits between them.  A warp's 16 positions of 128 dims against 4 columns take about 400
+// (32 matrix products, the rest unpacking codes, the two pieces of weight * step, softmax), issued in 64 of 100 cycles by four
+// warps a scheduler (eight columns: 49 of 100 by three, whose registers leave no room for a fourth); memory is not the limit:
+// 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 105 us, 3.5 TB/s; one sequence of 131072, 32 heads on 4: 34.6
+// us; 13 sequences, window 1024, hd 256: 17.9 us.  Where pages' largest weights differ much the reference moves often: scores
+// of twice that spread (2.4 units) 112 and 37.7 us, of four times 120 and 39.0.  The steps measured at the first of these: codes straight from memory to
 // fragments 188 us, the ring 107 us, weight * step in f16 pairs and the joins in the launch 103 us.
 constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_F = 16;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, pages of a matrix unit's sum
 // exponents of a page's largest weight: the range it may have (DEC_LOW: where each four positions have one as large), where it is put, and how far below the highest reference so far one may be
@@ -690,9 +692,9 @@ __global__ void __launch_bounds__(MG_T) kv4_merge_kernel(Kv4Attend a, Kv4Plan pl
 // Spans of decode: with `units` (sequence, KV head, tile) triples of P pages on `slots` resident CTAs, a CTA costs its pages
 // plus about FIX pages' time of set-up and join.  When all CTAs are resident at once the longest one counts; otherwise the
 // total work over the slots plus a last CTA (lengths of a ragged batch are taken as 0.6 of the limit).  The cut with the
-// least of that (64 sequences of up to 8192 positions, 32 heads on 8: 103 us).  A prompt is cut only to fill the GPU: the
-// joins move rows x heads x hd x spans f32 values (4096 rows at 4096 positions, 16 heads: 174 us whole, 250 us in two spans;
-// nine ragged sequences of up to 333 rows and 2900 positions 105 us whole, 124 us in two).
+// least of that (64 sequences of up to 8192 positions, 32 heads on 8: 105 us).  A prompt is cut only to fill the GPU: the
+// joins move rows x heads x hd x spans f32 values (4096 rows at 4096 positions, 16 heads: 175 us whole, 250 us in two spans;
+// nine ragged sequences of up to 333 rows and 2900 positions 104 us whole, 124 us in two).
 Kv4Plan kv4_plan(const Kv4Attend &a, int sms) {
     Kv4Plan p{};
     const long long cols = (long long)a.max_rows * a.G;

@@ -2,8 +2,10 @@
 // from a unit of the paged 4-bit KV cache, and the two-piece form of its f32 operands.
 //
 // A code of -8 .. 7 is exact in f16.  The other operand (a query value, or a softmax weight times a value step) is f32: it
-// goes in as hi + lo, two f16 of 11 bits each, in neighbouring columns of the narrow operand, so that products and sums
-// are f32's own to within 2^-23 of each term.  Both are first scaled by a power of two so that hi fits and lo keeps its bits.
+// goes in as hi + lo, two f16 of 11 bits each, in neighbouring columns of the narrow operand: 2^-23 of a term, down to
+// the smallest f16, 2^-24, where lo ends.  Both are first scaled by a power of two so that hi fits and the terms that count lie
+// far above that end: a query row by its largest value (the end is 2^-38 of it), weights by the largest of a page and not of all
+// (each kernel says what its end is).
 #pragma once
 #include "kv4.cuh"
 

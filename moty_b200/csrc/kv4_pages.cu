@@ -1,8 +1,9 @@
 // kv4_pages.cu -- moves of whole pages of the paged 4-bit KV cache: forks (copy on write of the last partial page) and
 // compaction.  A page is contiguous over its layers and heads, so both are copies of long runs of bytes; each does its
 // table work in the same launch.  Bound by memory: a page of 28 layers, 8 KV heads, hd 128 is 2 MB; 180 of them moved 126 us
-// (743 MB read and written, 5.9 TB/s), 48 forks with partial pages 28 us (the bytes alone 26.5 us at the copy rate), four
-// forks 8 us (16 MB: one wave of loads, launch and table look-ups), five pages of 100 KB 3 us.  A page is cut into chunks of
+// (743 MB read and written, 5.9 TB/s), 48 forks with partial pages 29 us (the bytes alone 26.5 us at the copy rate), four
+// forks 8 us (16 MB, 2.5 us at the copy rate: launch, table look-ups, and a CTA's eight copies one after the other, for a load
+// is not moved over the store before it), five pages of 100 KB 3 us.  A page is cut into chunks of
 // about 32 KB, a CTA each, so that a few pages fill the GPU.
 #include "kv4.cuh"
 

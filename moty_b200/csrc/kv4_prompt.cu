@@ -12,8 +12,9 @@
 // largest value step so far and 2^9, then lies below 2^15, and its pieces end at 2^-28 of those two's product at worst.
 // It serves the head widths that the tensor-memory kernel has no operand tiles for, and calls too short for that kernel's
 // set-up.  What bounds it: two pieces make two matrix instructions of half the rate a product, and turning codes into
-// operands is done by every warp for itself; 4096 rows at 4096 positions, 16 heads on 8, hd 128: 573 us (tensor memory:
-// 174 us), one sequence of 1024, 64 rows, 32 heads on 8: 20 us (25 us).
+// operands is done by every warp for itself; 4096 rows at 4096 positions, 16 heads on 8, hd 128: 586 us (tensor memory:
+// 175 us), one sequence of 1024, 64 rows, 32 heads on 8: 21 us (25 us); 2048 rows, 16 heads on 4: hd 32 106 us, 160 213,
+// 192 248, 224 291, 256 334.
 #include "kv4_frag.cuh"
 #include "kv4_attend.cuh"
 

@@ -22,7 +22,7 @@
 // and two tiles take 3900 cycles of tensor core (scores 48 K-steps of 49 cycles, which reading both operands from shared
 // memory costs at N = 64, where the matrix unit alone would need 33; output 24 of 65), and a page takes 2.1 us where few SMs
 // work, 2.6 us where all do and the power limit lowers the clock.  Beside that a CTA spends 13 us: 8 on its query rows (13 from
-// memory), 2 on its first page, 3 on its results.  4096 rows at 4096 positions, 16 heads on 8: 174 us (41 us at the tensor peak for one product each, 124
+// memory), 2 on its first page, 3 on its results.  4096 rows at 4096 positions, 16 heads on 8: 175 us back to back, 195 us by itself (41 us at the tensor peak for one product each, 124
 // for three); one tile a CTA 416 us, when staging was longer than a tile's products; unrolled loops in the roles 227 us
 // (their code outgrew the instruction cache); division instead of a reciprocal for the results 3 us a CTA.
 // Every wait is bounded; on expiry all roles leave and the error word is set.
@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(PT_T, 1) kv4_prompt_tc_kernel(Kv4Attend a, int
                     // weights as hi and lo pairs of consecutive positions, over the scores: 16 columns become 8 of hi and 8 of
                     // lo.  They are brought up to 2^15 by the largest of the line on THIS page (lo ends at 2^-24, which
                     // then is 2^-39 of it), not by the largest so far, which one position may hold; bn takes it back.  Both are
-                    // a whole number of base-2 units apart: a line that sees one position is that position's values exactly.
+                    // a whole number of base-2 units apart: a line that sees one position is that position's values,
+                    // unless its score's own rounding shows.
                     const float mm = mx == -INFINITY ? 0.f : m + ceilf(mx - m) - 15.f, bn = mx == -INFINITY ? 0.f : kv4_exp2(mm - m);
                     float s0 = 0.f, s1 = 0.f;
 #pragma unroll 1
