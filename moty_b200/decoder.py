@@ -628,21 +628,19 @@ class PagedDecoder(DenseDecoder):
 
                 reset()
                 body()                               # one plain run: scratch, kernel attributes (its rows are written again below)
+            # (the scratch is neither frozen nor set free here: this graph does not outlive the call, and another decoder's captured
+            # step may be relying on the freeze that it took)
             self.stream.synchronize()
-            _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 1))
-            try:
-                g = t.cuda.CUDAGraph()
-                with t.cuda.graph(g, stream=self.stream):
-                    body()
-                with t.cuda.stream(self.stream):
-                    reset()
-                    for _ in range(n):
-                        g.replay()
-                self.stream.synchronize()
-                self._check_kernels()
-                del g
-            finally:
-                _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 0))
+            g = t.cuda.CUDAGraph()
+            with t.cuda.graph(g, stream=self.stream):
+                body()
+            with t.cuda.stream(self.stream):
+                reset()
+                for _ in range(n):
+                    g.replay()
+            self.stream.synchronize()
+            self._check_kernels()
+            del g
             out = hist[:n].cpu().numpy().T.copy()
             self.lens[sids] += n                     # nothing can fail from here on
         return out

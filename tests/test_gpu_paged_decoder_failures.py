@@ -159,3 +159,23 @@ def test_what_forks_append_is_their_own(gpu, tokens):
         assert r[:, :, :tokens].tobytes() == before.tobytes()
     assert not np.array_equal(rows[0][:, :, tokens:], rows[1][:, :, tokens:]) and not np.array_equal(rows[1][:, :, tokens:], rows[2][:, :, tokens:])
     dec.close()
+
+
+def test_greedy_leaves_the_scratch_frozen_for_others(gpu):
+    """A captured step of another decoder holds the library's scratch addresses: after a greedy call beside it the scratch still
+    does not move."""
+    L = gpu.lib()
+    dec = make(gpu)
+    s = dec.new()
+    tok = dec.run([(s, np.arange(70))])
+    dec.greedy([s], tok, 2)                                  # (the scratch it needs is there)
+    W = gpu.Mat.i8(np.zeros((64, 4096), np.int8), np.ones(64, np.float32))
+    gpu._ck(L.moty_cuda_scratch_freeze(0, 1))
+    try:
+        dec.greedy([s], [1], 2)
+        with pytest.raises(gpu.MotyCudaError, match="frozen"):
+            gpu.mat_apply(W, np.zeros((60000, 4096), np.float32))
+    finally:
+        gpu._ck(L.moty_cuda_scratch_freeze(0, 0))
+    dec.greedy([s], [1], 2)
+    dec.close()
