@@ -79,10 +79,18 @@ class DenseDecoder:
         self.cap = S
 
     def _drop_graph(self):
-        """Forget the captured decode step and let the library's scratch grow again."""
+        """Forget the captured decode step and, unless another decoder holds one, let the library's scratch grow again."""
         if getattr(self, "_graph", None) is not None:
             self._graph = None
-            _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 0))
+            self._hold_scratch(-1)
+
+    _holders = {}                                # device -> captured steps that hold the addresses of its scratch
+
+    def _hold_scratch(self, n):
+        d = self.dev.index or 0
+        held = self._holders[d] = self._holders.get(d, 0) + n
+        if held == (1 if n > 0 else 0):
+            _ck(lib().moty_cuda_scratch_freeze(d, int(n > 0)))
 
     def _check_kernels(self):
         """After a stream synchronisation: did a bounded wait inside a kernel run out (incomplete results)?"""
@@ -205,10 +213,14 @@ class DenseDecoder:
                 self._decode_body(C.c_void_p(stream_handle(self.stream)))
             self.stream.synchronize()
             # from here on the library's scratch may not move: the graph holds its addresses
-            _ck(lib().moty_cuda_scratch_freeze(self.dev.index or 0, 1))
-            g = t.cuda.CUDAGraph()
-            with t.cuda.graph(g, stream=self.stream):
-                self._decode_body(C.c_void_p(stream_handle(t.cuda.current_stream())))
+            self._hold_scratch(1)
+            try:
+                g = t.cuda.CUDAGraph()
+                with t.cuda.graph(g, stream=self.stream):
+                    self._decode_body(C.c_void_p(stream_handle(t.cuda.current_stream())))
+            except BaseException:
+                self._hold_scratch(-1)
+                raise
             self._graph = g
         with t.cuda.stream(self.stream):
             reset(first_tok, pos0)

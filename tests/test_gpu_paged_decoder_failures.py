@@ -179,3 +179,20 @@ def test_greedy_leaves_the_scratch_frozen_for_others(gpu):
         gpu._ck(L.moty_cuda_scratch_freeze(0, 0))
     dec.greedy([s], [1], 2)
     dec.close()
+
+
+def test_a_decoder_that_closes_leaves_the_scratch_frozen_for_others(gpu):
+    """Two decoders with captured steps: the scratch moves again when the last of them has let go."""
+    from moty_b200.decoder import DenseDecoder
+    W, layers, head = _model(gpu, np.random.default_rng(4), H, KV, HD, 128, 256, V, 2, True)
+    one, two = (DenseDecoder(layers, head, W["final_norm"], H, KV, HD, 64) for _ in range(2))
+    want = one.greedy_graph(3, 0, 4)
+    assert two.greedy_graph(3, 0, 4) == want
+    two.close()
+    big = gpu.Mat.i8(np.zeros((64, 4096), np.int8), np.ones(64, np.float32))
+    x = np.zeros((60000, 4096), np.float32)
+    with pytest.raises(gpu.MotyCudaError, match="frozen"):
+        gpu.mat_apply(big, x)
+    assert one.greedy_graph(3, 0, 4) == want
+    one.close()
+    assert DenseDecoder._holders[0] == 0
