@@ -13,7 +13,7 @@
 // It serves the head widths that the tensor-memory kernel has no operand tiles for, and calls too short for that kernel's
 // set-up.  What bounds it: two pieces make two matrix instructions of half the rate a product, and turning codes into
 // operands is done by every warp for itself; 4096 rows at 4096 positions, 16 heads on 8, hd 128: 586 us (tensor memory:
-// 175 us), one sequence of 1024, 64 rows, 32 heads on 8: 21 us (25 us); 2048 rows, 16 heads on 4: hd 32 106 us, 160 213,
+// 175 us), one sequence of 1024, 64 rows, 32 heads on 8: 21 us (25 us); 2048 rows, 16 heads on 4: hd 32 110 us, 160 213,
 // 192 248, 224 291, 256 334.
 #include "kv4_frag.cuh"
 #include "kv4_attend.cuh"
@@ -31,7 +31,7 @@ template <int NG> struct PrL {
 };
 
 template <int NG>
-__global__ void __launch_bounds__(PR_W * 32, NG == 1 ? 4 : 2) kv4_prompt_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
+__global__ void __launch_bounds__(PR_W * 32, NG == 1 ? 5 : 2) kv4_prompt_kernel(Kv4Attend a, int ntile, int nsplit, int span, float *part) {
     constexpr int HD = NG * 32, UNIT = PrL<NG>::UNIT, PT = PrL<NG>::PT, NL = 16 * PR_W;
     extern __shared__ __align__(128) uint8_t sm_kv4p[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, j = lane & 3;
