@@ -19,9 +19,9 @@ namespace {
 // thread, which adds them.  Otherwise eight columns, and hi and lo are two products into the same sums: the same matrix
 // work a column, half the piece arithmetic.  Every warp keeps its own exponent of the largest value step, and for each column a
 // reference that weights are scaled by: the first page's largest weight is 2^10 exactly (a row that sees one position is that
-// position's values, unless its score's own rounding shows), and where that of a page leaves 2^6 .. 2^15 the reference is moved by a whole number of base-2
-// units to put that one at 2^10, up or down (at 2^15 where others of the page lie 10 below it), for the lower piece
-// ends at 2^-24, and one position that holds nearly all the weight must not take the bits of those beside and after it (that
+// position's values, unless its score's own rounding shows), and where that of a page leaves 2^6 .. 2^15 the reference is
+// moved by a whole number of base-2 units to put that one at 2^10, up or down (at 2^15 where others of the page lie 10 below
+// it), for the lower piece ends at 2^-24, and one position that holds nearly all the weight must not take the bits of those beside and after it (that
 // costs 2 %: 64 sequences of up to 8192 103.2 -> 105.5 us; a look at every column's largest on every page, and less
 // room above, 5 %).  Warps join in shared memory, spans
 // through `part` ({m, l, acc[hd]} per (row, head, split)): up to DEC_JOIN of them by the CTA of a tile that ends last
@@ -33,10 +33,12 @@ namespace {
 // warps a scheduler (eight columns: 49 of 100 by three, whose registers leave no room for a fourth); memory is not the limit:
 // 64 sequences of up to 8192 positions, 32 heads on 8, 369 MB: 105 us, 3.5 TB/s; one sequence of 131072, 32 heads on 4: 34.6
 // us; 13 sequences, window 1024, hd 256: 17.9 us.  Where pages' largest weights differ much the reference moves often: scores
-// of twice that spread (2.4 units) 112 and 37.7 us, of four times 120 and 39.0.  The steps measured at the first of these: codes straight from memory to
+// of twice that spread (2.4 units) 112 and 37.7 us, of four times 120 and 39.0.  The steps measured at the first of these, which
+// are without all that: codes straight from memory to
 // fragments 188 us, the ring 107 us, weight * step in f16 pairs and the joins in the launch 103 us.
 constexpr int DEC_W = 4, DEC_NP = 256, DEC_JOIN = 32, DEC_F = 16;      // warps a CTA, the most pages of a span, the most spans joined in the launch itself, pages of a matrix unit's sum
-// exponents of a page's largest weight: the range it may have (DEC_LOW: where each four positions have one as large), where it is put, and how far below the highest reference so far one may be
+// exponents of a page's largest weight: the range it may have (DEC_LOW: where each four positions have one as large), where it is
+// put, and how far below the highest reference so far one may be
 constexpr float DEC_HI = 15.f, DEC_LO = 6.f, DEC_LOW = 4.f, DEC_AT = 10.f, DEC_DOWN = 60.f;
 
 // the most pages of a span whose sums stay in the matrix unit (one or two products a page)

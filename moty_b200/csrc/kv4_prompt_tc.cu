@@ -22,8 +22,8 @@
 // and two tiles take 3900 cycles of tensor core (scores 48 K-steps of 49 cycles, which reading both operands from shared
 // memory costs at N = 64, where the matrix unit alone would need 33; output 24 of 65), and a page takes 2.1 us where few SMs
 // work, 2.6 us where all do and the power limit lowers the clock.  Beside that a CTA spends 13 us: 8 on its query rows (13 from
-// memory), 2 on its first page, 3 on its results.  4096 rows at 4096 positions, 16 heads on 8: 175 us back to back, 195 us by itself (41 us at the tensor peak for one product each, 124
-// for three); one tile a CTA 416 us, when staging was longer than a tile's products; unrolled loops in the roles 227 us
+// memory), 2 on its first page, 3 on its results.  4096 rows at 4096 positions, 16 heads on 8: 175 us back to back, 195 us by
+// itself (41 us at the tensor peak for one product each, 124 for three); one tile a CTA 416 us, when staging was longer than a tile's products; unrolled loops in the roles 227 us
 // (their code outgrew the instruction cache); division instead of a reciprocal for the results 3 us a CTA.
 // Every wait is bounded; on expiry all roles leave and the error word is set.
 // An infinity or NaN of a key makes its scores NaN; a NaN step of a value is taken out of the product (a weight of 0 would

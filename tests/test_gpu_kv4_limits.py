@@ -106,8 +106,8 @@ def test_attend_prompts_with_long_sums_of_one_sign(gpu, t, H, KV, nseq, rows, hd
 
 @pytest.mark.parametrize("H,rows,hd", [(8, 1, 32), (8, 1, 96), (64, 1, 128), (16, 1, 256), (32, 20, 32), (32, 20, 64), (32, 20, 128), (32, 20, 256)])
 def test_attend_of_one_position_is_its_values(gpu, t, H, rows, hd):
-    """A row that sees a single position, of a score without rounding, is that position's value row, to the bit: the first positions of sequences, and rows
-    with a window of one.  (Activations are quantised after this: values of few bits lie on ties there.)  Scores are exact in
+    """A row that sees a single position, of a score without rounding, is that position's value row, to the bit: the first
+    positions of sequences, and rows with a window of one.  (Activations are quantised after this: values of few bits lie on ties there.)  Scores are exact in
     the kernels' base-2 units: eighths, scaled by what is 1 after log2(e)."""
     T, log2e = 150, np.float32(1.44269504)
     scale = np.float32(1) / log2e
